@@ -188,6 +188,122 @@ int xt_ipc_close(void* base);
 int xt_matmul_launch_noalloc(const xt_module* module, const char* func, void* const* args, int n_args,
                              int64_t bid0_begin, int64_t bid0_end, void* stream);
 
+/* ------------------------------------------------------- serving operators
+ * No counterpart in the reference.  The operators between the matmuls of a
+ * decoder layer when a model answers: the norm that makes int8 rows, rotary
+ * positions, an int8 paged cache with its attention, and int8 data read back.
+ * Arrays are device memory of XT_ELEM_* types; a row's (head's) elements are
+ * contiguous and strides are in elements.  Every call checks its arguments on
+ * the host, is asynchronous on ``stream``, and reads and writes each array
+ * once.  What only the device knows (positions, lengths, page tables) is
+ * checked there: an entry that names something outside the arrays is not
+ * followed, its results are NaN or left unwritten, and xt_device_error gives
+ * 0x301 (rope position), 0x302 (append) or 0x303 (attention). */
+
+/* y = h * rsqrt(mean(h^2) + eps) * weight with h = x + residual, row by row.
+ * y_elem XT_ELEM_I8: y = rint(v / s) with the row's s = max|v| / 127 in
+ * scales (v: the normed row; s is 0 for rows under 1e-36, NaN for rows with
+ * NaN).  Sums are f32; the norm is of h before it is rounded into sum. */
+typedef struct xt_rms_norm_args {
+  const void* x;         /* [rows, cols], elem */
+  const void* residual;  /* like x, or NULL */
+  const void* weight;    /* [cols], weight_elem */
+  void* y;               /* [rows, cols], y_elem */
+  void* sum;             /* h, like x, or NULL; may be x or residual */
+  float* scales;         /* [rows], for int8 rows; else NULL */
+  int64_t rows, cols;
+  int64_t x_stride, residual_stride, y_stride, sum_stride; /* between rows */
+  int elem, weight_elem; /* XT_ELEM_F32 or XT_ELEM_BF16 */
+  int y_elem;            /* XT_ELEM_F32, XT_ELEM_BF16 or XT_ELEM_I8 */
+  float eps;
+} xt_rms_norm_args;
+int xt_rms_norm(const xt_rms_norm_args* args, void* stream);
+
+/* Turns the pairs of the first ``rot`` elements of each head by the table's
+ * row of the token's position: (a, b) -> (a cos - b sin, a sin + b cos), pairs
+ * (2i, 2i+1) if interleaved, else (i, i + rot/2).  inverse turns back, which
+ * is also the gradient.  y may be x (same strides and type). */
+typedef struct xt_rope_args {
+  const void* x;            /* [tokens, heads, dim], elem */
+  void* y;                  /* likewise, y_elem */
+  const int32_t* positions; /* [tokens] */
+  const float* table;       /* [table_rows, rot / 2, 2] of cos, sin */
+  int64_t tokens, heads, dim, rot, table_rows;
+  int64_t x_token, x_head, y_token, y_head;
+  int elem, y_elem;         /* f32 -> f32 or bf16, bf16 -> bf16 */
+  int interleaved, inverse;
+} xt_rope_args;
+int xt_rope(const xt_rope_args* args, void* stream);
+
+/* A paged cache of int8 keys and values with an f32 scale for each ``block``
+ * tokens of a head: token value = int8 * scale. */
+typedef struct xt_cache {
+  int8_t* k;       /* [pages, heads, page, dim], 16-byte aligned; dim a multiple of 16 up to 256 */
+  int8_t* v;
+  float* k_scale;  /* [pages, heads, page / block] */
+  float* v_scale;
+  int64_t pages;
+  int heads, page, dim, block;
+} xt_cache;
+
+/* A ragged batch.  Sequence b has lengths[b] tokens; the last ones of them,
+ * rows starts[b] .. starts[b + 1] - 1 of the packed arrays, are new.  Token j
+ * of it lies in row j % page of page table[b * table_stride + j / page]. */
+typedef struct xt_batch {
+  const int32_t* starts;   /* [seqs + 1] */
+  const int32_t* lengths;  /* [seqs] */
+  const int32_t* table;    /* [seqs, table_width] */
+  int seqs, tokens;        /* tokens: rows of the packed arrays */
+  int table_width;
+  int64_t table_stride;
+} xt_batch;
+
+/* Writes the new tokens' keys and values into the cache; keys are turned as
+ * by xt_rope at their positions if ``rope`` is given.  A block's scale becomes
+ * the larger of what it was (if it holds earlier tokens of the sequence) and
+ * max|x| / 127 over its new tokens; where it rises, the earlier tokens' rows
+ * are rounded anew.  A NaN makes its block's scale NaN.  Blocks of one call
+ * must not be shared by two sequences. */
+typedef struct xt_cache_append_args {
+  xt_cache cache;
+  xt_batch batch;
+  const void* k;       /* [tokens, heads, dim], elem */
+  const void* v;
+  int64_t k_token, k_head, v_token, v_head;
+  const float* rope;   /* [rope_rows, rot / 2, 2], or NULL */
+  int64_t rot, rope_rows;
+  int elem;            /* XT_ELEM_F32 or XT_ELEM_BF16 */
+  int interleaved;
+} xt_cache_append_args;
+int xt_cache_append(const xt_cache_append_args* args, void* stream);
+
+/* Attention of each new token over its sequence's tokens up to itself (the
+ * last ``window`` of them if window > 0); q_heads is a multiple of the cache's
+ * heads, consecutive query heads share one.  softcap > 0 caps the scaled
+ * scores: cap * tanh(score / cap).  A row that sees no token is 0.  The
+ * workspace (xt_cache_attention_workspace bytes, 16-byte aligned) is scratch
+ * of this call alone until its stream has finished it. */
+typedef struct xt_cache_attention_args {
+  xt_cache cache;
+  xt_batch batch;
+  const void* q;       /* [tokens, q_heads, dim], elem; strides multiples of 4, 16-byte aligned (bf16: 8) */
+  void* out;           /* likewise */
+  int64_t q_token, q_head, out_token, out_head;
+  int q_heads;
+  int max_new;         /* most new tokens of one sequence, as far as known: a hint for the choice of kernel; 0: unknown */
+  int window;          /* 0: none */
+  float scale, softcap;
+  int elem;            /* XT_ELEM_F32 or XT_ELEM_BF16 */
+  void* workspace;
+  size_t workspace_bytes;
+} xt_cache_attention_args;
+int xt_cache_attention_workspace(const xt_cache_attention_args* args, size_t* out_bytes);
+int xt_cache_attention(const xt_cache_attention_args* args, void* stream);
+
+/* out[i] = q[i] * scales[i / run]: int8 data (rows, or a cache's blocks) back
+ * as f32 or bf16 values.  q and out are 16-byte aligned. */
+int xt_dequantize(const int8_t* q, const float* scales, void* out, int64_t n, int64_t run, int elem, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

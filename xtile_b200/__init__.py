@@ -57,13 +57,14 @@ from .api import (
     xt_to_nova,
 )
 from .runtime import PeerArray, device_error, export_array, launch, run, sm_budget, wait_limit
+from .serving import KVCache, RopeTable, cache_append, cache_attention, dequantize, rms_norm, rope
 
 __all__ = [
-    "Array", "DType", "Module", "PeerArray", "add", "astype", "bfloat16", "bid", "canonicalize", "cdiv", "compile",
-    "convert",
-    "cos", "device_error", "exp", "export_array", "float32", "int8", "kernel", "launch", "load", "load_conv2d",
+    "Array", "DType", "KVCache", "Module", "PeerArray", "RopeTable", "add", "astype", "bfloat16", "bid",
+    "cache_append", "cache_attention", "canonicalize", "cdiv", "compile", "convert",
+    "cos", "dequantize", "device_error", "exp", "export_array", "float32", "int8", "kernel", "launch", "load", "load_conv2d",
     "matmul", "max", "mma", "mul", "nova_allocate", "nova_barrier", "nova_optimize",
-    "nova_threading", "nova_to_x1", "parse", "reciprocal", "reshape", "rsqrt", "run",
+    "nova_threading", "nova_to_x1", "parse", "reciprocal", "reshape", "rms_norm", "rope", "rsqrt", "run",
     "save_compile_results", "save_ir", "sigmoid", "silu", "sin", "sm_budget", "store", "sub", "sum", "tanh",
     "transpose", "truediv", "wait_limit", "xt_serialize", "xt_to_nova",
 ]

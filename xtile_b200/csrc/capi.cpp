@@ -348,6 +348,17 @@ std::shared_ptr<Plan> module_plan(const xt_module* module, const char* func) {
 // Records ``msg`` as the calling thread's last error and returns ``code``.
 int record_error(int code, const std::string& msg) { return fail(code, msg); }
 
+// The current device's error word, which xt_device_error reads and clears.
+int device_error_word(uint32_t** out) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  Workspace* ws = nullptr;
+  if (e == cudaSuccess) e = workspace(device, &ws);
+  if (e != cudaSuccess) return cuda_fail(e, "workspace allocation");
+  *out = ws->error_word;
+  return XT_OK;
+}
+
 }  // namespace xt
 
 extern "C" {

@@ -1,0 +1,128 @@
+// 16-byte and single-element access to f32 and bf16 arrays as f32 values, and
+// the int8 rounding that the serving kernels share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace xt {
+namespace dev {
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Two f32 rounded to bf16 (to nearest even), ``lo`` in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// V consecutive elements as f32: 16-byte loads where V fills them, else one
+// element.  ``p`` is aligned to the access.
+template <class T, int V>
+struct Vec;
+
+template <>
+struct Vec<float, 4> {
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+};
+
+template <>
+struct Vec<__nv_bfloat16, 4> {
+  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[4]) {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_lo(t.x), v[1] = bf16_hi(t.x), v[2] = bf16_lo(t.y), v[3] = bf16_hi(t.y);
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[4]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+  }
+};
+
+template <>
+struct Vec<__nv_bfloat16, 8> {
+  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 t = *reinterpret_cast<const uint4*>(p);
+    v[0] = bf16_lo(t.x), v[1] = bf16_hi(t.x), v[2] = bf16_lo(t.y), v[3] = bf16_hi(t.y);
+    v[4] = bf16_lo(t.z), v[5] = bf16_hi(t.z), v[6] = bf16_lo(t.w), v[7] = bf16_hi(t.w);
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  }
+};
+
+template <>
+struct Vec<float, 8> {
+  static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
+
+template <>
+struct Vec<float, 1> {
+  static __device__ __forceinline__ void load(const float* p, float (&v)[1]) { v[0] = *p; }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[1]) { *p = v[0]; }
+};
+
+template <>
+struct Vec<__nv_bfloat16, 1> {
+  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[1]) { v[0] = __bfloat162float(*p); }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[1]) { *p = __float2bfloat16_rn(v[0]); }
+};
+
+// The larger of two values; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// int8 scale of values whose largest magnitude is ``top``: top / 127, and 0
+// (all values round to 0) for a top under 1e-36, whose reciprocal would leave
+// f32's range.  A NaN top gives a NaN scale, so that whoever reads the values
+// back sees it.
+constexpr float kQuantTiny = 1e-36f;
+__device__ __forceinline__ float quant_scale(float top) { return top < kQuantTiny ? 0.0f : top * (1.0f / 127.0f); }
+__device__ __forceinline__ float quant_inverse(float scale) { return scale > 0.0f ? 1.0f / scale : 0.0f; }
+
+// x times the inverse scale, rounded to the nearest whole number (ties to
+// even) within +-127; NaN gives 0.
+__device__ __forceinline__ int quantize(float x, float inverse) {
+  const int q = __float2int_rn(x * inverse);
+  return min(max(q, -127), 127);
+}
+
+__device__ __forceinline__ uint32_t pack_i8(int a, int b, int c, int d) {
+  return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
+}
+
+// V values as int8 at ``p`` (aligned to V bytes).
+template <int V>
+__device__ __forceinline__ void store_i8(int8_t* p, const float (&x)[V], float inverse) {
+  if constexpr (V == 8) {
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(pack_i8(quantize(x[0], inverse), quantize(x[1], inverse), quantize(x[2], inverse), quantize(x[3], inverse)),
+                   pack_i8(quantize(x[4], inverse), quantize(x[5], inverse), quantize(x[6], inverse), quantize(x[7], inverse)));
+  } else if constexpr (V == 4) {
+    *reinterpret_cast<uint32_t*>(p) =
+        pack_i8(quantize(x[0], inverse), quantize(x[1], inverse), quantize(x[2], inverse), quantize(x[3], inverse));
+  } else {
+    *p = static_cast<int8_t>(quantize(x[0], inverse));
+  }
+}
+
+}  // namespace dev
+}  // namespace xt
