@@ -2,7 +2,9 @@
 
 * ``libxt_b200.so``  -- the C ABI (include/xt_b200.h): parser, verifier,
   planner and the sm_100a kernels (nvcc, -gencode arch=compute_100a,code=sm_100a);
-* ``_xtile*.so``     -- the Python extension (pybind11) over that library.
+* ``_xtile*.so``     -- the Python extension (pybind11) over that library;
+* ``_serving*.so``   -- the serving operators on torch tensors, built against
+  torch's headers and loaded with torch at their first use.
 
 Objects go to ``xtile_b200/_build``; a source is recompiled when it or any
 header it can include is newer than its object.
@@ -34,6 +36,7 @@ def ext_suffix() -> str:
 
 
 EXT = PKG / f"_xtile{ext_suffix()}"
+SERVING_EXT = PKG / f"_serving{ext_suffix()}"
 
 
 def _headers() -> list[Path]:
@@ -81,14 +84,36 @@ def _embed_op_math() -> None:
         inc.write_text(body)
 
 
+def _torch_dir() -> Path:
+    import importlib.util
+
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("the serving extension is built against torch, which is not installed")
+    return Path(spec.submodule_search_locations[0])
+
+
+def _build_serving(force: bool, deps: list[Path]) -> bool:
+    """Compiles the serving extension's object; True if it is newer than the extension."""
+    src, obj = CSRC / "serving_module.cpp", BUILD / "serving_module.o"
+    torch = _torch_dir()
+    if force or _stale(obj, src, [d for d in deps if d.parent == ROOT / "include"]):
+        inc = torch / "include"
+        _run(["g++", "-O2", "-fPIC", "-std=c++20", f"-I{sysconfig.get_paths()['include']}", f"-I{inc}",
+              f"-I{inc / 'torch/csrc/api/include'}", f"-I{CUDA / 'include'}", "-c", str(src), "-o", str(obj)])
+    return not SERVING_EXT.exists() or obj.stat().st_mtime > SERVING_EXT.stat().st_mtime
+
+
 def build(force: bool = False, verbose: bool = False) -> None:
     BUILD.mkdir(exist_ok=True)
     _embed_op_math()
     deps = _headers()
-    lib_srcs = [p for p in sorted(CSRC.rglob("*.cpp")) if p.name != "xt_module.cpp"]
+    lib_srcs = [p for p in sorted(CSRC.rglob("*.cpp")) if p.name not in ("xt_module.cpp", "serving_module.cpp")]
     lib_srcs += sorted(CSRC.rglob("*.cu"))
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as pool:
+        serving = pool.submit(_build_serving, force, deps)
         objs = list(pool.map(lambda s: _compile(s, force, deps), lib_srcs))
+        link_serving = serving.result()
     if force or not LIB.exists() or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs):
         _run([NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objs), "-lcudart_static", "-ldl",
               "-lrt", "-lpthread"])
@@ -110,6 +135,13 @@ def build(force: bool = False, verbose: bool = False) -> None:
               "-Wl,-rpath,$ORIGIN"])
         if verbose:
             print("linked", EXT)
+    if force or link_serving or LIB.stat().st_mtime > SERVING_EXT.stat().st_mtime:
+        lib = _torch_dir() / "lib"
+        _run(["g++", "-shared", "-o", str(SERVING_EXT), str(BUILD / "serving_module.o"), f"-L{PKG}", "-lxt_b200",
+              f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN",
+              f"-Wl,-rpath,{lib}"])
+        if verbose:
+            print("linked", SERVING_EXT)
 
 
 def main() -> None:

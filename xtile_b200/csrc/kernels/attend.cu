@@ -28,6 +28,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../serve.h"
 #include "batch.cuh"
 #include "pdl.cuh"
@@ -727,11 +729,29 @@ int64_t worker_count(int sms) {
   return static_cast<int64_t>(sms) * S::kCtas * S::kWarps;
 }
 
+constexpr int kMaxDevices = 64;
+
 int sm_count() {
+  static std::atomic<int> known[kMaxDevices];
   int device = 0, sms = 148;
   cudaGetDevice(&device);
+  const bool keep = device >= 0 && device < kMaxDevices;
+  if (keep && known[device]) return known[device];
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (keep) known[device] = sms;
   return sms;
+}
+
+// Grants ``kernel`` its shared memory, once a device.
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[kMaxDevices]) {
+  int device = 0;
+  cudaGetDevice(&device);
+  const bool keep = device >= 0 && device < kMaxDevices;
+  if (keep && done[device]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && keep) done[device] = true;
+  return e;
 }
 
 template <int DP, bool F32>
@@ -744,7 +764,8 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream) {
   p.part_ml = reinterpret_cast<float2*>(p.part + p.workers * 2 * kTile * p.a.cache.dim);
   constexpr int kSmem = S::kWarps * S::kWarpBytes;
   static_assert(kSmem * S::kCtas <= 227 * 1024, "the CTAs of an SM share 227 KB");
-  cudaError_t e = cudaFuncSetAttribute(attend_units<DP, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<bool> allowed[kMaxDevices];
+  cudaError_t e = allow_smem(attend_units<DP, F32>, kSmem, allowed);
   if (e != cudaSuccess) return e;
   PdlLaunch launch(dim3(static_cast<unsigned>(sms * S::kCtas)), dim3(S::kWarps * 32), kSmem, stream);
   e = launch(attend_units<DP, F32>, p);

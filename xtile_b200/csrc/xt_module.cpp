@@ -164,17 +164,6 @@ uint32_t device_error() {
   return code;
 }
 
-void* ptr(uintptr_t p) { return reinterpret_cast<void*>(p); }
-
-void check(int status, const char* context) {
-  if (status != XT_OK) raise_status(status, context);
-}
-
-xt_batch batch(uintptr_t starts, uintptr_t lengths, uintptr_t table, int seqs, int tokens, int width, int64_t stride) {
-  return {reinterpret_cast<const int32_t*>(starts), reinterpret_cast<const int32_t*>(lengths),
-          reinterpret_cast<const int32_t*>(table), seqs, tokens, width, stride};
-}
-
 }  // namespace
 
 PYBIND11_MODULE(_xtile, m) {
@@ -264,67 +253,4 @@ PYBIND11_MODULE(_xtile, m) {
   m.def("func_names", &func_names, py::arg("module"));
   m.def("func_args", &func_args, py::arg("module"), py::arg("func") = py::none());
   m.def("device_error", &device_error);
-
-  // the serving operators: pointers and extents, checked by the C ABI
-  py::class_<xt_cache>(m, "CacheView")
-      .def(py::init([](uintptr_t k, uintptr_t v, uintptr_t k_scale, uintptr_t v_scale, int64_t pages, int heads, int page,
-                       int dim, int block) {
-        return xt_cache{reinterpret_cast<int8_t*>(k), reinterpret_cast<int8_t*>(v), reinterpret_cast<float*>(k_scale),
-                        reinterpret_cast<float*>(v_scale), pages, heads, page, dim, block};
-      }));
-  m.def("rms_norm", [](uintptr_t x, uintptr_t residual, uintptr_t weight, uintptr_t y, uintptr_t sum, uintptr_t scales,
-                       int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride, int64_t y_stride,
-                       int64_t sum_stride, int elem, int weight_elem, int y_elem, float eps, uintptr_t stream) {
-    const xt_rms_norm_args a{ptr(x), ptr(residual), ptr(weight), ptr(y), ptr(sum), reinterpret_cast<float*>(scales),
-                             rows, cols, x_stride, residual_stride, y_stride, sum_stride, elem, weight_elem, y_elem, eps};
-    check(xt_rms_norm(&a, ptr(stream)), "rms_norm");
-  });
-  m.def("rope", [](uintptr_t x, uintptr_t y, uintptr_t positions, uintptr_t table, int64_t tokens, int64_t heads,
-                   int64_t dim, int64_t rot, int64_t table_rows, int64_t x_token, int64_t x_head, int64_t y_token,
-                   int64_t y_head, int elem, int y_elem, bool interleaved, bool inverse, uintptr_t stream) {
-    const xt_rope_args a{ptr(x), ptr(y), reinterpret_cast<const int32_t*>(positions), reinterpret_cast<const float*>(table),
-                         tokens, heads, dim, rot, table_rows, x_token, x_head, y_token, y_head, elem, y_elem,
-                         interleaved, inverse};
-    check(xt_rope(&a, ptr(stream)), "rope");
-  });
-  m.def("cache_append", [](const xt_cache& cache, uintptr_t starts, uintptr_t lengths, uintptr_t table, int seqs,
-                           int tokens, int width, int64_t stride, uintptr_t k, uintptr_t v, int64_t k_token,
-                           int64_t k_head, int64_t v_token, int64_t v_head, uintptr_t rope, int64_t rot,
-                           int64_t rope_rows, int elem, bool interleaved, uintptr_t stream) {
-    const xt_cache_append_args a{cache, batch(starts, lengths, table, seqs, tokens, width, stride), ptr(k), ptr(v),
-                                 k_token, k_head, v_token, v_head, reinterpret_cast<const float*>(rope), rot,
-                                 rope_rows, elem, interleaved};
-    check(xt_cache_append(&a, ptr(stream)), "cache_append");
-  });
-  m.def("cache_attention_workspace", [](const xt_cache& cache, int seqs, int tokens, int width, int q_heads, int max_new,
-                                        int elem) {
-    xt_cache_attention_args a{};
-    a.cache = cache;
-    a.batch.seqs = seqs;
-    a.batch.tokens = tokens;
-    a.batch.table_width = width;
-    a.q_heads = q_heads;
-    a.max_new = max_new;
-    a.elem = elem;
-    // the arrays do not matter for the size
-    static const int32_t none = 0;
-    a.batch.starts = a.batch.lengths = a.batch.table = &none;
-    size_t bytes = 0;
-    check(xt_cache_attention_workspace(&a, &bytes), "cache_attention");
-    return bytes;
-  });
-  m.def("cache_attention", [](const xt_cache& cache, uintptr_t starts, uintptr_t lengths, uintptr_t table, int seqs,
-                              int tokens, int width, int64_t stride, uintptr_t q, uintptr_t out, int64_t q_token,
-                              int64_t q_head, int64_t out_token, int64_t out_head, int q_heads, int max_new, int window,
-                              float scale, float softcap, int elem, uintptr_t workspace, size_t bytes, uintptr_t stream) {
-    const xt_cache_attention_args a{cache, batch(starts, lengths, table, seqs, tokens, width, stride), ptr(q), ptr(out),
-                                    q_token, q_head, out_token, out_head, q_heads, max_new, window, scale, softcap, elem,
-                                    ptr(workspace), bytes};
-    check(xt_cache_attention(&a, ptr(stream)), "cache_attention");
-  });
-  m.def("dequantize", [](uintptr_t q, uintptr_t scales, uintptr_t out, int64_t n, int64_t run, int elem, uintptr_t stream) {
-    check(xt_dequantize(reinterpret_cast<const int8_t*>(q), reinterpret_cast<const float*>(scales), ptr(out), n, run, elem,
-                        ptr(stream)),
-          "dequantize");
-  });
 }
