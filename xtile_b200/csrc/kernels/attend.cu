@@ -7,16 +7,22 @@
 // and a window if one is set).  A token's reads are 2 dim int8 bytes a kv
 // head, so single-token decoding is bound by HBM.
 //
-// Work is cut into units of 16 tokens of one (sequence, kv head, 16 packed
-// query rows) segment; a row is a (new token, head of the group) pair, so the
-// heads of a group share the cache's reads.  The units of all segments stand
-// in one line, and each warp of a grid that fills the GPU takes an equal run
-// of it: ragged lengths, a single long sequence and many short ones all load
-// every SM alike.  A warp works alone, without a CTA barrier: it streams its
-// own tiles with cp.async through its own ring in shared memory, runs the two
-// products on mma.sync m16n8k16 in f16 and keeps the running maximum, sum and
-// output of its rows in registers.  Segments that several warps share are
-// joined by a second kernel from f32 partial results.
+// Work is cut into units of kTile tokens of one (sequence, kv head, packed query
+// rows) segment; a row is a (new token, head of the group) pair, so the heads
+// of a group share the cache's reads.  The units of all segments stand in one
+// line, and each warp of a grid that fills the GPU takes an equal run of it:
+// ragged lengths, a single long sequence and many short ones all load every SM
+// alike.  A warp works alone, without a CTA barrier: it streams its own tiles
+// with cp.async through its own ring in shared memory, runs the two products
+// on mma.sync m16n8k16 in f16 and keeps the running reference, sum and output
+// of its rows in registers.  Segments that several warps share are joined by a
+// second kernel from f32 partial results.
+//
+// Tokens (and the output's dims) are the products' m, query rows their n: the
+// converted cache bytes are A operands that all of a segment's rows share, and
+// a group of up to 8 heads fills one n8 tile.  What a unit costs is mostly the
+// conversion of its bytes (three instructions for four key bytes, six for four
+// value bytes), not the products.
 //
 // int8 values are exact in f16, and so is a bf16 query divided by a power of
 // two that brings its row's largest magnitude near 2^10 (elements under 2^-35
@@ -39,17 +45,26 @@ namespace xt {
 namespace dev {
 namespace {
 
-constexpr int kTile = 16;  // tokens of a unit, and query rows of a segment
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNone = -1e30f;  // reference of a row that has seen no token
 
-template <int DP, bool F32>
+// How one instance of the kernel is laid out.  DP: dims, padded; NR: n8 tiles
+// of query rows.
+template <int DP, bool F32, int NR>
 struct Shape {
+  static constexpr int kRows = 8 * NR;  // query rows of a segment
+  static constexpr int kMTiles = 1;     // m16 tiles of tokens in a unit
+  static constexpr int kTile = 16 * kMTiles;
   static constexpr int kWarps = DP <= 128 ? 4 : 2;
-  static constexpr int kStages = DP <= 64 ? 8 : DP <= 128 ? 4 : 3;
-  static constexpr int kCtas = F32 ? 2 : 3;                       // CTAs an SM
+  static constexpr bool kHeavy = F32 || NR == 4 || DP > 128;
+  static constexpr int kCtas = DP > 128 ? (F32 && NR > 1 ? 2 : 3) : kHeavy ? 2 : NR == 2 ? 3 : 4;  // CTAs an SM
   static constexpr int kStageBytes = 2 * kTile * DP + 2 * kTile * 4;  // keys, values, their scales
-  static constexpr bool kQueryInSmem = F32 || DP > 128;           // else its fragments stay in registers
-  static constexpr int kQueryBytes = kQueryInSmem ? (DP / 16) * 512 * (F32 ? 2 : 1) : 0;
+  static constexpr bool kQueryInSmem = kHeavy;                        // else its fragments stay in registers
+  static constexpr int kQueryBytes = kQueryInSmem ? (DP / 16) * NR * 256 * (F32 ? 2 : 1) : 0;
+  static constexpr int kSpare = 226 * 1024 / kCtas - 1024;            // shared memory of a CTA
+  static constexpr int kFit = (kSpare / kWarps - kQueryBytes) / kStageBytes;
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static_assert(kStages >= 3, "a warp's ring holds three stages at least");
   static constexpr int kWarpBytes = kStages * kStageBytes + kQueryBytes;
 };
 
@@ -57,8 +72,8 @@ struct AttendDev {
   AttendArgs a;
   FastDiv page_div, block_div, group_div;
   int group;
-  float* part;     // [workers][2][16][dim] partial outputs
-  float2* part_ml; // [workers][2][16] (reference, sum)
+  float* part;      // [workers][2][rows][dim] partial outputs
+  float2* part_ml;  // [workers][2][rows] (reference, sum)
   int64_t workers;
 };
 
@@ -71,14 +86,15 @@ struct Segments {
   }
 };
 
+template <int ROWS, int TILE>
 __device__ __forceinline__ Segments load_segments(const AttendDev& p, int b) {
   Segments g;
   g.seq = load_sequence(p.a.batch, p.a.cache.page, b);
   if (!g.seq.ok) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
-  g.row_tiles = static_cast<int>((static_cast<int64_t>(g.seq.count) * p.group + kTile - 1) / kTile);
+  g.row_tiles = static_cast<int>((static_cast<int64_t>(g.seq.count) * p.group + ROWS - 1) / ROWS);
   const int64_t first_seen = p.a.window > 0 ? static_cast<int64_t>(g.seq.length) - g.seq.count - p.a.window + 1 : 0;
-  g.lo = first_seen > 0 ? static_cast<int>(first_seen) / kTile : 0;
-  g.hi = (g.seq.length + kTile - 1) / kTile;
+  g.lo = first_seen > 0 ? static_cast<int>(first_seen) / TILE : 0;
+  g.hi = (g.seq.length + TILE - 1) / TILE;
   if (g.lo > g.hi) g.lo = g.hi;
   return g;
 }
@@ -90,10 +106,11 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 }
 
 // Units of all sequences, and of those before ``b``.  A whole warp calls.
+template <int ROWS, int TILE>
 __device__ __forceinline__ int64_t count_units(const AttendDev& p, int b, int64_t* before) {
   int64_t total = 0, front = 0;
   for (int i = threadIdx.x & 31; i < p.a.batch.seqs; i += 32) {
-    const int64_t u = load_segments(p, i).units(p.a.cache.heads);
+    const int64_t u = load_segments<ROWS, TILE>(p, i).units(p.a.cache.heads);
     total += u;
     if (i < b) front += u;
   }
@@ -102,6 +119,7 @@ __device__ __forceinline__ int64_t count_units(const AttendDev& p, int b, int64_
 }
 
 // A place in the line of units.
+template <int ROWS, int TILE>
 struct Cursor {
   Segments seg;
   int b, head, row_tile, tile;
@@ -112,7 +130,7 @@ struct Cursor {
     b = 0;
     for (int base = 0; base < p.a.batch.seqs; base += 32) {
       const int i = base + lane;
-      const int64_t mine = i < p.a.batch.seqs ? load_segments(p, i).units(heads) : 0;
+      const int64_t mine = i < p.a.batch.seqs ? load_segments<ROWS, TILE>(p, i).units(heads) : 0;
       int64_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -128,7 +146,7 @@ struct Cursor {
       }
       front += __shfl_sync(0xffffffffu, upto, 31);
     }
-    seg = load_segments(p, b);
+    seg = load_segments<ROWS, TILE>(p, b);
     const int tiles = seg.hi - seg.lo;
     const int64_t at = u - front, line = at / tiles;
     tile = seg.lo + static_cast<int>(at - line * tiles);
@@ -146,7 +164,7 @@ struct Cursor {
     head = 0;
     do {
       ++b;
-      seg = load_segments(p, b);
+      seg = load_segments<ROWS, TILE>(p, b);
     } while (seg.units(1) == 0 && b + 1 < p.a.batch.seqs);
     tile = seg.lo;
   }
@@ -166,12 +184,26 @@ __device__ __forceinline__ void cp_async_wait() {
 }
 
 // c += a b for 16 x 16 f16 a, 16 x 8 f16 b, f32 c.
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+
+// The transpose of an 8 x 8 matrix of 16-bit elements, a row's pairs over a quad.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// 2^x, at most 2^-22 of it off; 0 for -inf.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // Two biased bytes (int8 + 128), picked by ``sel`` from w, as f16 values: the
@@ -189,10 +221,11 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float2 unpack_half2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
 // What two values leave after their rounding to f16, as f16.
 __device__ __forceinline__ uint32_t rest_half2(float lo, float hi, uint32_t rounded) {
-  const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
+  const float2 r = unpack_half2(rounded);
   return pack_half2(lo - r.x, hi - r.y);
 }
 
@@ -209,21 +242,27 @@ __device__ __forceinline__ uint32_t value_place(int row, int c) {
   return row * DP + ((DP >= 128 ? c ^ (((row >> 1) & 3) << 1) : c ^ (((row >> 1) & 1) << 1)) << 4);
 }
 
-template <int DP, bool F32>
-__global__ void __launch_bounds__(Shape<DP, F32>::kWarps * 32, Shape<DP, F32>::kCtas)
+__device__ __forceinline__ void lds128(uint32_t (&w)[4], uint32_t at) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+}
+
+template <int DP, bool F32, int NR>
+__global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32, NR>::kCtas)
     attend_units(const __grid_constant__ AttendDev p) {
-  using S = Shape<DP, F32>;
+  using S = Shape<DP, F32, NR>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+  constexpr int kTile = S::kTile, kMTiles = S::kMTiles, kRows = S::kRows;
   constexpr int kSteps = DP / 16;    // k16 steps of the score product
-  constexpr int kOut = DP / 8;       // n8 tiles of the output
+  constexpr int kOut = DP / 16;      // m16 tiles of the output
   constexpr int kChunks = DP / 16;   // 16-byte chunks of a token
   constexpr int kRowsAtOnce = 32 / kChunks;
+  constexpr int kSpan = DP >= 128 ? 16 : 8;  // consecutive dims that a lane reads of a value row
   extern __shared__ __align__(128) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   unsigned char* ring = smem + warp * S::kWarpBytes;
   const uint32_t ring_addr = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  uint4* query = reinterpret_cast<uint4*>(ring + S::kStages * S::kStageBytes);
+  uint2* query = reinterpret_cast<uint2*>(ring + S::kStages * S::kStageBytes);
   const CacheView& cache = p.a.cache;
   const int dim = cache.dim;
 
@@ -237,54 +276,80 @@ __global__ void __launch_bounds__(Shape<DP, F32>::kWarps * 32, Shape<DP, F32>::k
   griddep_wait();
 
   int64_t unused;
-  const int64_t total = count_units(p, 0, &unused);
+  const int64_t total = count_units<kRows, kTile>(p, 0, &unused);
   const int64_t per = (total + p.workers - 1) / p.workers;
   const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
-  const int64_t begin = worker * per, end = begin + per < total ? begin + per : total;
-  if (begin >= end) return;
+  const int64_t begin = worker * per;
+  if (begin >= total) return;
+  int left = static_cast<int>(total - begin < per ? total - begin : per);  // units to do, and to issue
+  int to_issue = left;
 
-  Cursor at;
+  Cursor<kRows, kTile> at;
   at.seek(p, begin);
-  Cursor ahead = at;
-  int64_t to_issue = end - begin;
+  Cursor<kRows, kTile> ahead = at;
 
-  // --- loading: lane l & 15 looks up the page of token l of the tile to come
+  // --- loading.  Where pages hold whole tiles (page a multiple of kTile) a tile
+  // is one run of rows; else lane l % kTile looks up token l of the tile.
+  const bool one_page = cache.page % kTile == 0;
+  const int my_chunk = lane % kChunks, my_row = lane / kChunks;
   int page_id = 0, page_row = 0;
-  bool token_there = false;
   auto look_up = [&] {
-    const int token = ahead.tile * kTile + (lane & 15);
-    token_there = token < ahead.seg.seq.length;
+    const int token = ahead.tile * kTile + (one_page ? 0 : lane % kTile);
     const int index = p.page_div.quot(token);
     page_row = token - index * cache.page;
-    page_id = token_there ? p.a.batch.table[ahead.b * p.a.batch.table_stride + index] : 0;
+    page_id = token < ahead.seg.seq.length ? p.a.batch.table[ahead.b * p.a.batch.table_stride + index] : 0;
   };
   auto issue = [&](int stage) {
     if (to_issue > 0) {
       const uint32_t base = ring_addr + stage * S::kStageBytes;
+      const int there = min(ahead.seg.seq.length - ahead.tile * kTile, kTile);  // tokens of the tile
       const bool bad = page_id < 0 || page_id >= cache.pages;
-      const bool there = token_there && !bad;
       const int64_t line = static_cast<int64_t>(bad ? 0 : page_id) * cache.heads + ahead.head;
       const int64_t row_at = line * cache.page + page_row;
-      const int64_t scale_at = line * (cache.page / cache.block) + p.block_div.quot(page_row);
-      const uint32_t scale_to = base + 2 * kTile * DP + lane * 4;
-      if (token_there && bad) {
-        // a page outside the cache: recorded, and NaN for whoever attends to it
-        atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(scale_to), "r"(0x7fc00000u) : "memory");
-      } else {
-        cp_async4(scale_to, (lane < kTile ? cache.k_scale : cache.v_scale) + (there ? scale_at : 0), there ? 4 : 0);
-      }
-      const unsigned rows_there = __ballot_sync(0xffffffffu, there);
-      const int chunk = lane % kChunks;
+      // the scales: a lane a token, keys' and values'
 #pragma unroll
-      for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-        const int row = i * kRowsAtOnce + lane / kChunks;
-        const int64_t from = __shfl_sync(0xffffffffu, row_at, row) * dim + chunk * 16;
-        if (chunk * 16 >= dim) continue;
-        // rows behind the sequence's end are left as they are: finite int8, and their weight is 0
-        if (!(rows_there >> row & 1)) continue;
-        cp_async16(base + key_place<DP>(row, chunk), cache.k + from);
-        cp_async16(base + kTile * DP + value_place<DP>(row, chunk), cache.v + from);
+      for (int i = 0; i < 2 * kTile / 32; ++i) {
+        const int slot = i * 32 + lane, token = slot % kTile;
+        const int row = page_row + (one_page ? token : 0);
+        const int64_t scale_at = line * (cache.page / cache.block) + p.block_div.quot(row);
+        const uint32_t to = base + 2 * kTile * DP + slot * 4;
+        const bool mine = token < there;
+        if (mine && bad) {
+          // a page outside the cache: recorded, and NaN for whoever attends to it
+          atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(0x7fc00000u) : "memory");
+        } else {
+          cp_async4(to, (slot < kTile ? cache.k_scale : cache.v_scale) + (mine ? scale_at : 0), mine ? 4 : 0);
+        }
+      }
+      // Rows behind the sequence's end, and of a bad page, are left as they are:
+      // finite int8, and their weight is 0 or NaN.
+      if (one_page) {
+        const int rows = bad || my_chunk * 16 >= dim ? 0 : there;
+        const int64_t from = (row_at + my_row) * dim + my_chunk * 16;
+        const int8_t* k = cache.k + from;
+        const int8_t* v = cache.v + from;
+#pragma unroll
+        for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
+          const int row = i * kRowsAtOnce + my_row;
+          if (row < rows) {
+            cp_async16(base + key_place<DP>(row, my_chunk), k);
+            cp_async16(base + kTile * DP + value_place<DP>(row, my_chunk), v);
+          }
+          k += kRowsAtOnce * dim;
+          v += kRowsAtOnce * dim;
+        }
+      } else {
+        const unsigned rows_there = __ballot_sync(0xffffffffu, lane % kTile < there && !bad);
+#pragma unroll
+        for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
+          const int row = i * kRowsAtOnce + my_row;
+          const int64_t from = __shfl_sync(0xffffffffu, row_at, row) * dim + my_chunk * 16;
+          if (my_chunk * 16 < dim && (rows_there >> row & 1)) {
+            cp_async16(base + key_place<DP>(row, my_chunk), cache.k + from);
+            cp_async16(base + kTile * DP + value_place<DP>(row, my_chunk), cache.v + from);
+          }
+        }
       }
       if (--to_issue > 0) {
         ahead.advance(p);
@@ -298,16 +363,20 @@ __global__ void __launch_bounds__(Shape<DP, F32>::kWarps * 32, Shape<DP, F32>::k
   for (int i = 0; i < S::kStages - 1; ++i) issue(i);
 
   // --- the segment at hand
-  uint4 qf[S::kQueryInSmem ? 1 : kSteps];
-  float o[kOut][4];
-  float ref[2], sum[2], row_scale[2];   // rows g and g + 8: reference of the exponents, sum of the weights
-  int row_pos[2];                       // positions of their queries
-  int value_exp = 0;                    // the weights carry vs 2^(10 - value_exp); set by the first token seen
-  bool value_set = false, whole = true; // whole: the segment's first unit is this worker's
+  uint2 qf[S::kQueryInSmem ? 1 : NR][S::kQueryInSmem ? 1 : kSteps];
+  float o[kOut][NR][4];
+  // rows 2 t and 2 t + 1 of each n8 tile: reference of the exponents, sum of
+  // the weights, factor of the score, the score's start, position of the query
+  float ref[NR][2], sum[NR][2], row_scale[NR][2], start[NR][2];
+  int row_pos[NR][2];
+  int pos_min = 0, pos_max = 0;
+  int value_exp = 0;                     // the weights carry vs 2^(10 - value_exp); set by the first token seen
+  bool value_set = false, whole = true;  // whole: the segment's first unit is this worker's
   const float cap = p.a.softcap;
+  const bool negative = p.a.scale < 0.0f;
 
   auto row_of = [&](int r, int* token) {  // packed row r of the row tile: its new token and query head, or -1
-    const int packed = at.row_tile * kTile + r;
+    const int packed = at.row_tile * kRows + r;
     const int i = p.group_div.quot(packed);
     *token = i;
     return i < at.seg.seq.count ? at.head * p.group + packed - i * p.group : -1;
@@ -317,102 +386,111 @@ __global__ void __launch_bounds__(Shape<DP, F32>::kWarps * 32, Shape<DP, F32>::k
     whole = at.tile == at.seg.lo;
     value_set = false;
     value_exp = 0;
-#pragma unroll
-    for (int i = 0; i < kOut; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-    float q[2][kSteps][4];
-    float top[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      int i;
-      const int head = row_of(g + 8 * r, &i);
-      row_pos[r] = head < 0 ? -1 : at.seg.seq.length - at.seg.seq.count + i;
-      const T* from = static_cast<const T*>(p.a.q) + static_cast<int64_t>(at.seg.seq.first + i) * p.a.q_token +
-                      static_cast<int64_t>(head) * p.a.q_head;
-      top[r] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);  // the lane's four dims of this step
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[r][s][e] = 0.0f;
-        if (head >= 0 && d < dim) Vec<T, 4>::load(from + d, q[r][s]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top[r] = fmaxf(top[r], fabsf(q[r][s][e]));
-      }
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      // the row times 2^(10 - exponent of its largest magnitude)
-      const int e = min(max(static_cast<int>(__float_as_uint(top[r]) >> 23), 11), 243);
-      const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23);
-      const float down = __uint_as_float(static_cast<uint32_t>(e - 10) << 23);
-      row_scale[r] = down * p.a.scale * (cap > 0.0f ? 1.0f / cap : kLog2e);
-      ref[r] = -INFINITY;
-      sum[r] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) q[r][s][e2] *= up;
-    }
+    const int before = at.seg.seq.length - at.seg.seq.count;
+    pos_min = before + p.group_div.quot(at.row_tile * kRows);
+    pos_max = before + min(static_cast<int>(p.group_div.quot(at.row_tile * kRows + kRows - 1)), at.seg.seq.count - 1);
     if constexpr (S::kQueryInSmem) __syncwarp();
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const uint4 f = make_uint4(pack_half2(q[0][s][0], q[0][s][1]), pack_half2(q[1][s][0], q[1][s][1]),
-                                 pack_half2(q[0][s][2], q[0][s][3]), pack_half2(q[1][s][2], q[1][s][3]));
-      if constexpr (S::kQueryInSmem) {
-        query[s * 32 + lane] = f;  // read back by this lane alone
-        if constexpr (F32)
-          query[(kSteps + s) * 32 + lane] =
-              make_uint4(rest_half2(q[0][s][0], q[0][s][1], f.x), rest_half2(q[1][s][0], q[1][s][1], f.y),
-                         rest_half2(q[0][s][2], q[0][s][3], f.z), rest_half2(q[1][s][2], q[1][s][3], f.w));
-      } else {
-        qf[s] = f;
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int i = 0; i < kOut; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][nr][j] = 0.0f;
+      // the lane's part of row g: four dims of each step
+      float q[kSteps][4], top = 0.0f;
+      int i;
+      const int head = row_of(8 * nr + g, &i);
+      const T* from = static_cast<const T*>(p.a.q) + static_cast<int64_t>(at.seg.seq.first + i) * p.a.q_token +
+                      static_cast<int64_t>(head) * p.a.q_head;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[s][e] = 0.0f;
+        if (head >= 0 && d < dim) Vec<T, 4>::load(from + d, q[s]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(q[s][e]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the row times 2^(10 - exponent of its largest magnitude), and the scale's sign
+      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 243);
+      const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23 | (negative ? 0x80000000u : 0u));
+      float total_q = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) q[s][x] *= up;
+        const uint2 f = make_uint2(pack_half2(q[s][0], q[s][1]), pack_half2(q[s][2], q[s][3]));
+        if constexpr (S::kQueryInSmem)
+          query[(nr * kSteps + s) * 32 + lane] = f;  // read back by this lane alone
+        else
+          qf[nr][s] = f;
+        if constexpr (F32) {
+          query[((NR + nr) * kSteps + s) * 32 + lane] =
+              make_uint2(rest_half2(q[s][0], q[s][1], f.x), rest_half2(q[s][2], q[s][3], f.y));
+        } else {
+          const float2 a = unpack_half2(f.x), b = unpack_half2(f.y);
+          total_q += (a.x + a.y) + (b.x + b.y);
+        }
+      }
+      total_q += __shfl_xor_sync(0xffffffffu, total_q, 1);
+      total_q += __shfl_xor_sync(0xffffffffu, total_q, 2);
+      // The keys' bytes enter as f16 subnormals (byte + 128) 2^-24: the score
+      // starts at what the 128s will add.  In f32 they enter as themselves.
+      const float down = __uint_as_float(static_cast<uint32_t>(e - 10) << 23) * (F32 ? 1.0f : 16777216.0f) *
+                         fabsf(p.a.scale) * (cap > 0.0f ? 1.0f / cap : kLog2e);
+      const float offset = F32 ? 0.0f : total_q * (-128.0f / 16777216.0f);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        row_scale[nr][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
+        start[nr][c] = __shfl_sync(0xffffffffu, offset, (2 * t + c) * 4);
+        row_pos[nr][c] = before + static_cast<int>(p.group_div.quot(at.row_tile * kRows + 8 * nr + 2 * t + c));
+        ref[nr][c] = kNone;
+        sum[nr][c] = 0.0f;
       }
     }
   };
 
   auto finish_segment = [&](bool last_unit) {
     const float up = __uint_as_float(static_cast<uint32_t>(value_exp + 117) << 23);
+    const bool done = whole && last_unit;
+    const int64_t slot = worker * 2 + (whole ? 1 : 0);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-      int i;
-      const int head = row_of(g + 8 * r, &i);
-      if (head < 0) continue;
-      constexpr int kSpan = DP >= 128 ? 32 : 16;  // consecutive dims that the lane holds of a row
-      const bool done = whole && last_unit;
-      const float by = done ? (sum[r] > 0.0f || sum[r] != sum[r] ? up / sum[r] : 0.0f) : up;
-      const int64_t slot = worker * 2 + (whole ? 1 : 0);
-      T* to = static_cast<T*>(p.a.out) + static_cast<int64_t>(at.seg.seq.first + i) * p.a.out_token +
-              static_cast<int64_t>(head) * p.a.out_head;
-      float* part = p.part + (slot * kTile + g + 8 * r) * dim;
+    for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int h = 0; h < kOut * 2 / kSpan; ++h) {
-        // C columns 2 t and 2 t + 1 of n-tile i stand for dims (2 t) kSpan / 2 + i and (2 t + 1) kSpan / 2 + i
+      for (int c = 0; c < 2; ++c) {
+        float s = sum[nr][c];
 #pragma unroll
-        for (int d = 0; d < kSpan; d += 4) {
+        for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        const int row = 8 * nr + 2 * t + c;
+        int i;
+        const int head = row_of(row, &i);
+        if (head < 0) continue;
+        const float by = done ? (s > 0.0f || s != s ? up / s : 0.0f) : up;
+        T* to = static_cast<T*>(p.a.out) + static_cast<int64_t>(at.seg.seq.first + i) * p.a.out_token +
+                static_cast<int64_t>(head) * p.a.out_head;
+        float* part = p.part + (slot * kRows + row) * dim;
+#pragma unroll
+        for (int x = 0; x < kOut * 2; x += 4) {
+          // m16 tile i's rows g and g + 8 stand for two neighbouring dims of the lane's span
           float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int x = d + e, nt = h * (kSpan / 2) + x % (kSpan / 2);
-            y[e] = o[nt][2 * r + x / (kSpan / 2)] * by;
-          }
-          const int dim_at = h * 4 * kSpan + t * kSpan + d;
-          if (dim_at >= dim) continue;
+          for (int e = 0; e < 4; ++e) y[e] = o[(x + e) / 2][nr][2 * ((x + e) % 2) + c] * by;
+          const int d = x / kSpan * 8 * kSpan + g * kSpan + x % kSpan;
+          if (d >= dim) continue;
           if (done)
-            Vec<T, 4>::store(to + dim_at, y);
+            Vec<T, 4>::store(to + d, y);
           else
-            *reinterpret_cast<float4*>(part + dim_at) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4*>(part + d) = make_float4(y[0], y[1], y[2], y[3]);
         }
+        if (!done && g == 0) p.part_ml[slot * kRows + row] = make_float2(ref[nr][c], s);
       }
-      if (!done && t == 0) p.part_ml[slot * kTile + g + 8 * r] = make_float2(ref[r], sum[r]);
-    }
   };
 
   start_segment();
   int stage = 0;
-  for (int64_t u = begin; u < end; ++u) {
+  while (true) {
     cp_async_wait<S::kStages - 2>();
     __syncwarp();
     issue(stage == 0 ? S::kStages - 1 : stage - 1);
@@ -420,177 +498,212 @@ __global__ void __launch_bounds__(Shape<DP, F32>::kWarps * 32, Shape<DP, F32>::k
     const uint32_t values = keys + kTile * DP;
     const float* scales = reinterpret_cast<const float*>(ring + stage * S::kStageBytes + 2 * kTile * DP);
 
-    // --- scores: two n8 tiles of tokens
-    float z[2][4];
+    // --- scores: token rows g and g + 8 of each m16 tile
+    float z[kMTiles][NR][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int m = 0; m < kMTiles; ++m) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[n][e] = 0.0f;
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[m][nr][e] = start[nr][e & 1];
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j) {
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(keys + key_place<DP>(8 * n + g, 4 * j + t)));
+        uint32_t u[4], w[4];
+        lds128(u, keys + key_place<DP>(16 * m + g, 4 * j + t));
+        lds128(w, keys + key_place<DP>(16 * m + g + 8, 4 * j + t));
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const uint32_t biased = w[s] ^ 0x80808080u;
-          const uint32_t b0 = bytes_to_half2<kLow>(biased), b1 = bytes_to_half2<kHigh>(biased);
+          const uint32_t x = u[s] ^ 0x80808080u, y = w[s] ^ 0x80808080u;
           const int step = 4 * j + s;
-          if constexpr (S::kQueryInSmem) {
-            mma_16816(z[n], query[step * 32 + lane], b0, b1);
-            if constexpr (F32) mma_16816(z[n], query[(kSteps + step) * 32 + lane], b0, b1);
+          uint32_t a0, a1, a2, a3;
+          if constexpr (F32) {
+            a0 = bytes_to_half2<kLow>(x), a2 = bytes_to_half2<kHigh>(x);
+            a1 = bytes_to_half2<kLow>(y), a3 = bytes_to_half2<kHigh>(y);
           } else {
-            mma_16816(z[n], qf[step], b0, b1);
+            a0 = __byte_perm(x, 0, kLow), a2 = __byte_perm(x, 0, kHigh);
+            a1 = __byte_perm(y, 0, kLow), a3 = __byte_perm(y, 0, kHigh);
+          }
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) {
+            if constexpr (S::kQueryInSmem) {
+              mma_16816(z[m][nr], a0, a1, a2, a3, query[(nr * kSteps + step) * 32 + lane]);
+              if constexpr (F32) mma_16816(z[m][nr], a0, a1, a2, a3, query[((NR + nr) * kSteps + step) * 32 + lane]);
+            } else {
+              mma_16816(z[m][nr], a0, a1, a2, a3, qf[nr][step]);
+            }
           }
         }
       }
     }
 
-    // --- weights
+    // --- weights: z becomes the score over the row's factor (with a cap: the
+    // capped score in the exponent's unit), y its exponent
     const int token0 = at.tile * kTile;
-    float vs[2][2];
-    float top[2] = {-INFINITY, -INFINITY};
-    bool some = false;
+    // every row sees all of the tile's tokens
+    const bool open = token0 + kTile - 1 <= pos_min && (p.a.window == 0 || token0 > pos_max - p.a.window);
+    float vs[kMTiles][2], y[kMTiles][NR][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const float2 ks = *reinterpret_cast<const float2*>(scales + 8 * n + 2 * t);
-      const float2 v = *reinterpret_cast<const float2*>(scales + kTile + 8 * n + 2 * t);
-      vs[n][0] = v.x, vs[n][1] = v.y;
+    for (int m = 0; m < kMTiles; ++m) {
+      const float k0 = scales[16 * m + g], k1 = scales[16 * m + g + 8];
+      vs[m][0] = scales[kTile + 16 * m + g], vs[m][1] = scales[kTile + 16 * m + g + 8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = z[n][e] * ((e & 1) ? ks.y : ks.x) * row_scale[e >> 1];
-        if (cap > 0.0f) x = tanhf(x) * (cap * kLog2e);
-        const int j = token0 + 8 * n + 2 * t + (e & 1), pos = row_pos[e >> 1];
-        const bool seen = j <= pos && (p.a.window == 0 || j > pos - p.a.window);
-        z[n][e] = seen ? x : -INFINITY;
-        some |= seen;
-        top[e >> 1] = fmaxf(top[e >> 1], z[n][e]);
-      }
-    }
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-    }
-    // The reference of a row's exponents follows its maximum only when that has
-    // risen by more than 2^4, so that most units leave the output as it is.
-    const bool rise = top[0] > ref[0] + 4.0f || top[1] > ref[1] + 4.0f;
-    if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float now = fmaxf(ref[r], top[r]);
-        const float f = now == -INFINITY ? 1.0f : exp2f(ref[r] - now);
-        ref[r] = now;
-        sum[r] *= f;
-#pragma unroll
-        for (int i = 0; i < kOut; ++i) {
-          o[i][2 * r] *= f;
-          o[i][2 * r + 1] *= f;
+        for (int e = 0; e < 4; ++e) {
+          z[m][nr][e] *= e < 2 ? k0 : k1;
+          if (cap > 0.0f) z[m][nr][e] = tanhf(z[m][nr][e] * row_scale[nr][e & 1]) * (cap * kLog2e);
         }
-      }
     }
-    // The values' scales enter the weights as multiples of a power of two that
-    // the first scale seen sets, and that changes only where a weight would
-    // leave f16's range.  2^10 of room below the largest weights keeps f16's
+    auto exponents = [&] {
+      float top = -INFINITY;
+#pragma unroll
+      for (int m = 0; m < kMTiles; ++m)
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float by = cap > 0.0f ? 1.0f : row_scale[nr][e & 1];
+            y[m][nr][e] = fmaf(z[m][nr][e], by, -ref[nr][e & 1]);
+            if (!open) {
+              const int j = token0 + 16 * m + g + 8 * (e >> 1), pos = row_pos[nr][e & 1];
+              if (j > pos || (p.a.window > 0 && j <= pos - p.a.window)) y[m][nr][e] = -INFINITY;
+            }
+            top = fmaxf(top, y[m][nr][e]);
+          }
+      return top;
+    };
+    const float top = exponents();
+    float shift = __uint_as_float(static_cast<uint32_t>(137 - value_exp) << 23);
+    float most = 0.0f;
+#pragma unroll
+    for (int m = 0; m < kMTiles; ++m) most = fmaxf(most, fmaxf(vs[m][0], vs[m][1]));
+    // The reference of a row's exponents follows its maximum only when that has
+    // risen by more than 2^4, and the values' scales enter the weights as
+    // multiples of a power of two that the first scales seen set and that
+    // changes only where a weight could leave f16's range: most units leave
+    // the output as it is.  2^10 of room below the largest weights keeps f16's
     // subnormals (2^-24 apart) at 2^-34 of them.
-    auto exponent_of_scales = [&] {
+    if (__any_sync(0xffffffffu, top > 4.0f || most * shift > 2048.0f || !value_set)) {
       int e = 0;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int m = 0; m < kMTiles; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float seen = -INFINITY;
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr)
+            seen = fmaxf(seen, fmaxf(y[m][nr][2 * r], y[m][nr][2 * r + 1]));
+          const int b = static_cast<int>(__float_as_uint(vs[m][r]) >> 23 & 255);
+          if (seen > -INFINITY && b < 255) e = max(e, b);
+        }
+      e = __reduce_max_sync(0xffffffffu, e);
+      float fall = 1.0f;
+      if (e > 0) {
+        e = min(max(e, 11), 250) - 127;
+        if (!value_set) {
+          value_exp = e;
+        } else if (e > value_exp) {
+          fall = __uint_as_float(static_cast<uint32_t>(max(127 + value_exp - e, 0)) << 23);
+          value_exp = e;
+        }
+        value_set = true;
+        shift = __uint_as_float(static_cast<uint32_t>(137 - value_exp) << 23);
+      }
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const bool seen = z[n][c] != -INFINITY || z[n][c + 2] != -INFINITY;
-          const int b = static_cast<int>(__float_as_uint(vs[n][c]) >> 23 & 255);
-          if (seen && b < 255) e = max(e, b);
+          float rise = -INFINITY;
+#pragma unroll
+          for (int m = 0; m < kMTiles; ++m) rise = fmaxf(rise, fmaxf(y[m][nr][c], y[m][nr][c + 2]));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) rise = fmaxf(rise, __shfl_xor_sync(0xffffffffu, rise, x));
+          const float by = cap > 0.0f ? 1.0f : row_scale[nr][c];
+          float best = -INFINITY;
+#pragma unroll
+          for (int m = 0; m < kMTiles; ++m) {
+            if (y[m][nr][c] > -INFINITY) best = fmaxf(best, z[m][nr][c] * by);
+            if (y[m][nr][c + 2] > -INFINITY) best = fmaxf(best, z[m][nr][c + 2] * by);
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
+          float f = 1.0f;
+          if (rise > 0.0f) {
+            f = exp2_fast(ref[nr][c] - best);
+            ref[nr][c] = best;
+          }
+          sum[nr][c] *= f;
+          f *= fall;
+#pragma unroll
+          for (int i = 0; i < kOut; ++i) {
+            o[i][nr][c] *= f;
+            o[i][nr][c + 2] *= f;
+          }
         }
-      return __reduce_max_sync(0xffffffffu, e);
-    };
-    if (!value_set && __any_sync(0xffffffffu, some)) {
-      const int e = exponent_of_scales();
-      value_set = e > 0;
-      value_exp = e > 0 ? min(max(e, 11), 250) - 127 : 0;
+      exponents();
     }
-    float shift = __uint_as_float(static_cast<uint32_t>(137 - value_exp) << 23);
-    float w[2][4];
-    bool large = false;
+    uint2 wf[kMTiles][NR], wl[F32 ? kMTiles : 1][F32 ? NR : 1];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float base = ref[r] == -INFINITY ? 0.0f : ref[r];
+    for (int m = 0; m < kMTiles; ++m) {
+      const float v0 = vs[m][0] * shift, v1 = vs[m][1] * shift;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int nr = 0; nr < NR; ++nr) {
+        float w[4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float x = z[n][2 * r + c];
-          const float e = exp2f(x - base);
-          sum[r] += e;
-          w[n][2 * r + c] = x == -INFINITY ? 0.0f : e * (vs[n][c] * shift);
-          large |= w[n][2 * r + c] > 60000.0f;
+        for (int e = 0; e < 4; ++e) {
+          const float weight = exp2_fast(y[m][nr][e]);
+          sum[nr][e & 1] += weight;
+          w[e] = weight * (e < 2 ? v0 : v1);
+          // a token that is not seen may have any scale
+          if (!open && y[m][nr][e] == -INFINITY) w[e] = 0.0f;
         }
-    }
-    if (__any_sync(0xffffffffu, large)) {
-      const int e = min(max(exponent_of_scales(), 11), 250) - 127;
-      if (e > value_exp) {
-        const float f = __uint_as_float(static_cast<uint32_t>(max(127 + value_exp - e, 0)) << 23);
-        value_exp = e;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) w[n][c] *= f;
-#pragma unroll
-        for (int i = 0; i < kOut; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[i][c] *= f;
+        const uint32_t a = pack_half2(w[0], w[1]), b = pack_half2(w[2], w[3]);
+        wf[m][nr] = make_uint2(transpose_8x8(a), transpose_8x8(b));
+        if constexpr (F32)
+          wl[m][nr] = make_uint2(transpose_8x8(rest_half2(w[0], w[1], a)), transpose_8x8(rest_half2(w[2], w[3], b)));
       }
     }
-    uint4 wf, wl;
-    wf = make_uint4(pack_half2(w[0][0], w[0][1]), pack_half2(w[0][2], w[0][3]), pack_half2(w[1][0], w[1][1]),
-                    pack_half2(w[1][2], w[1][3]));
-    if constexpr (F32)
-      wl = make_uint4(rest_half2(w[0][0], w[0][1], wf.x), rest_half2(w[0][2], w[0][3], wf.y),
-                      rest_half2(w[1][0], w[1][1], wf.z), rest_half2(w[1][2], w[1][3], wf.w));
 
-    // --- output: the lane's tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-    constexpr int kWords = DP >= 128 ? 4 : 2;  // words of a token that one read brings
+    // --- output: the lane's tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each m16 tile
+    constexpr int kWords = kSpan / 4;  // words of a token that one read brings
 #pragma unroll
-    for (int h = 0; h < DP / (32 * kWords); ++h) {
-      uint32_t v[4][kWords];
+    for (int h = 0; h < DP / (8 * kSpan); ++h) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-        if constexpr (DP >= 128) {
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v[i][0]), "=r"(v[i][1]), "=r"(v[i][kWords - 2]), "=r"(v[i][kWords - 1])
-                       : "r"(values + value_place<DP>(row, 8 * h + g)));
-        } else {
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                       : "=r"(v[i][0]), "=r"(v[i][1])
-                       : "r"(values + value_place<DP>(row, g >> 1) + (g & 1) * 8));
+      for (int m = 0; m < kMTiles; ++m) {
+        uint32_t v[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 16 * m + 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (DP >= 128) {
+            lds128(v[i], values + value_place<DP>(row, 8 * h + g));
+          } else {
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                         : "=r"(v[i][0]), "=r"(v[i][1])
+                         : "r"(values + value_place<DP>(row, g >> 1) + (g & 1) * 8));
+          }
         }
 #pragma unroll
-        for (int k = 0; k < kWords; ++k) v[i][k] ^= 0x80808080u;
-      }
+        for (int k = 0; k < kWords; ++k) {
 #pragma unroll
-      for (int k = 0; k < kWords; ++k) {
+          for (int half = 0; half < 2; ++half) {
+            // bytes 2 half and 2 half + 1 of two tokens, side by side
+            const uint32_t a = __byte_perm(v[0][k], v[1][k], half ? 0x7362u : 0x5140u) ^ 0x80808080u;
+            const uint32_t b = __byte_perm(v[2][k], v[3][k], half ? 0x7362u : 0x5140u) ^ 0x80808080u;
+            const uint32_t a0 = bytes_to_half2<kLow>(a), a1 = bytes_to_half2<kHigh>(a);
+            const uint32_t a2 = bytes_to_half2<kLow>(b), a3 = bytes_to_half2<kHigh>(b);
+            const int i = h * kSpan / 2 + 2 * k + half;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // bytes 2 half and 2 half + 1 of two tokens, side by side
-          const uint32_t a = __byte_perm(v[0][k], v[1][k], half ? 0x7362u : 0x5140u);
-          const uint32_t b = __byte_perm(v[2][k], v[3][k], half ? 0x7362u : 0x5140u);
+            for (int nr = 0; nr < NR; ++nr) {
+              if constexpr (F32) {
+                // a fresh sum for the tile, added in f32: the tensor cores' own sums round toward zero
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_16816(c, a0, a1, a2, a3, wl[m][nr]);
+                mma_16816(c, a0, a1, a2, a3, wf[m][nr]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int nt = h * 4 * kWords + 4 * k + 2 * half + e;
-            const uint32_t b0 = e ? bytes_to_half2<kHigh>(a) : bytes_to_half2<kLow>(a);
-            const uint32_t b1 = e ? bytes_to_half2<kHigh>(b) : bytes_to_half2<kLow>(b);
-            if constexpr (F32) {
-              // a fresh sum for the unit, added in f32: the tensor cores' own sums round toward zero
-              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              mma_16816(c, wl, b0, b1);
-              mma_16816(c, wf, b0, b1);
-#pragma unroll
-              for (int x = 0; x < 4; ++x) o[nt][x] += c[x];
-            } else {
-              mma_16816(o[nt], wf, b0, b1);
+                for (int x = 0; x < 4; ++x) o[i][nr][x] += c[x];
+              } else {
+                mma_16816(o[i][nr], a0, a1, a2, a3, wf[m][nr]);
+              }
             }
           }
         }
@@ -599,12 +712,12 @@ __global__ void __launch_bounds__(Shape<DP, F32>::kWarps * 32, Shape<DP, F32>::k
     stage = stage == S::kStages - 1 ? 0 : stage + 1;
 
     const bool last_unit = at.tile + 1 == at.seg.hi;
-    if (last_unit || u + 1 == end) {
+    --left;
+    if (last_unit || left == 0) {
       finish_segment(last_unit);
-      if (u + 1 < end) {
-        at.advance(p);
-        start_segment();
-      }
+      if (left == 0) break;
+      at.advance(p);
+      start_segment();
     } else {
       ++at.tile;
     }
@@ -614,7 +727,7 @@ __global__ void __launch_bounds__(Shape<DP, F32>::kWarps * 32, Shape<DP, F32>::k
 
 // Joins the partial results of the segments that several workers had.  WARPS
 // warps have one (new token, query head): each takes every WARPS-th partial.
-template <class T, int DP, int WARPS>
+template <class T, int DP, int ROWS, int TILE, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(const __grid_constant__ AttendDev p) {
   constexpr int kPer = DP / 32;  // dims a lane
   __shared__ float shared_o[WARPS == 1 ? 1 : WARPS][WARPS == 1 ? 1 : DP];
@@ -626,7 +739,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
   if (index >= static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads) return;
   const int token = static_cast<int>(index / p.a.q_heads), q_head = static_cast<int>(index % p.a.q_heads);
   const int b = last_at_most(p.a.batch.seqs, token, [&](int i) { return static_cast<int64_t>(p.a.batch.starts[i]); });
-  const Segments seg = load_segments(p, b);
+  const Segments seg = load_segments<ROWS, TILE>(p, b);
   const int i = token - seg.seq.first;
   T* out = static_cast<T*>(p.a.out) + static_cast<int64_t>(token) * p.a.out_token + static_cast<int64_t>(q_head) * p.a.out_head;
   if (!seg.seq.ok) {
@@ -639,7 +752,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
   }
   if (i < 0 || i >= seg.seq.count) return;  // a row of no sequence
   int64_t front;
-  const int64_t total = count_units(p, b, &front);
+  const int64_t total = count_units<ROWS, TILE>(p, b, &front);
   const int64_t per = (total + p.workers - 1) / p.workers;
   const int head = q_head / p.group;
   const int packed = i * p.group + q_head % p.group;
@@ -651,11 +764,11 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
     }
     return;
   }
-  const int64_t u0 = front + (static_cast<int64_t>(head) * seg.row_tiles + packed / kTile) * tiles;
+  const int64_t u0 = front + (static_cast<int64_t>(head) * seg.row_tiles + packed / ROWS) * tiles;
   const int64_t first = u0 / per, last = (u0 + tiles - 1) / per;
   if (first == last) return;  // one worker had it all, and has written it
-  const int row = packed % kTile, dim = p.a.cache.dim;
-  auto slot_of = [&](int64_t c) { return (c * 2 + (c == first ? 1 : 0)) * kTile + row; };
+  const int row = packed % ROWS, dim = p.a.cache.dim;
+  auto slot_of = [&](int64_t c) { return (c * 2 + (c == first ? 1 : 0)) * ROWS + row; };
 
   float ref = -INFINITY, sum = 0.0f, y[kPer];
 #pragma unroll
@@ -723,12 +836,6 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
   }
 }
 
-template <int DP, bool F32>
-int64_t worker_count(int sms) {
-  using S = Shape<DP, F32>;
-  return static_cast<int64_t>(sms) * S::kCtas * S::kWarps;
-}
-
 constexpr int kMaxDevices = 64;
 
 int sm_count() {
@@ -754,45 +861,50 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[kMaxDevice
   return e;
 }
 
-template <int DP, bool F32>
-cudaError_t launch_shape(AttendDev& p, cudaStream_t stream) {
-  using S = Shape<DP, F32>;
+template <int DP, bool F32, int NR>
+cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
+  using S = Shape<DP, F32, NR>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-  const int sms = sm_count();
-  p.workers = worker_count<DP, F32>(sms);
+  const int sms = sm_count(), dim = p.a.cache.dim;
+  p.workers = static_cast<int64_t>(sms) * S::kCtas * S::kWarps;
+  if (bytes) {
+    *bytes = static_cast<size_t>(p.workers) * 2 * S::kRows * (dim + 2) * sizeof(float);
+    return cudaSuccess;
+  }
   p.part = static_cast<float*>(p.a.workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part + p.workers * 2 * kTile * p.a.cache.dim);
+  p.part_ml = reinterpret_cast<float2*>(p.part + p.workers * 2 * S::kRows * dim);
   constexpr int kSmem = S::kWarps * S::kWarpBytes;
-  static_assert(kSmem * S::kCtas <= 227 * 1024, "the CTAs of an SM share 227 KB");
   static std::atomic<bool> allowed[kMaxDevices];
-  cudaError_t e = allow_smem(attend_units<DP, F32>, kSmem, allowed);
+  cudaError_t e = allow_smem(attend_units<DP, F32, NR>, kSmem, allowed);
   if (e != cudaSuccess) return e;
   PdlLaunch launch(dim3(static_cast<unsigned>(sms * S::kCtas)), dim3(S::kWarps * 32), kSmem, stream);
-  e = launch(attend_units<DP, F32>, p);
+  e = launch(attend_units<DP, F32, NR>, p);
   if (e != cudaSuccess) return e;
   const int64_t rows = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
   // a row's partials are spread over eight warps where the rows alone would not fill the GPU
   if (rows <= 4 * sms) {
     PdlLaunch join(dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream);
-    return join(attend_join<T, DP, 8>, p);
+    return join(attend_join<T, DP, S::kRows, S::kTile, 8>, p);
   }
   PdlLaunch join(dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream);
-  return join(attend_join<T, DP, 1>, p);
+  return join(attend_join<T, DP, S::kRows, S::kTile, 1>, p);
 }
 
-}  // namespace
-
-size_t attend_workspace_bytes(int dim, int, int, int, int, int, uint8_t elem) {
-  const int sms = sm_count();
-  const bool f32 = elem == kF32;
-  const int64_t workers = dim <= 64    ? (f32 ? worker_count<64, true>(sms) : worker_count<64, false>(sms))
-                          : dim <= 128 ? (f32 ? worker_count<128, true>(sms) : worker_count<128, false>(sms))
-                                       : (f32 ? worker_count<256, true>(sms) : worker_count<256, false>(sms));
-  return static_cast<size_t>(workers) * 2 * kTile * (dim + 2) * sizeof(float);
+// Query rows of a segment: 8, 16 or 32, by the rows that a sequence's new
+// tokens and the group make.  Registers hold 16 at dims over 128 and in f32.
+template <int DP, bool F32>
+cudaError_t launch_rows_for(AttendDev& p, cudaStream_t stream, size_t* bytes) {
+  const int new_tokens = p.a.max_new > 0 && p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens;
+  const int64_t rows = static_cast<int64_t>(p.a.batch.tokens <= p.a.batch.seqs ? 1 : new_tokens) * p.group;
+  if (rows <= 8) return launch_shape<DP, F32, 1>(p, stream, bytes);
+  if constexpr (DP <= 128 && !F32) {
+    if (rows > 16) return launch_shape<DP, F32, 4>(p, stream, bytes);
+  }
+  return launch_shape<DP, F32, 2>(p, stream, bytes);
 }
 
-cudaError_t launch_cache_attention(const AttendArgs& a, cudaStream_t stream) {
-  if (a.batch.tokens <= 0 || a.batch.seqs <= 0 || a.q_heads <= 0) return cudaSuccess;
+// Launches, or tells the size of the workspace where ``bytes`` is given.
+cudaError_t launch_any(const AttendArgs& a, cudaStream_t stream, size_t* bytes) {
   AttendDev p{};
   p.a = a;
   p.group = a.q_heads / a.cache.heads;
@@ -801,10 +913,26 @@ cudaError_t launch_cache_attention(const AttendArgs& a, cudaStream_t stream) {
   p.group_div.set(static_cast<uint32_t>(p.group));
   const int dim = a.cache.dim;
   if (a.elem == kF32)
-    return dim <= 64 ? launch_shape<64, true>(p, stream)
-                     : dim <= 128 ? launch_shape<128, true>(p, stream) : launch_shape<256, true>(p, stream);
-  return dim <= 64 ? launch_shape<64, false>(p, stream)
-                   : dim <= 128 ? launch_shape<128, false>(p, stream) : launch_shape<256, false>(p, stream);
+    return dim <= 64    ? launch_rows_for<64, true>(p, stream, bytes)
+           : dim <= 128 ? launch_rows_for<128, true>(p, stream, bytes)
+                        : launch_rows_for<256, true>(p, stream, bytes);
+  return dim <= 64    ? launch_rows_for<64, false>(p, stream, bytes)
+         : dim <= 128 ? launch_rows_for<128, false>(p, stream, bytes)
+                      : launch_rows_for<256, false>(p, stream, bytes);
+}
+
+}  // namespace
+
+size_t attend_workspace_bytes(const AttendArgs& a) {
+  if (a.batch.tokens <= 0 || a.batch.seqs <= 0) return 0;
+  size_t bytes = 0;
+  launch_any(a, nullptr, &bytes);
+  return bytes;
+}
+
+cudaError_t launch_cache_attention(const AttendArgs& a, cudaStream_t stream) {
+  if (a.batch.tokens <= 0 || a.batch.seqs <= 0 || a.q_heads <= 0) return cudaSuccess;
+  return launch_any(a, stream, nullptr);
 }
 
 }  // namespace dev

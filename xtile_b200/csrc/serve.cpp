@@ -58,6 +58,11 @@ xt::dev::BatchView view(const xt_batch& b) {
   return {b.starts, b.lengths, b.table, b.seqs, b.tokens, b.table_width, b.table_stride};
 }
 
+xt::dev::AttendArgs attend_args(const xt_cache_attention_args& a, uint32_t* error_word) {
+  return {view(a.cache), view(a.batch), a.q, a.out, a.q_token, a.q_head, a.out_token, a.out_head, a.q_heads, a.max_new,
+          a.window, a.scale, a.softcap, code_of(a.elem), a.workspace, a.workspace_bytes, error_word};
+}
+
 int check_attention(const char* who, const xt_cache_attention_args* a) {
   if (!a) return bad(who, "null argument");
   if (int st = check_cache(who, a->cache)) return st;
@@ -140,8 +145,7 @@ int xt_cache_attention_workspace(const xt_cache_attention_args* a, size_t* out_b
   const char* who = "xt_cache_attention_workspace";
   if (!out_bytes) return bad(who, "null argument");
   if (int st = check_attention(who, a)) return st;
-  *out_bytes = xt::dev::attend_workspace_bytes(a->cache.dim, a->batch.seqs, a->batch.tokens, a->q_heads, a->cache.heads,
-                                               a->max_new, code_of(a->elem));
+  *out_bytes = xt::dev::attend_workspace_bytes(attend_args(*a, nullptr));
   return XT_OK;
 }
 
@@ -153,16 +157,12 @@ int xt_cache_attention(const xt_cache_attention_args* a, void* stream) {
   const int64_t bytes = 4 * size_of(a->elem);
   if (!aligned(a->q, bytes) || !aligned(a->out, bytes) || a->q_token % 4 || a->q_head % 4 || a->out_token % 4 || a->out_head % 4)
     return bad(who, "q and out must be aligned to four elements, and their strides multiples of four");
-  const size_t need = xt::dev::attend_workspace_bytes(a->cache.dim, a->batch.seqs, a->batch.tokens, a->q_heads,
-                                                      a->cache.heads, a->max_new, code_of(a->elem));
+  const size_t need = xt::dev::attend_workspace_bytes(attend_args(*a, nullptr));
   if (need > 0 && (!a->workspace || !aligned(a->workspace, 16) || a->workspace_bytes < need))
     return bad(who, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
   uint32_t* word = nullptr;
   if (int st = xt::device_error_word(&word)) return st;
-  xt::dev::AttendArgs p{view(a->cache), view(a->batch), a->q, a->out, a->q_token, a->q_head, a->out_token, a->out_head,
-                        a->q_heads, a->max_new, a->window, a->scale, a->softcap, code_of(a->elem),
-                        a->workspace, a->workspace_bytes, word};
-  return finish(who, xt::dev::launch_cache_attention(p, static_cast<cudaStream_t>(stream)));
+  return finish(who, xt::dev::launch_cache_attention(attend_args(*a, word), static_cast<cudaStream_t>(stream)));
 }
 
 int xt_dequantize(const int8_t* q, const float* scales, void* out, int64_t n, int64_t run, int elem, void* stream) {

@@ -114,7 +114,7 @@ struct AttendArgs {
   uint32_t* error_word;
 };
 // Bytes of device memory that launch_cache_attention needs beside its arguments.
-size_t attend_workspace_bytes(int dim, int seqs, int tokens, int q_heads, int kv_heads, int max_new, uint8_t elem);
+size_t attend_workspace_bytes(const AttendArgs& a);
 cudaError_t launch_cache_attention(const AttendArgs& a, cudaStream_t stream);
 
 // -------------------------------------------------------------- dequantize
