@@ -71,7 +71,7 @@ struct Shape {
 struct AttendDev {
   AttendArgs a;
   FastDiv page_div, block_div, group_div;
-  int group;
+  int group, blocks;  // query heads a kv head, blocks a page
   float* part;      // [workers][2][rows][dim] partial outputs
   float2* part_ml;  // [workers][2][rows] (reference, sum)
   int64_t workers;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       for (int i = 0; i < 2 * kTile / 32; ++i) {
         const int slot = i * 32 + lane, token = slot % kTile;
         const int row = page_row + (one_page ? token : 0);
-        const int64_t scale_at = line * (cache.page / cache.block) + p.block_div.quot(row);
+        const int64_t scale_at = line * p.blocks + p.block_div.quot(row);
         const uint32_t to = base + 2 * kTile * DP + slot * 4;
         const bool mine = token < there;
         if (mine && bad) {
@@ -366,8 +366,9 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   uint2 qf[S::kQueryInSmem ? 1 : NR][S::kQueryInSmem ? 1 : kSteps];
   float o[kOut][NR][4];
   // rows 2 t and 2 t + 1 of each n8 tile: reference of the exponents, sum of
-  // the weights, factor of the score, the score's start, position of the query
-  float ref[NR][2], sum[NR][2], row_scale[NR][2], start[NR][2];
+  // the weights, factor of the score in the exponent (1 behind a cap, whose own
+  // factor is capped_scale), the score's start, position of the query
+  float ref[NR][2], sum[NR][2], row_scale[NR][2], capped_scale[NR][2], start[NR][2];
   int row_pos[NR][2];
   int pos_min = 0, pos_max = 0;
   int value_exp = 0;                     // the weights carry vs 2^(10 - value_exp); set by the first token seen
@@ -443,7 +444,8 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       const float offset = F32 ? 0.0f : total_q * (-128.0f / 16777216.0f);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        row_scale[nr][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
+        capped_scale[nr][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
+        row_scale[nr][c] = cap > 0.0f ? 1.0f : capped_scale[nr][c];
         start[nr][c] = __shfl_sync(0xffffffffu, offset, (2 * t + c) * 4);
         row_pos[nr][c] = before + static_cast<int>(p.group_div.quot(at.row_tile * kRows + 8 * nr + 2 * t + c));
         ref[nr][c] = kNone;
@@ -549,10 +551,16 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          z[m][nr][e] *= e < 2 ? k0 : k1;
-          if (cap > 0.0f) z[m][nr][e] = tanhf(z[m][nr][e] * row_scale[nr][e & 1]) * (cap * kLog2e);
-        }
+        for (int e = 0; e < 4; ++e) z[m][nr][e] *= e < 2 ? k0 : k1;
+    }
+    if (cap > 0.0f) {
+#pragma unroll
+      for (int m = 0; m < kMTiles; ++m)
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            z[m][nr][e] = tanhf(z[m][nr][e] * capped_scale[nr][e & 1]) * (cap * kLog2e);
     }
     auto exponents = [&] {
       float top = -INFINITY;
@@ -562,8 +570,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float by = cap > 0.0f ? 1.0f : row_scale[nr][e & 1];
-            y[m][nr][e] = fmaf(z[m][nr][e], by, -ref[nr][e & 1]);
+            y[m][nr][e] = fmaf(z[m][nr][e], row_scale[nr][e & 1], -ref[nr][e & 1]);
             if (!open) {
               const int j = token0 + 16 * m + g + 8 * (e >> 1), pos = row_pos[nr][e & 1];
               if (j > pos || (p.a.window > 0 && j <= pos - p.a.window)) y[m][nr][e] = -INFINITY;
@@ -618,7 +625,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
           for (int m = 0; m < kMTiles; ++m) rise = fmaxf(rise, fmaxf(y[m][nr][c], y[m][nr][c + 2]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) rise = fmaxf(rise, __shfl_xor_sync(0xffffffffu, rise, x));
-          const float by = cap > 0.0f ? 1.0f : row_scale[nr][c];
+          const float by = row_scale[nr][c];
           float best = -INFINITY;
 #pragma unroll
           for (int m = 0; m < kMTiles; ++m) {
@@ -908,6 +915,7 @@ cudaError_t launch_any(const AttendArgs& a, cudaStream_t stream, size_t* bytes) 
   AttendDev p{};
   p.a = a;
   p.group = a.q_heads / a.cache.heads;
+  p.blocks = a.cache.page / a.cache.block;
   p.page_div.set(static_cast<uint32_t>(a.cache.page));
   p.block_div.set(static_cast<uint32_t>(a.cache.block));
   p.group_div.set(static_cast<uint32_t>(p.group));
