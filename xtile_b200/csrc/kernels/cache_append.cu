@@ -4,10 +4,13 @@
 //   s' = max(s, max|x| / 127)   (s: the block's scale, if it has earlier tokens)
 //   q  = rint(x / s');  the earlier tokens' rows become rint(q s / s') if s' > s.
 //
-// Bound by HBM for prompts (each new element read once, one byte written) and
-// by latency for single tokens.  One CTA has one block of one head, of the
-// keys or of the values: its new rows stay in registers between the largest
-// magnitude and the rounding.
+// Each new element is read once and one byte of it written, but what bounds a
+// prompt is instructions: about 20 an element pair for the rotation, the
+// largest magnitude and the rounding.  So a unit (one block of one head, of the
+// keys or of the values) belongs to as few lanes as hold it in registers
+// between the largest magnitude and the rounding, and what finds the block's
+// place is done once a warp: 17.5k tokens of 8 heads took 73 us with a CTA of
+// four warps a unit.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -21,44 +24,61 @@ namespace xt {
 namespace dev {
 namespace {
 
-// Items (two vectors of V elements) a thread holds in registers; blocks with
-// more are read a second time, from L2.
-constexpr int kHeld = 4;
+constexpr int kThreads = 256;
 
-// CTAs of a prompt's launch: sequence b's blocks start at slot
-// starts[b] / block + 2 b, which leaves room for every block that its tokens
-// can touch (at most count / block + 2), so that a slot finds its sequence by
-// a search in starts alone.
-struct Unit {
-  int seq, lo, first, last;  // block's first position; new positions [first, last)
-  bool mine;
+struct AppendDev {
+  AppendArgs a;
+  FastDiv items_div;      // items of a row: dim / (2 V)
+  int64_t warps;          // by units of a warp
+  int warps_a_slot;
+  bool by_token;
 };
 
-template <class T, int V, int THREADS>
-__global__ void __launch_bounds__(THREADS) cache_append_blocks(const AppendArgs a, bool by_token) {
-  __shared__ float part[THREADS / 32];
+// Slots of a launch: sequence b's blocks start at slot starts[b] / block + 2 b,
+// which leaves room for every block that its tokens can touch (at most count /
+// block + 2), so that a slot finds its sequence by a search in starts alone.
+// With few tokens each token has a slot (by_token), and the first new token of
+// a block does its block's work.
+//
+// LANES lanes (8, 32, or a CTA's 256) have a unit; a thread holds HELD items
+// (two vectors of V elements) of it in registers, and the rest of a longer
+// block is read a second time, from L2.
+template <class T, int V, int LANES, int HELD>
+__global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_constant__ AppendDev p) {
+  constexpr bool kCta = LANES == kThreads;
+  __shared__ float part[kThreads / 32];
   griddep_launch_dependents();
   griddep_wait();
+  const AppendArgs& a = p.a;
   const BatchView& bt = a.batch;
-  const int block = a.cache.block, page = a.cache.page, dim = a.cache.dim;
-  const int slot = blockIdx.x, head = blockIdx.y;
-  const bool keys = blockIdx.z == 0;
+  const int block = a.cache.block, page = a.cache.page, dim = a.cache.dim, heads = a.cache.heads;
+  const int64_t index = kCta ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (index >= p.warps) return;
+  const int64_t slot = index / p.warps_a_slot;
+  const int lane = threadIdx.x % LANES;
+  // the unit of its slot: keys' heads, then values'
+  const int unit = static_cast<int>(index - slot * p.warps_a_slot) * (kCta ? 1 : 32 / LANES) +
+                   (kCta ? 0 : (threadIdx.x & 31) / LANES);
+  const bool there = unit < 2 * heads;
+  const bool keys = unit < heads;
+  const int head = keys ? unit : there ? unit - heads : 0;
 
-  const int b = by_token
+  const int b = p.by_token
                     ? last_at_most(bt.seqs, slot, [&](int i) { return static_cast<int64_t>(bt.starts[i]); })
                     : last_at_most(bt.seqs, slot, [&](int i) { return bt.starts[i] / block + 2 * static_cast<int64_t>(i); });
   const Sequence s = load_sequence(bt, page, b);
   const int begin = s.length - s.count;
   if (!s.ok || begin < 0) {
-    if (threadIdx.x == 0) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrAppendTable));
+    if (lane == 0) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrAppendTable));
     return;
   }
   int lo;
-  if (by_token) {
-    const int i = slot - s.first;
+  if (p.by_token) {
+    const int64_t i = slot - s.first;
     if (i < 0 || i >= s.count) return;
-    if (i != 0 && (begin + i) % block != 0) return;  // the block's first new token has the CTA
-    lo = (begin + i) / block * block;
+    const int at = begin + static_cast<int>(i);
+    if (i != 0 && at % block != 0) return;  // the block's first new token has the work
+    lo = at / block * block;
   } else {
     const int64_t k = slot - (s.first / block + 2 * static_cast<int64_t>(b));
     const int64_t at = (begin / block + k) * block;
@@ -66,21 +86,17 @@ __global__ void __launch_bounds__(THREADS) cache_append_blocks(const AppendArgs 
     lo = static_cast<int>(at);
   }
   const int first = max(lo, begin), last = min(lo + block, s.length);
-  const int into = bt.table[b * bt.table_stride + lo / page];
-  if (into < 0 || into >= a.cache.pages) {
-    if (threadIdx.x == 0) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrAppendTable));
-    return;
-  }
+  const int into = bt.table[b * bt.table_stride + lo / page];  // checked once the new rows are on their way
 
   const int rot = keys && a.rope ? static_cast<int>(a.rot) : 0;
   const int64_t token_stride = keys ? a.k_token : a.v_token;
   const T* x = static_cast<const T*>(keys ? a.k : a.v) + head * (keys ? a.k_head : a.v_head) +
                (s.first + first - begin) * token_stride;
-  const int items = dim / (2 * V), work = (last - first) * items;
+  const int items = p.items_div.d, work = there ? (last - first) * items : 0;
 
   auto load = [&](int w, float (&u)[V], float (&v)[V]) {
-    const int row = w / items;
-    const RopeSpan span = rope_span<V>(w % items, rot, a.interleaved);
+    const int row = p.items_div.quot(w);
+    const RopeSpan span = rope_span<V>(w - row * items, rot, a.interleaved);
     Vec<T, V>::load(x + row * token_stride + span.first, u);
     Vec<T, V>::load(x + row * token_stride + span.second, v);
     if (span.pair < 0) return;
@@ -96,72 +112,76 @@ __global__ void __launch_bounds__(THREADS) cache_append_blocks(const AppendArgs 
     rope_item<V>(u, v, cs, a.interleaved);
   };
 
-  float u[kHeld][V], v[kHeld][V];
+  float u[HELD][V], v[HELD][V];
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const int w = i * THREADS + threadIdx.x;
+  for (int i = 0; i < HELD; ++i) {
+    const int w = i * LANES + lane;
     if (w >= work) continue;
     load(w, u[i], v[i]);
 #pragma unroll
     for (int j = 0; j < V; ++j) top = max_nan(top, max_nan(fabsf(u[i][j]), fabsf(v[i][j])));
   }
-  for (int w = kHeld * THREADS + threadIdx.x; w < work; w += THREADS) {
-    float p[V], q[V];
-    load(w, p, q);
+  if constexpr (kCta) {
+    for (int w = HELD * LANES + lane; w < work; w += LANES) {
+      float y[V], z[V];
+      load(w, y, z);
 #pragma unroll
-    for (int j = 0; j < V; ++j) top = max_nan(top, max_nan(fabsf(p[j]), fabsf(q[j])));
+      for (int j = 0; j < V; ++j) top = max_nan(top, max_nan(fabsf(y[j]), fabsf(z[j])));
+    }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (into < 0 || into >= a.cache.pages) {
+    if (lane == 0) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrAppendTable));
+    return;
+  }
   float* scale_at = (keys ? a.cache.k_scale : a.cache.v_scale) +
-                    (static_cast<int64_t>(into) * a.cache.heads + head) * (page / block) + lo % page / block;
-  const float was = first > lo ? *scale_at : 0.0f;  // read by every thread before the barrier, written behind it
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-  __syncthreads();
+                    (static_cast<int64_t>(into) * heads + head) * (page / block) + lo % page / block;
+  // read by every lane of the unit before the barrier, written behind it
+  const float was = there && first > lo ? *scale_at : 0.0f;
+  if constexpr (kCta) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) top = max_nan(top, part[i]);
+    for (int i = 0; i < kThreads / 32; ++i) top = max_nan(top, part[i]);
+  } else {
+    __syncwarp();
+  }
+  if (!there) return;
   float scale = quant_scale(top);
   if (first > lo) scale = max_nan(scale, was);
   const float inverse = quant_inverse(scale);
 
-  int8_t* rows = (keys ? a.cache.k : a.cache.v) +
-                 ((static_cast<int64_t>(into) * a.cache.heads + head) * page + lo % page) * dim;
+  int8_t* rows = (keys ? a.cache.k : a.cache.v) + ((static_cast<int64_t>(into) * heads + head) * page + lo % page) * dim;
+  if (lane == 0 && (first == lo || !(scale == was))) *scale_at = scale;
   if (scale > was && first > lo) {
-    if (threadIdx.x == 0) *scale_at = scale;
     const float ratio = was / scale;
-    for (int c = threadIdx.x; c < (first - lo) * (dim / 16); c += THREADS) {
+    for (int c = lane; c < (first - lo) * (dim / 16); c += LANES) {
       int4* at = reinterpret_cast<int4*>(rows) + c;
       int4 w = *at;
-      int* words = &w.x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int old = words[j];
-        words[j] = static_cast<int>(pack_i8(quantize(static_cast<float>(static_cast<int8_t>(old)), ratio),
-                                            quantize(static_cast<float>(static_cast<int8_t>(old >> 8)), ratio),
-                                            quantize(static_cast<float>(static_cast<int8_t>(old >> 16)), ratio),
-                                            quantize(static_cast<float>(static_cast<int8_t>(old >> 24)), ratio)));
-      }
+      w.x = requantize(w.x, ratio), w.y = requantize(w.y, ratio), w.z = requantize(w.z, ratio), w.w = requantize(w.w, ratio);
       *at = w;
     }
-  } else if (!(scale == was) || first == lo) {
-    if (threadIdx.x == 0) *scale_at = scale;  // a fresh block, or NaN
   }
-  auto store = [&](int w, const float (&p)[V], const float (&q)[V]) {
-    const RopeSpan span = rope_span<V>(w % items, rot, a.interleaved);
-    int8_t* to = rows + static_cast<int64_t>(first - lo + w / items) * dim;
-    store_i8<V>(to + span.first, p, inverse);
-    store_i8<V>(to + span.second, q, inverse);
+  auto store = [&](int w, const float (&y)[V], const float (&z)[V]) {
+    const int row = p.items_div.quot(w);
+    const RopeSpan span = rope_span<V>(w - row * items, rot, a.interleaved);
+    int8_t* to = rows + static_cast<int64_t>(first - lo + row) * dim;
+    store_i8<V>(to + span.first, y, inverse);
+    store_i8<V>(to + span.second, z, inverse);
   };
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const int w = i * THREADS + threadIdx.x;
+  for (int i = 0; i < HELD; ++i) {
+    const int w = i * LANES + lane;
     if (w < work) store(w, u[i], v[i]);
   }
-  for (int w = kHeld * THREADS + threadIdx.x; w < work; w += THREADS) {
-    float p[V], q[V];
-    load(w, p, q);
-    store(w, p, q);
+  if constexpr (kCta) {
+    for (int w = HELD * LANES + lane; w < work; w += LANES) {
+      float y[V], z[V];
+      load(w, y, z);
+      store(w, y, z);
+    }
   }
 }
 
@@ -169,15 +189,27 @@ template <class T, int V>
 cudaError_t launch_typed(const AppendArgs& a, cudaStream_t stream) {
   const BatchView& bt = a.batch;
   const int64_t by_block = bt.tokens / a.cache.block + 2 * static_cast<int64_t>(bt.seqs);
-  const bool by_token = bt.tokens <= by_block;
-  const dim3 grid(static_cast<unsigned>(by_token ? bt.tokens : by_block), static_cast<unsigned>(a.cache.heads), 2);
-  const int items = a.cache.block * (a.cache.dim / (2 * V));
-  if (items <= kHeld * 128) {
-    PdlLaunch launch(grid, dim3(128), 0, stream);
-    return launch(cache_append_blocks<T, V, 128>, a, by_token);
-  }
-  PdlLaunch launch(grid, dim3(512), 0, stream);
-  return launch(cache_append_blocks<T, V, 512>, a, by_token);
+  AppendDev p{};
+  p.a = a;
+  p.by_token = bt.tokens <= by_block;
+  const int row = a.cache.dim / (2 * V);
+  p.items_div.set(static_cast<uint32_t>(row));
+  const int64_t slots = p.by_token ? bt.tokens : by_block;
+  auto go = [&](auto kernel, int lanes) {
+    const bool cta = lanes == kThreads;
+    const int units_a_warp = cta ? 1 : 32 / lanes;
+    p.warps_a_slot = (2 * a.cache.heads + units_a_warp - 1) / units_a_warp;
+    p.warps = slots * p.warps_a_slot;
+    const int64_t ctas = cta ? p.warps : (p.warps + kThreads / 32 - 1) / (kThreads / 32);
+    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    PdlLaunch launch(dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, stream);
+    return launch(kernel, p);
+  };
+  // the fewest lanes that hold a whole block (4 items a lane: 64 bf16 elements)
+  const int64_t items = static_cast<int64_t>(a.cache.block) * row;
+  if (items <= 8) return go(cache_append_blocks<T, V, 8, 1>, 8);
+  if (items <= 128) return go(cache_append_blocks<T, V, 32, 4>, 32);
+  return go(cache_append_blocks<T, V, kThreads, 4>, kThreads);
 }
 
 }  // namespace

@@ -98,27 +98,40 @@ constexpr float kQuantTiny = 1e-36f;
 __device__ __forceinline__ float quant_scale(float top) { return top < kQuantTiny ? 0.0f : top * (1.0f / 127.0f); }
 __device__ __forceinline__ float quant_inverse(float scale) { return scale > 0.0f ? 1.0f / scale : 0.0f; }
 
-// x times the inverse scale, rounded to the nearest whole number (ties to
-// even) within +-127; NaN gives 0.
-__device__ __forceinline__ int quantize(float x, float inverse) {
-  const int q = __float2int_rn(x * inverse);
-  return min(max(q, -127), 127);
+// x * inverse rounded to the nearest whole number (ties to even) in the low
+// byte of a float's bits: 1.5 * 2^23 leaves no bits behind the point.  For
+// |x * inverse| < 2^22, so for any value under its block's scale; NaN gives
+// some byte (its scale is NaN).
+__device__ __forceinline__ uint32_t quantize_bits(float x, float inverse) {
+  return __float_as_uint(__fmaf_rn(x, inverse, 12582912.0f));
+}
+__device__ __forceinline__ int quantize(float x, float inverse) { return static_cast<int8_t>(quantize_bits(x, inverse)); }
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040u), __byte_perm(c, d, 0x0040u), 0x5410u);
 }
 
-__device__ __forceinline__ uint32_t pack_i8(int a, int b, int c, int d) {
-  return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
+// Four int8 values times ``ratio`` (at most 1), rounded again.
+__device__ __forceinline__ int requantize(int w, float ratio) {
+  auto value = [&](int shift) { return static_cast<float>(static_cast<int8_t>(w >> shift)); };
+  return static_cast<int>(low_bytes(quantize_bits(value(0), ratio), quantize_bits(value(8), ratio),
+                                    quantize_bits(value(16), ratio), quantize_bits(value(24), ratio)));
 }
 
 // V values as int8 at ``p`` (aligned to V bytes).
 template <int V>
 __device__ __forceinline__ void store_i8(int8_t* p, const float (&x)[V], float inverse) {
-  if constexpr (V == 8) {
-    *reinterpret_cast<uint2*>(p) =
-        make_uint2(pack_i8(quantize(x[0], inverse), quantize(x[1], inverse), quantize(x[2], inverse), quantize(x[3], inverse)),
-                   pack_i8(quantize(x[4], inverse), quantize(x[5], inverse), quantize(x[6], inverse), quantize(x[7], inverse)));
-  } else if constexpr (V == 4) {
-    *reinterpret_cast<uint32_t*>(p) =
-        pack_i8(quantize(x[0], inverse), quantize(x[1], inverse), quantize(x[2], inverse), quantize(x[3], inverse));
+  if constexpr (V >= 4) {
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      w[i] = low_bytes(quantize_bits(x[4 * i], inverse), quantize_bits(x[4 * i + 1], inverse),
+                       quantize_bits(x[4 * i + 2], inverse), quantize_bits(x[4 * i + 3], inverse));
+    if constexpr (V == 8)
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(p) = w[0];
   } else {
     *p = static_cast<int8_t>(quantize(x[0], inverse));
   }
