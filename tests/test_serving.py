@@ -88,7 +88,7 @@ CACHE_FAULTS = [
 
 @pytest.mark.parametrize("kw, word", CACHE_FAULTS + [
     (dict(elem=I8), "f32 or bf16"), (dict(rope=AT, rot=7), "rot"), (dict(rope=AT, rot=66), "rot"),
-    (dict(rope=AT, rot=0), "rot"), (dict(k_in=None), "null"),
+    (dict(rope=AT, rot=0), "rot"), (dict(rope=AT, rot=64), "no positions"), (dict(k_in=None), "null"),
 ])
 def test_cache_append_refuses(kw, word):
     kw = dict(kw)

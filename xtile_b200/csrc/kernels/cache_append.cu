@@ -28,9 +28,10 @@ constexpr int kThreads = 256;
 
 struct AppendDev {
   AppendArgs a;
-  FastDiv items_div;      // items of a row: dim / (2 V)
-  int64_t warps;          // by units of a warp
-  int warps_a_slot;
+  FastDiv items_div;      // by the items of a row: dim / (2 V)
+  FastDiv slot_div;       // by the warps (CTAs) of a slot
+  FastDiv block_div, page_div;
+  int warps, page_blocks;
   bool by_token;
 };
 
@@ -52,12 +53,12 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
   const AppendArgs& a = p.a;
   const BatchView& bt = a.batch;
   const int block = a.cache.block, page = a.cache.page, dim = a.cache.dim, heads = a.cache.heads;
-  const int64_t index = kCta ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int index = kCta ? blockIdx.x : blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (index >= p.warps) return;
-  const int64_t slot = index / p.warps_a_slot;
+  const int slot = p.slot_div.quot(index);
   const int lane = threadIdx.x % LANES;
   // the unit of its slot: keys' heads, then values'
-  const int unit = static_cast<int>(index - slot * p.warps_a_slot) * (kCta ? 1 : 32 / LANES) +
+  const int unit = (index - slot * static_cast<int>(p.slot_div.d)) * (kCta ? 1 : 32 / LANES) +
                    (kCta ? 0 : (threadIdx.x & 31) / LANES);
   const bool there = unit < 2 * heads;
   const bool keys = unit < heads;
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
 
   const int b = p.by_token
                     ? last_at_most(bt.seqs, slot, [&](int i) { return static_cast<int64_t>(bt.starts[i]); })
-                    : last_at_most(bt.seqs, slot, [&](int i) { return bt.starts[i] / block + 2 * static_cast<int64_t>(i); });
+                    : last_at_most(bt.seqs, slot, [&](int i) { return p.block_div.quot(bt.starts[i]) + 2 * static_cast<int64_t>(i); });
   const Sequence s = load_sequence(bt, page, b);
   const int begin = s.length - s.count;
   if (!s.ok || begin < 0) {
@@ -74,58 +75,97 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
   }
   int lo;
   if (p.by_token) {
-    const int64_t i = slot - s.first;
+    const int i = slot - s.first, at = begin + i;
     if (i < 0 || i >= s.count) return;
-    const int at = begin + static_cast<int>(i);
-    if (i != 0 && at % block != 0) return;  // the block's first new token has the work
-    lo = at / block * block;
+    lo = p.block_div.quot(at) * block;
+    if (i != 0 && at != lo) return;  // the block's first new token has the work
   } else {
-    const int64_t k = slot - (s.first / block + 2 * static_cast<int64_t>(b));
-    const int64_t at = (begin / block + k) * block;
+    const int64_t k = slot - (p.block_div.quot(s.first) + 2 * static_cast<int64_t>(b));
+    const int64_t at = (p.block_div.quot(begin) + k) * block;
     if (s.count == 0 || k < 0 || at >= s.length) return;
     lo = static_cast<int>(at);
   }
   const int first = max(lo, begin), last = min(lo + block, s.length);
-  const int into = bt.table[b * bt.table_stride + lo / page];  // checked once the new rows are on their way
+  const int page_at = p.page_div.quot(lo), row_at = lo - page_at * page;
+  const int into = bt.table[b * bt.table_stride + page_at];  // checked once the new rows are on their way
 
   const int rot = keys && a.rope ? static_cast<int>(a.rot) : 0;
   const int64_t token_stride = keys ? a.k_token : a.v_token;
   const T* x = static_cast<const T*>(keys ? a.k : a.v) + head * (keys ? a.k_head : a.v_head) +
                (s.first + first - begin) * token_stride;
-  const int items = p.items_div.d, work = there ? (last - first) * items : 0;
+  const int items = p.items_div.d, new_rows = last - first, work = new_rows * items;
 
-  auto load = [&](int w, float (&u)[V], float (&v)[V]) {
-    const int row = p.items_div.quot(w);
-    const RopeSpan span = rope_span<V>(w - row * items, rot, a.interleaved);
-    Vec<T, V>::load(x + row * token_stride + span.first, u);
-    Vec<T, V>::load(x + row * token_stride + span.second, v);
-    if (span.pair < 0) return;
-    float2 cs[V];
-    const int pos = first + row;
-    if (pos < a.rope_rows) {
-      load_turns<V>(a.rope + static_cast<int64_t>(pos) * (rot / 2) + span.pair, cs);
-    } else {
-      atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrRopePosition));
-#pragma unroll
-      for (int j = 0; j < V; ++j) cs[j] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
-    }
-    rope_item<V>(u, v, cs, a.interleaved);
+  // Loads come without a branch, from the last item again behind the end, so
+  // that all of a thread's are under way before the first is waited for (the
+  // keys' in one chain of an item after another made a prompt 55 us).
+  struct Item {
+    int row;  // at or behind new_rows: none
+    RopeSpan span;
   };
+  const int row0 = p.items_div.quot(lane), item0 = lane - row0 * items;
+  const int row_step = p.items_div.quot(LANES), item_step = LANES - row_step * items;
+  auto item_at = [&](int i) {  // item i * LANES + lane
+    int row = row0 + i * row_step, at = item0 + i * item_step;
+    if (item_step) {
+      const int carry = p.items_div.quot(at);
+      row += carry;
+      at -= carry * items;
+    }
+    return Item{row, rope_span<V>(at, rot, a.interleaved)};
+  };
+  auto fetch = [&](const Item& it, float (&u)[V], float (&v)[V]) {
+    const T* from = x + min(it.row, new_rows - 1) * token_stride;
+    Vec<T, V>::load(from + it.span.first, u);
+    Vec<T, V>::load(from + it.span.second, v);
+  };
+  auto fetch_turns = [&](const Item& it, float2 (&cs)[V]) {
+    const int64_t pos = min(static_cast<int64_t>(first + min(it.row, new_rows - 1)), a.rope_rows - 1);
+    load_turns<V>(a.rope + pos * (rot / 2) + max(it.span.pair, 0), cs);
+  };
+  auto rotate = [&](const Item& it, float (&u)[V], float (&v)[V], const float2 (&cs)[V]) {
+    if (it.span.pair >= 0) rope_item<V>(u, v, cs, a.interleaved);
+  };
+  auto load = [&](const Item& it, float (&u)[V], float (&v)[V]) {
+    fetch(it, u, v);
+    if (rot) {
+      float2 cs[V];
+      fetch_turns(it, cs);
+      rotate(it, u, v, cs);
+    }
+  };
+  const bool off_table = rot && last > a.rope_rows;  // its scale is NaN, then
 
   float u[HELD][V], v[HELD][V];
+  if (HELD > 1 && work <= LANES) {  // single tokens: one item a lane
+    load(item_at(0), u[0], v[0]);
+#pragma unroll
+    for (int i = 1; i < HELD; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) u[i][j] = v[i][j] = 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) fetch(item_at(i), u[i], v[i]);
+    if (rot) {
+      constexpr int kAtOnce = HELD < 2 ? 1 : 2;  // items whose turns registers hold
+#pragma unroll
+      for (int i = 0; i < HELD; i += kAtOnce) {
+        float2 cs[kAtOnce][V];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) fetch_turns(item_at(i + k), cs[k]);
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) rotate(item_at(i + k), u[i + k], v[i + k], cs[k]);
+      }
+    }
+  }
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    const int w = i * LANES + lane;
-    if (w >= work) continue;
-    load(w, u[i], v[i]);
+  for (int i = 0; i < HELD; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) top = max_nan(top, max_nan(fabsf(u[i][j]), fabsf(v[i][j])));
-  }
   if constexpr (kCta) {
-    for (int w = HELD * LANES + lane; w < work; w += LANES) {
+    for (int i = HELD; i * LANES < work; ++i) {
       float y[V], z[V];
-      load(w, y, z);
+      load(item_at(i), y, z);
 #pragma unroll
       for (int j = 0; j < V; ++j) top = max_nan(top, max_nan(fabsf(y[j]), fabsf(z[j])));
     }
@@ -137,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
     return;
   }
   float* scale_at = (keys ? a.cache.k_scale : a.cache.v_scale) +
-                    (static_cast<int64_t>(into) * heads + head) * (page / block) + lo % page / block;
+                    (static_cast<int64_t>(into) * heads + head) * p.page_blocks + p.block_div.quot(row_at);
   // read by every lane of the unit before the barrier, written behind it
   const float was = there && first > lo ? *scale_at : 0.0f;
   if constexpr (kCta) {
@@ -149,11 +189,15 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
     __syncwarp();
   }
   if (!there) return;
+  if (off_table) {
+    if (lane == 0) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrRopePosition));
+    top = __int_as_float(0x7fc00000);
+  }
   float scale = quant_scale(top);
   if (first > lo) scale = max_nan(scale, was);
   const float inverse = quant_inverse(scale);
 
-  int8_t* rows = (keys ? a.cache.k : a.cache.v) + ((static_cast<int64_t>(into) * heads + head) * page + lo % page) * dim;
+  int8_t* rows = (keys ? a.cache.k : a.cache.v) + ((static_cast<int64_t>(into) * heads + head) * page + row_at) * dim;
   if (lane == 0 && (first == lo || !(scale == was))) *scale_at = scale;
   if (scale > was && first > lo) {
     const float ratio = was / scale;
@@ -164,23 +208,19 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
       *at = w;
     }
   }
-  auto store = [&](int w, const float (&y)[V], const float (&z)[V]) {
-    const int row = p.items_div.quot(w);
-    const RopeSpan span = rope_span<V>(w - row * items, rot, a.interleaved);
-    int8_t* to = rows + static_cast<int64_t>(first - lo + row) * dim;
-    store_i8<V>(to + span.first, y, inverse);
-    store_i8<V>(to + span.second, z, inverse);
+  auto store = [&](const Item& it, const float (&y)[V], const float (&z)[V]) {
+    if (it.row >= new_rows) return;
+    int8_t* to = rows + static_cast<int64_t>(first - lo + it.row) * dim;
+    store_i8<V>(to + it.span.first, y, inverse);
+    store_i8<V>(to + it.span.second, z, inverse);
   };
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    const int w = i * LANES + lane;
-    if (w < work) store(w, u[i], v[i]);
-  }
+  for (int i = 0; i < HELD; ++i) store(item_at(i), u[i], v[i]);
   if constexpr (kCta) {
-    for (int w = HELD * LANES + lane; w < work; w += LANES) {
+    for (int i = HELD; i * LANES < work; ++i) {
       float y[V], z[V];
-      load(w, y, z);
-      store(w, y, z);
+      load(item_at(i), y, z);
+      store(item_at(i), y, z);
     }
   }
 }
@@ -194,14 +234,19 @@ cudaError_t launch_typed(const AppendArgs& a, cudaStream_t stream) {
   p.by_token = bt.tokens <= by_block;
   const int row = a.cache.dim / (2 * V);
   p.items_div.set(static_cast<uint32_t>(row));
+  p.block_div.set(static_cast<uint32_t>(a.cache.block));
+  p.page_div.set(static_cast<uint32_t>(a.cache.page));
+  p.page_blocks = a.cache.page / a.cache.block;
   const int64_t slots = p.by_token ? bt.tokens : by_block;
   auto go = [&](auto kernel, int lanes) {
     const bool cta = lanes == kThreads;
     const int units_a_warp = cta ? 1 : 32 / lanes;
-    p.warps_a_slot = (2 * a.cache.heads + units_a_warp - 1) / units_a_warp;
-    p.warps = slots * p.warps_a_slot;
-    const int64_t ctas = cta ? p.warps : (p.warps + kThreads / 32 - 1) / (kThreads / 32);
-    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    const int64_t a_slot = (2 * static_cast<int64_t>(a.cache.heads) + units_a_warp - 1) / units_a_warp;
+    const int64_t warps = slots * a_slot;
+    if (warps > 0x7fffff00) return cudaErrorInvalidValue;
+    p.slot_div.set(static_cast<uint32_t>(a_slot));
+    p.warps = static_cast<int>(warps);
+    const int64_t ctas = cta ? warps : (warps + kThreads / 32 - 1) / (kThreads / 32);
     PdlLaunch launch(dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, stream);
     return launch(kernel, p);
   };

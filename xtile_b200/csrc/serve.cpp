@@ -129,6 +129,7 @@ int xt_cache_append(const xt_cache_append_args* a, void* stream) {
   if (int st = check_batch(who, a->batch, a->cache.page)) return st;
   if (!is_float(a->elem)) return bad(who, "k and v must be f32 or bf16");
   if (a->rope && (a->rot < 2 || a->rot % 2 || a->rot > a->cache.dim)) return bad(who, "rot must be even, positive and at most dim");
+  if (a->rope && a->rope_rows < 1) return bad(who, "the rotation table has no positions");
   if (a->batch.tokens == 0 || a->batch.seqs == 0) return XT_OK;
   if (!a->k || !a->v) return bad(who, "null array");
   if (!aligned(a->k, size_of(a->elem)) || !aligned(a->v, size_of(a->elem)) || !aligned(a->rope, 8))
