@@ -34,9 +34,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
-
 #include "../serve.h"
+#include "attend.cuh"
 #include "batch.cuh"
 #include "pdl.cuh"
 #include "vec.cuh"
@@ -44,9 +43,6 @@
 namespace xt {
 namespace dev {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNone = -1e30f;  // reference of a row that has seen no token
 
 // How one instance of the kernel is laid out.  DP: dims, padded; NR: n8 tiles
 // of query rows.
@@ -66,15 +62,6 @@ struct Shape {
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static_assert(kStages >= 3, "a warp's ring holds three stages at least");
   static constexpr int kWarpBytes = kStages * kStageBytes + kQueryBytes;
-};
-
-struct AttendDev {
-  AttendArgs a;
-  FastDiv page_div, block_div, group_div;
-  int group, blocks;  // query heads a kv head, blocks a page
-  float* part;      // [workers][2][rows][dim] partial outputs
-  float2* part_ml;  // [workers][2][rows] (reference, sum)
-  int64_t workers;
 };
 
 // The units of sequence b: kv heads x row tiles x token tiles [lo, hi).
@@ -198,30 +185,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-
-// 2^x, at most 2^-22 of it off; 0 for -inf.
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// Two biased bytes (int8 + 128), picked by ``sel`` from w, as f16 values: the
-// byte lands in the mantissa of 1024, and 1152 is taken off again, exactly.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t biased) {
-  const uint32_t h = __byte_perm(biased, 0x64646464u, SEL);
-  const uint32_t off = 0x64806480u;
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&off));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-constexpr uint32_t kLow = 0x4140u, kHigh = 0x4342u;  // bytes 0, 1 and bytes 2, 3
-
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_half2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
 // What two values leave after their rounding to f16, as f16.
 __device__ __forceinline__ uint32_t rest_half2(float lo, float hi, uint32_t rounded) {
@@ -843,8 +806,6 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
   }
 }
 
-constexpr int kMaxDevices = 64;
-
 int sm_count() {
   static std::atomic<int> known[kMaxDevices];
   int device = 0, sms = 148;
@@ -854,18 +815,6 @@ int sm_count() {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (keep) known[device] = sms;
   return sms;
-}
-
-// Grants ``kernel`` its shared memory, once a device.
-template <class K>
-cudaError_t allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[kMaxDevices]) {
-  int device = 0;
-  cudaGetDevice(&device);
-  const bool keep = device >= 0 && device < kMaxDevices;
-  if (keep && done[device]) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && keep) done[device] = true;
-  return e;
 }
 
 template <int DP, bool F32, int NR>
@@ -897,12 +846,24 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   return join(attend_join<T, DP, S::kRows, S::kTile, 1>, p);
 }
 
+// New tokens of a sequence, as far as the caller knows; else their mean.
+int new_tokens(const AttendDev& p) {
+  const int mean = (p.a.batch.tokens + p.a.batch.seqs - 1) / p.a.batch.seqs;
+  return p.a.max_new > 0 ? (p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens) : mean;
+}
+
+// Whether the tcgen05 kernel for many query rows runs the call.
+bool for_prompt(const AttendDev& p) {
+  const int64_t rows = static_cast<int64_t>(new_tokens(p)) * p.group;
+  const int64_t ctas = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads / 256;
+  return p.a.elem == kBF16 && p.a.cache.dim <= 128 && rows >= 128 && ctas >= 1;
+}
+
 // Query rows of a segment: 8, 16 or 32, by the rows that a sequence's new
 // tokens and the group make.  Registers hold 16 at dims over 128 and in f32.
 template <int DP, bool F32>
 cudaError_t launch_rows_for(AttendDev& p, cudaStream_t stream, size_t* bytes) {
-  const int new_tokens = p.a.max_new > 0 && p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens;
-  const int64_t rows = static_cast<int64_t>(p.a.batch.tokens <= p.a.batch.seqs ? 1 : new_tokens) * p.group;
+  const int64_t rows = static_cast<int64_t>(new_tokens(p)) * p.group;
   if (rows <= 8) return launch_shape<DP, F32, 1>(p, stream, bytes);
   if constexpr (DP <= 128 && !F32) {
     if (rows > 16) return launch_shape<DP, F32, 4>(p, stream, bytes);
@@ -920,6 +881,11 @@ cudaError_t launch_any(const AttendArgs& a, cudaStream_t stream, size_t* bytes) 
   p.block_div.set(static_cast<uint32_t>(a.cache.block));
   p.group_div.set(static_cast<uint32_t>(p.group));
   const int dim = a.cache.dim;
+  if (for_prompt(p)) {
+    if (!bytes) return launch_attend_prompt(p, stream);
+    *bytes = 0;
+    return cudaSuccess;
+  }
   if (a.elem == kF32)
     return dim <= 64    ? launch_rows_for<64, true>(p, stream, bytes)
            : dim <= 128 ? launch_rows_for<128, true>(p, stream, bytes)
