@@ -8,17 +8,20 @@
 //
 //   warps 0-3, 4-7   softmax of query tile 0 and 1, one row a thread: scores
 //                    from TMEM, weights as f16 back to TMEM over the scores'
-//                    columns; they also divide and store the result
+//                    columns; they also divide and store the result.  Warps 0
+//                    and 4 issue their tile's tcgen05.mma: S = Q K^T (both in
+//                    shared memory) and O += P V (P in TMEM, V read N-major)
 //   warps 8-11       load the int8 rows, turn them into f16 in shared memory
 //                    (128-byte swizzle), two stages each of keys and values
-//   warp 12          issues tcgen05.mma: S = Q K^T (both in shared memory) and
-//                    O += P V (P in TMEM, V read N-major), M = 128
 //
 // While one query tile's softmax runs, the tensor cores work for the other.
 // The scores of the next token tile go to the same columns as the weights that
 // the product before it reads: the MMAs of one thread execute in order.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <climits>
+#include <type_traits>
 
 #include "attend.cuh"
 #include "batch.cuh"
@@ -34,9 +37,9 @@ using namespace sm100;
 
 constexpr int kTokens = 128;  // tokens of a tile
 constexpr int kTileRows = 128, kRows = 2 * kTileRows;
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 12 * 32;
 constexpr int kScaleSlots = 4;
-enum : uint32_t { kErrSoftmaxWait = 0x304, kErrConvertWait = 0x305, kErrMmaWait = 0x306 };
+enum : uint32_t { kErrSoftmaxWait = 0x304, kErrConvertWait = 0x305 };
 
 template <int DP>
 struct Layout {
@@ -52,9 +55,8 @@ struct Layout {
 
 struct Bars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_ready[2], q_ready[2], o_full[2];
+  uint64_t s_full[2], o_full[2], drain[2];
   uint64_t scales_full[kScaleSlots];
-  uint64_t drain;
   float most[kScaleSlots][4];  // largest value scale of a tile, a converting warp each
   uint32_t tmem;
   int abort;
@@ -76,6 +78,11 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
@@ -121,7 +128,7 @@ struct Work {
   int lo, hi;
 };
 
-template <int DP>
+template <int DP, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_constant__ AttendDev p, int slots) {
   using L = Layout<DP>;
   extern __shared__ uint8_t smem_raw[];
@@ -175,20 +182,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.k_full[i], 128);
-      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.k_empty[i], queries);
       mbar_init(&bars.v_full[i], 128);
-      mbar_init(&bars.v_empty[i], 1);
+      mbar_init(&bars.v_empty[i], queries);
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_ready[i], 128);
-      mbar_init(&bars.q_ready[i], 128);
       mbar_init(&bars.o_full[i], 1);
+      mbar_init(&bars.drain[i], 1);
     }
     for (int i = 0; i < kScaleSlots; ++i) mbar_init(&bars.scales_full[i], 128);
-    mbar_init(&bars.drain, 1);
     bars.abort = 0;
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 11) {
     tmem_alloc(&bars.tmem, 512);
     tmem_relinquish();
   }
@@ -246,199 +251,253 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
               make_uint4(h[0], h[1], h[2], h[3]);
         }
         fence_proxy_async_smem();
-        mbar_arrive(&bars.q_ready[w]);
       }
 
-      const uint32_t scores = score_at(w) + quarter, output = out_at(w) + quarter;
+      // --- the tile's products, issued by its first warp
+      constexpr uint32_t kScoreDesc = instr_desc(1, 0, 0, 0, 0, 128, kTokens);
+      constexpr uint32_t kOutDesc = instr_desc(1, 0, 0, 0, 1, 128, DP);
+      const uint32_t base = smem_addr(smem);
+      auto score = [&](int j) {  // S = Q K^T of token tile j; false: a wait gave up
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.k_full[j & 1], (j >> 1) & 1, ab, kErrSoftmaxWait))) return false;
+        tc_fence_after();
+        if (elect_sync()) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint64_t q = smem_desc_sw128(base + L::kQuery + w * L::kMatrix + k / 4 * L::kHalf, 16, 1024) + (k & 3) * 2;
+            const uint64_t c =
+                smem_desc_sw128(base + L::kKeys + (j & 1) * L::kMatrix + k / 4 * L::kHalf, 16, 1024) + (k & 3) * 2;
+            umma_bf16(score_at(w), q, c, kScoreDesc, k != 0);
+          }
+          umma_commit(&bars.s_full[w]);
+          umma_commit(&bars.k_empty[j & 1]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto output = [&](int j) {  // O += P V of token tile j
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.v_full[j & 1], (j >> 1) & 1, ab, kErrSoftmaxWait))) return false;
+        tc_fence_after();
+        if (elect_sync()) {
+          const uint64_t c = smem_desc_sw128(base + L::kValues + (j & 1) * L::kMatrix, L::kHalf, 1024);
+#pragma unroll
+          for (int k = 0; k < kTokens / 16; ++k)
+            umma_f16_ts(out_at(w), score_at(w) + k * 8, c + k * 128, kOutDesc, (j | k) != 0);
+          umma_commit(&bars.v_empty[j & 1]);
+          if (j + 1 == tiles) umma_commit(&bars.o_full[w]);
+        }
+        __syncwarp();
+        return true;
+      };
+      const bool issuer = (warp & 3) == 0;
+      auto meet = [&] {  // the tile's four warps
+        tc_fence_before();
+        named_barrier_sync(1 + w, 128);
+        tc_fence_after();
+      };
+
+      const uint32_t scores = score_at(w) + quarter, result = out_at(w) + quarter;
       const float factor = cap > 0.0f ? 1.0f : row_scale;
-      float ref = kNone, shift = 1.0f;
-      int value_exp = 0;
+      // Weights are 2^(score - ref + up): ``up`` (10 - the exponent of the
+      // values' scales, within -60 .. 100) brings weight * value scale near 2^10
+      // in f16; the sum carries it too, which takes it out of the result again.
+      float ref = kNone, up = 0.0f, value_limit = 0.0f;
       bool value_set = false, ok = true;
       uint64_t sum = pack2(0.0f, 0.0f);
       const int pos_min = __shfl_sync(0xffffffffu, pos, 0);  // of the warp's rows
       const int pos_max = __shfl_sync(0xffffffffu, pos, 31);
+      const int window = p.a.window > 0 ? p.a.window : INT_MAX;
+      const float *key_scales = nullptr, *value_scales = nullptr;
+      int token0 = 0;
 
-      for (int j = 0; j < tiles; ++j) {
-        ok = mbar_wait_warp(&bars.s_full[w], j & 1, ab, kErrSoftmaxWait) &&
-             mbar_wait_warp(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, ab, kErrSoftmaxWait);
-        if (!ok) break;
-        tc_fence_after();
-        const float* key_scales = reinterpret_cast<const float*>(smem + L::kScales) + (j % kScaleSlots) * 2 * kTokens;
-        const float* value_scales = key_scales + kTokens;
-        const float* most4 = bars.most[j % kScaleSlots];
-        const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
-        const int token0 = (work.lo + j) * kTokens;
-        // every row of the warp sees all of the tile's tokens
-        const bool open = token0 + kTokens - 1 <= pos_min && (p.a.window == 0 || token0 > pos_max - p.a.window);
-
+      // Chunk c (32 tokens) of a tile: scores from TMEM, weights to TMEM.
+      auto chunk = [&](auto is_open, int j, int c, float most) {
+        constexpr bool kOpen = decltype(is_open)::value;
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(scores + c * 32, r);
+        tmem_wait_ld();
+        const float4* ks = reinterpret_cast<const float4*>(key_scales + c * 32);
+        const float4* vs = reinterpret_cast<const float4*>(value_scales + c * 32);
+        uint64_t y[16];
+        float less = up - ref;
+        // The reference follows a row's maximum only when that has risen by
+        // more than 2^4, and the values' exponent only when a weight could
+        // leave f16's range, so the first turn is mostly the only one; the
+        // second takes the scores themselves.
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(scores + c * 32, r);
-          tmem_wait_ld();
-          const float4* ks = reinterpret_cast<const float4*>(key_scales + c * 32);
-          const float4* vs = reinterpret_cast<const float4*>(value_scales + c * 32);
-          uint64_t z[16];
+        for (int turn = 0;; ++turn) {
+          const uint64_t by = pack2(factor, factor), add = pack2(less, less);
+          float top = -INFINITY;
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             const float4 k = ks[x];
-            z[2 * x] = mul2(pack2(__uint_as_float(r[4 * x]), __uint_as_float(r[4 * x + 1])), pack2(k.x, k.y));
-            z[2 * x + 1] = mul2(pack2(__uint_as_float(r[4 * x + 2]), __uint_as_float(r[4 * x + 3])), pack2(k.z, k.w));
-          }
-          if (cap > 0.0f) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              float a, b;
-              unpack2(z[x], a, b);
-              z[x] = pack2(tanhf(a * row_scale) * (cap * kLog2e), tanhf(b * row_scale) * (cap * kLog2e));
-            }
-          }
-          float top = -INFINITY;
-          uint64_t y[16];
-          auto exponents = [&] {
-            const uint64_t by = pack2(factor, factor), less = pack2(-ref, -ref);
-            top = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              y[x] = fma2(z[x], by, less);
-              float a, b;
-              unpack2(y[x], a, b);
-              if (!open) {
-                const int t0 = token0 + c * 32 + 2 * x;
-                if (t0 > pos || (p.a.window > 0 && t0 <= pos - p.a.window)) a = -INFINITY;
-                if (t0 + 1 > pos || (p.a.window > 0 && t0 + 1 <= pos - p.a.window)) b = -INFINITY;
-                y[x] = pack2(a, b);
-              }
-              top = fmaxf(top, fmaxf(a, b));
-            }
-          };
-          exponents();
-          // as in attend.cu: the reference and the values' exponent move rarely
-          if (__any_sync(0xffffffffu, top > 4.0f || most * shift > 2048.0f || !value_set)) {
-            float best = -INFINITY;
-            int e = 0;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              float a, b, ya, yb;
-              unpack2(z[x], a, b);
-              unpack2(y[x], ya, yb);
-              const float2 v = reinterpret_cast<const float2*>(vs)[x];
-              const int ea = static_cast<int>(__float_as_uint(v.x) >> 23 & 255);
-              const int eb = static_cast<int>(__float_as_uint(v.y) >> 23 & 255);
-              if (ya > -INFINITY) best = fmaxf(best, a * factor), e = max(e, ea < 255 ? ea : 0);
-              if (yb > -INFINITY) best = fmaxf(best, b * factor), e = max(e, eb < 255 ? eb : 0);
-            }
-            float f = 1.0f, fall = 1.0f;
-            if (best > ref) {
-              f = exp2_fast(ref - best);
-              ref = best;
-            }
-            if (e > 0) {
-              e = min(max(e, 11), 250) - 127;
-              if (!value_set) {
-                value_exp = e;
-              } else if (e > value_exp) {
-                fall = __uint_as_float(static_cast<uint32_t>(max(127 + value_exp - e, 0)) << 23);
-                value_exp = e;
-              }
-              value_set = true;
-              shift = __uint_as_float(static_cast<uint32_t>(137 - value_exp) << 23);
-            }
-            sum = mul2(sum, pack2(f, f));
-            f *= fall;
-            if (__any_sync(0xffffffffu, f != 1.0f)) {
-              // the output so far (S being there, the product before it is done), and this tile's weights so far
-              if (j > 0) {
-#pragma unroll 1
-                for (int d = 0; d < DP; d += 32) {
-                  uint32_t o[32];
-                  tmem_ld_32x32b_x32(output + d, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                  uint32_t half[16];
-#pragma unroll
-                  for (int x = 0; x < 16; ++x) half[x] = o[x];
-                  tmem_st_x16(output + d, half);
-#pragma unroll
-                  for (int x = 0; x < 16; ++x) half[x] = o[16 + x];
-                  tmem_st_x16(output + d + 16, half);
-                }
-              }
-#pragma unroll 1
-              for (int d = 0; d < c; ++d) {
-                uint32_t h[16];
-                tmem_wait_st();
-                tmem_ld_x16(scores + d * 16, h);
-                tmem_wait_ld();
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                  const float2 v = unpack_half2(h[x]);
-                  h[x] = pack_half2(v.x * f, v.y * f);
-                }
-                tmem_st_x16(scores + d * 16, h);
-              }
-            }
-            exponents();
-          }
-          uint32_t weights[16];
-          const uint64_t shift2 = pack2(shift, shift);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const float4 v = vs[x];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float a, b;
-              unpack2(y[2 * x + h], a, b);
-              const float ea = exp2_fast(a), eb = exp2_fast(b);
-              const uint64_t e2 = pack2(ea, eb);
-              sum = add2(sum, e2);
-              float wa, wb;
-              unpack2(mul2(e2, mul2(h ? pack2(v.z, v.w) : pack2(v.x, v.y), shift2)), wa, wb);
-              if (!open) {  // a token that is not seen may have any scale
-                if (a == -INFINITY) wa = 0.0f;
-                if (b == -INFINITY) wb = 0.0f;
+              uint64_t z = mul2(pack2(__uint_as_float(r[4 * x + 2 * h]), __uint_as_float(r[4 * x + 2 * h + 1])),
+                                h ? pack2(k.z, k.w) : pack2(k.x, k.y));
+              if constexpr (CAP) {
+                float a, b;
+                unpack2(z, a, b);
+                z = pack2(tanhf(a * row_scale) * (cap * kLog2e), tanhf(b * row_scale) * (cap * kLog2e));
               }
-              weights[2 * x + h] = pack_half2(wa, wb);
+              z = fma2(z, by, add);
+              float a, b;
+              unpack2(z, a, b);
+              if constexpr (!kOpen) {
+                const int back = pos - (token0 + c * 32 + 4 * x + 2 * h);  // tokens behind the query
+                if (back < 0 || back >= window) a = -INFINITY;
+                if (back < 1 || back - 1 >= window) b = -INFINITY;
+                z = pack2(a, b);
+              }
+              top = max3(top, a, b);
+              y[2 * x + h] = z;
             }
           }
-          tmem_st_x16(scores + c * 16, weights);
+          if (turn == 2) break;
+          if (turn == 0) {
+            if (!__any_sync(0xffffffffu, top > up + 4.0f || most > value_limit)) break;
+            less = 0.0f;
+            continue;
+          }
+          int e = 0;
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            float a, b;
+            unpack2(y[x], a, b);
+            const float2 v = reinterpret_cast<const float2*>(vs)[x];
+            const int ea = static_cast<int>(__float_as_uint(v.x) >> 23 & 255);
+            const int eb = static_cast<int>(__float_as_uint(v.y) >> 23 & 255);
+            if (a > -INFINITY && ea < 255) e = max(e, ea);
+            if (b > -INFINITY && eb < 255) e = max(e, eb);
+          }
+          float f = 1.0f;  // of what the row has so far
+          if (top > ref) {
+            f = exp2_fast(ref - top);
+            ref = top;
+          }
+          if (e > 0) {
+            const float now = 10.0f - static_cast<float>(min(max(e, 37), 197) - 127);
+            if (!value_set || now < up) {
+              f *= exp2_fast(now - up);
+              up = now;
+              value_limit = exp2_fast(11.0f - up);
+            }
+            value_set = true;
+          }
+          sum = mul2(sum, pack2(f, f));
+          if (__any_sync(0xffffffffu, f != 1.0f)) {
+            // the output so far (the scores being there, the products before them are done) ...
+            if (j > 0) {
+#pragma unroll 1
+              for (int d = 0; d < DP; d += 16) {
+                uint32_t o[16];
+                tmem_ld_x16(result + d, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                tmem_st_x16(result + d, o);
+              }
+            }
+            // ... and the tile's earlier weights
+            tmem_wait_st();
+#pragma unroll 1
+            for (int d = 0; d < c; ++d) {
+              uint32_t o[16];
+              tmem_ld_x16(scores + d * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                const float2 v = unpack_half2(o[x]);
+                o[x] = pack_half2(v.x * f, v.y * f);
+              }
+              tmem_st_x16(scores + d * 16, o);
+            }
+          }
+          less = up - ref;
+        }
+        uint32_t weights[16];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float4 v = vs[x];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float a, b;
+            unpack2(y[2 * x + h], a, b);
+            const uint64_t e2 = pack2(exp2_fast(a), exp2_fast(b));
+            sum = add2(sum, e2);
+            float wa, wb;
+            unpack2(mul2(e2, h ? pack2(v.z, v.w) : pack2(v.x, v.y)), wa, wb);
+            if constexpr (!kOpen) {  // a token that is not seen may have any scale
+              if (a == -INFINITY) wa = 0.0f;
+              if (b == -INFINITY) wb = 0.0f;
+            }
+            weights[2 * x + h] = pack_half2(wa, wb);
+          }
+        }
+        tmem_st_x16(scores + c * 16, weights);
+      };
+
+      meet();  // the query tile stands in shared memory
+      if (issuer && tiles > 0) ok = score(0);
+      for (int j = 0; j < tiles; ++j) {
+        // A wait that gives up leaves the rest of the loop to run on whatever is
+        // there, without another long wait: the barriers below stay whole.
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[w], j & 1, ab, kErrSoftmaxWait)) && ok;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, ab,
+                                               kErrSoftmaxWait)) && ok;
+        tc_fence_after();
+        key_scales = reinterpret_cast<const float*>(smem + L::kScales) + (j % kScaleSlots) * 2 * kTokens;
+        value_scales = key_scales + kTokens;
+        const float* most4 = bars.most[j % kScaleSlots];
+        const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
+        token0 = (work.lo + j) * kTokens;
+        // every row of the warp sees all of the tile's tokens
+        if (token0 + kTokens - 1 <= pos_min && pos_max - token0 < window) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) chunk(std::true_type{}, j, c, most);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) chunk(std::false_type{}, j, c, most);
         }
         tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bars.p_ready[w]);
+        meet();
+        if (issuer) {
+          ok = output(j) && ok;
+          if (j + 1 < tiles) ok = score(j + 1) && ok;
+        }
       }
 
       // --- the result: output over the sum
-      if (ok && tiles > 0) ok = mbar_wait_warp(&bars.o_full[w], 0, ab, kErrSoftmaxWait);
+      if (tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[w], 0, ab, kErrSoftmaxWait)) && ok;
       tc_fence_after();
       float s0, s1;
       unpack2(sum, s0, s1);
       s0 += s1;
-      const float up = __uint_as_float(static_cast<uint32_t>(value_exp + 117) << 23);
-      const float by = s0 > 0.0f || s0 != s0 ? up / s0 : 0.0f;
+      const float over = s0 > 0.0f || s0 != s0 ? 1.0f / s0 : 0.0f;
       __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.a.out) +
                           static_cast<int64_t>(work.seq.first + i) * p.a.out_token + static_cast<int64_t>(q_head) * p.a.out_head;
-      if (ok) {
 #pragma unroll 1
-        for (int d = 0; d < DP && d < dim; d += 32) {
-          uint32_t o[32];
-          if (tiles > 0) {
-            tmem_ld_32x32b_x32(output + d, o);
-            tmem_wait_ld();
-          }
-          if (!there) continue;
+      for (int d = 0; d < dim; d += 16) {
+        uint32_t o[16];
+        if (tiles > 0) {
+          tmem_ld_x16(result + d, o);
+          tmem_wait_ld();
+        }
+        if (!there || !ok) continue;
 #pragma unroll
-          for (int x = 0; x < 32; x += 4) {
-            if (d + x >= dim) continue;
-            float v[4];
+        for (int x = 0; x < 16; x += 4) {
+          float v[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) v[y] = tiles > 0 ? __uint_as_float(o[x + y]) * by : 0.0f;
-            Vec<__nv_bfloat16, 4>::store(to + d + x, v);
-          }
+          for (int y = 0; y < 4; ++y) v[y] = tiles > 0 ? __uint_as_float(o[x + y]) * over : 0.0f;
+          Vec<__nv_bfloat16, 4>::store(to + d + x, v);
         }
       }
       tc_fence_before();
+      if (issuer && *ab.flag) {
+        // what was issued still ends before the memory goes
+        if (elect_sync()) umma_commit(&bars.drain[w]);
+        __syncwarp();
+        mbar_wait_drain(&bars.drain[w], 0, 500000000ull);
+      }
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------- converting
@@ -537,85 +596,30 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       mbar_arrive(&bars.v_full[stage]);
       if (more) fetch(cache.v, v);
     }
-  } else {
-    // ------------------------------------------------------------- the products
-    constexpr uint32_t kScoreDesc = instr_desc(1, 0, 0, 0, 0, 128, kTokens);
-    constexpr uint32_t kOutDesc = instr_desc(1, 0, 0, 0, 1, 128, DP);
-    const uint32_t base = smem_addr(smem);
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, kErrMmaWait));
-      tc_fence_after();
-      return ok;
-    };
-    auto score = [&](int w, int j) {
-      if (elect_sync()) {
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint64_t q = smem_desc_sw128(base + L::kQuery + w * L::kMatrix + k / 4 * L::kHalf, 16, 1024) + (k & 3) * 2;
-          const uint64_t c =
-              smem_desc_sw128(base + L::kKeys + (j & 1) * L::kMatrix + k / 4 * L::kHalf, 16, 1024) + (k & 3) * 2;
-          umma_bf16(score_at(w), q, c, kScoreDesc, k != 0);
-        }
-        umma_commit(&bars.s_full[w]);
-        if (w == queries - 1) umma_commit(&bars.k_empty[j & 1]);
-      }
-      __syncwarp();
-    };
-    auto output = [&](int w, int j) {
-      if (elect_sync()) {
-        const uint64_t c = smem_desc_sw128(base + L::kValues + (j & 1) * L::kMatrix, L::kHalf, 1024);
-#pragma unroll
-        for (int k = 0; k < kTokens / 16; ++k)
-          umma_f16_ts(out_at(w), score_at(w) + k * 8, c + k * 128, kOutDesc, (j | k) != 0);
-        if (w == queries - 1) umma_commit(&bars.v_empty[j & 1]);
-        if (j + 1 == tiles) umma_commit(&bars.o_full[w]);
-      }
-      __syncwarp();
-    };
-    bool ok = tiles > 0;
-    for (int w = 0; w < queries && ok; ++w) ok = wait(&bars.q_ready[w], 0);
-    if (ok) ok = wait(&bars.k_full[0], 0);
-    for (int w = 0; w < queries && ok; ++w) score(w, 0);
-    for (int j = 0; j < tiles && ok; ++j) {
-      ok = wait(&bars.v_full[j & 1], (j >> 1) & 1);
-      for (int w = 0; w < queries && ok; ++w) {
-        ok = wait(&bars.p_ready[w], j & 1);
-        if (!ok) break;
-        output(w, j);
-        if (j + 1 < tiles) {
-          if (w == 0) ok = wait(&bars.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
-          if (ok) score(w, j + 1);
-        }
-      }
-    }
-    if (*ab.flag) {
-      // what was issued still ends before the memory goes
-      if (elect_sync()) umma_commit(&bars.drain);
-      __syncwarp();
-      mbar_wait_drain(&bars.drain, 0, 500000000ull);
-    }
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 11) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
-template <int DP>
+template <int DP, bool CAP>
 cudaError_t launch_dims(const AttendDev& p, cudaStream_t stream) {
   static std::atomic<bool> allowed[kMaxDevices];
-  const cudaError_t e = allow_smem(attend_prompt<DP>, Layout<DP>::kBytes, allowed);
+  const cudaError_t e = allow_smem(attend_prompt<DP, CAP>, Layout<DP>::kBytes, allowed);
   if (e != cudaSuccess) return e;
   const int64_t slots = static_cast<int64_t>(p.a.batch.tokens) * p.group / kRows + p.a.batch.seqs;
   PdlLaunch launch(dim3(static_cast<unsigned>(slots * p.a.cache.heads)), dim3(kThreads), Layout<DP>::kBytes, stream);
-  return launch(attend_prompt<DP>, p, static_cast<int>(slots));
+  return launch(attend_prompt<DP, CAP>, p, static_cast<int>(slots));
 }
 
 }  // namespace
 
 cudaError_t launch_attend_prompt(const AttendDev& p, cudaStream_t stream) {
-  return p.a.cache.dim <= 64 ? launch_dims<64>(p, stream) : launch_dims<128>(p, stream);
+  const bool cap = p.a.softcap > 0.0f;
+  if (p.a.cache.dim <= 64) return cap ? launch_dims<64, true>(p, stream) : launch_dims<64, false>(p, stream);
+  return cap ? launch_dims<128, true>(p, stream) : launch_dims<128, false>(p, stream);
 }
 
 }  // namespace dev
