@@ -856,7 +856,9 @@ int new_tokens(const AttendDev& p) {
 bool for_prompt(const AttendDev& p) {
   const int64_t rows = static_cast<int64_t>(new_tokens(p)) * p.group;
   const int64_t ctas = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads / 256;
-  return p.a.elem == kBF16 && p.a.cache.dim <= 128 && rows >= 128 && ctas >= 1;
+  const bool vectors = reinterpret_cast<uintptr_t>(p.a.q) % 16 == 0 && reinterpret_cast<uintptr_t>(p.a.out) % 16 == 0 &&
+                       p.a.q_token % 8 == 0 && p.a.q_head % 8 == 0 && p.a.out_token % 8 == 0 && p.a.out_head % 8 == 0;
+  return p.a.elem == kBF16 && p.a.cache.dim <= 128 && vectors && rows >= 128 && ctas >= 1;
 }
 
 // Query rows of a segment: 8, 16 or 32, by the rows that a sequence's new

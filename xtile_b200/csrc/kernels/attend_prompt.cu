@@ -11,9 +11,11 @@
 //                    columns; they also divide and store the result.  Warps 0
 //                    and 4 issue their tile's tcgen05.mma: S = Q K^T (both in
 //                    shared memory) and O += P V (P in TMEM, V read N-major)
-//   warps 8-11       load the int8 rows, turn them into f16 in shared memory
-//                    (128-byte swizzle), two stages each of keys and values
+//   warps 8-11, 12-15  load the int8 rows of the keys and of the values and
+//                    turn them into f16 in shared memory (128-byte swizzle,
+//                    two stages); one such group for both was the bottleneck
 //
+// Registers go where the rows are: 168 a softmax thread, 88 a converting one.
 // While one query tile's softmax runs, the tensor cores work for the other.
 // The scores of the next token tile go to the same columns as the weights that
 // the product before it reads: the MMAs of one thread execute in order.
@@ -37,7 +39,8 @@ using namespace sm100;
 
 constexpr int kTokens = 128;  // tokens of a tile
 constexpr int kTileRows = 128, kRows = 2 * kTileRows;
-constexpr int kThreads = 12 * 32;
+constexpr int kThreads = 16 * 32;
+constexpr int kSoftmaxRegs = 168, kConvertRegs = 88;  // 256 threads each: the 64 K registers of the launch at 128
 constexpr int kScaleSlots = 4;
 enum : uint32_t { kErrSoftmaxWait = 0x304, kErrConvertWait = 0x305 };
 
@@ -79,6 +82,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// Four f32 values at a shared-memory address, as two pairs.
+__device__ __forceinline__ void lds_pairs(uint64_t (&v)[2], uint32_t at) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[0]), "=l"(v[1]) : "r"(at));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -189,11 +196,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       mbar_init(&bars.o_full[i], 1);
       mbar_init(&bars.drain[i], 1);
     }
-    for (int i = 0; i < kScaleSlots; ++i) mbar_init(&bars.scales_full[i], 128);
+    for (int i = 0; i < kScaleSlots; ++i) mbar_init(&bars.scales_full[i], 256);
     bars.abort = 0;
     fence_barrier_init();
   }
-  if (warp == 11) {
+  if (warp == 15) {
     tmem_alloc(&bars.tmem, 512);
     tmem_relinquish();
   }
@@ -208,47 +215,60 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
 
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int w = warp >> 2;
     if (w < queries) {
       const int local = (threadIdx.x & 127), row = w * kTileRows + local;  // TMEM lane = local
       const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;      // lane offset 32 * (warp & 3)
       const int packed = work.row0 + row;
       const int i = p.group_div.quot(packed);
-      const bool there = row < work.rows;
       const int pos = work.seq.length - work.seq.count + i;
-      const int q_head = work.head * p.group + packed - i * p.group;
       const float cap = p.a.softcap;
 
-      // --- the query row as f16 times 2^(10 - exponent of its largest magnitude)
-      float row_scale;
+      // --- the query rows as f16 times 2^(10 - exponent of the row's largest
+      // magnitude).  DP / 8 lanes have a row, 16 bytes each, and all of a warp's
+      // loads are under way at once (a row a thread, its stores below likewise,
+      // took 9 us of a CTA's time).
+      constexpr int kRowLanes = DP / 8, kWarpRows = 32 / kRowLanes, kSteps = 32 / kWarpRows;
+      const int part = lane % kRowLanes, sub = lane / kRowLanes;
+      const int warp_row = w * kTileRows + (warp & 3) * 32;  // the warp's first row
+      auto row_at = [&](int step, int64_t token_stride, int64_t head_stride) {  // offset of the lane's part of row step; -1: none
+        const int r = warp_row + step * kWarpRows + sub;
+        const int at = work.row0 + r, token = p.group_div.quot(at);
+        if (r >= work.rows || part * 8 >= dim) return static_cast<int64_t>(-1);
+        return static_cast<int64_t>(work.seq.first + token) * token_stride +
+               static_cast<int64_t>(work.head * p.group + at - token * p.group) * head_stride + part * 8;
+      };
+      float row_scale = 0.0f;
       {
-        const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(p.a.q) +
-                                    static_cast<int64_t>(work.seq.first + i) * p.a.q_token +
-                                    static_cast<int64_t>(q_head) * p.a.q_head;
-        float top = 0.0f;
-        if (there)
-          for (int d = 0; d < dim; d += 4) {
-            float v[4];
-            Vec<__nv_bfloat16, 4>::load(from + d, v);
-            top = fmaxf(fmaxf(fmaxf(top, fabsf(v[0])), fmaxf(fabsf(v[1]), fabsf(v[2]))), fabsf(v[3]));
-          }
-        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 243);
-        const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23 | (p.a.scale < 0.0f ? 0x80000000u : 0u));
-        row_scale = __uint_as_float(static_cast<uint32_t>(e - 10) << 23) * fabsf(p.a.scale) *
-                    (cap > 0.0f ? 1.0f / cap : kLog2e);
-        uint8_t* to = smem + L::kQuery + w * L::kMatrix + local * 128;
+        uint4 raw[kSteps];
 #pragma unroll
-        for (int c = 0; c < DP / 8; ++c) {
-          uint32_t h[4] = {0, 0, 0, 0};
-          if (there && c * 8 < dim) {
-            float v[4], u[4];
-            Vec<__nv_bfloat16, 4>::load(from + c * 8, v);
-            Vec<__nv_bfloat16, 4>::load(from + c * 8 + 4, u);
-            h[0] = pack_half2(v[0] * up, v[1] * up), h[1] = pack_half2(v[2] * up, v[3] * up);
-            h[2] = pack_half2(u[0] * up, u[1] * up), h[3] = pack_half2(u[2] * up, u[3] * up);
-          }
-          *reinterpret_cast<uint4*>(to + c / 8 * L::kHalf + (((c & 7) ^ (local & 7)) << 4)) =
-              make_uint4(h[0], h[1], h[2], h[3]);
+        for (int x = 0; x < kSteps; ++x) {
+          const int64_t at = row_at(x, p.a.q_token, p.a.q_head);
+          raw[x] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.a.q) + at)
+                           : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int x = 0; x < kSteps; ++x) {
+          const uint32_t v[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+          float top = 0.0f;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[y])), fabsf(bf16_hi(v[y]))));
+#pragma unroll
+          for (int o = kRowLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 243);
+          const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23 | (p.a.scale < 0.0f ? 0x80000000u : 0u));
+          const float down = __uint_as_float(static_cast<uint32_t>(e - 10) << 23) * fabsf(p.a.scale) *
+                             (cap > 0.0f ? 1.0f / cap : kLog2e);
+          // to the thread that has the row
+          const float mine = __shfl_sync(0xffffffffu, down, lane % kWarpRows * kRowLanes);
+          if (lane / kWarpRows == x) row_scale = mine;
+          const int r = (warp & 3) * 32 + x * kWarpRows + sub;
+          uint32_t h[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) h[y] = pack_half2(bf16_lo(v[y]) * up, bf16_hi(v[y]) * up);
+          *reinterpret_cast<uint4*>(smem + L::kQuery + w * L::kMatrix + part / 8 * L::kHalf + r * 128 +
+                                    (((part & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         fence_proxy_async_smem();
       }
@@ -306,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       const int pos_min = __shfl_sync(0xffffffffu, pos, 0);  // of the warp's rows
       const int pos_max = __shfl_sync(0xffffffffu, pos, 31);
       const int window = p.a.window > 0 ? p.a.window : INT_MAX;
-      const float *key_scales = nullptr, *value_scales = nullptr;
+      uint32_t key_scales = 0, value_scales = 0;  // shared-memory addresses
       int token0 = 0;
 
       // Chunk c (32 tokens) of a tile: scores from TMEM, weights to TMEM.
@@ -315,8 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         uint32_t r[32];
         tmem_ld_32x32b_x32(scores + c * 32, r);
         tmem_wait_ld();
-        const float4* ks = reinterpret_cast<const float4*>(key_scales + c * 32);
-        const float4* vs = reinterpret_cast<const float4*>(value_scales + c * 32);
+        const uint32_t ks = key_scales + c * 128, vs = value_scales + c * 128;
         uint64_t y[16];
         float less = up - ref;
         // The reference follows a row's maximum only when that has risen by
@@ -329,11 +348,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
           float top = -INFINITY;
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
-            const float4 k = ks[x];
+            uint64_t k[2];
+            lds_pairs(k, ks + x * 16);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint64_t z = mul2(pack2(__uint_as_float(r[4 * x + 2 * h]), __uint_as_float(r[4 * x + 2 * h + 1])),
-                                h ? pack2(k.z, k.w) : pack2(k.x, k.y));
+              uint64_t z = mul2(pack2(__uint_as_float(r[4 * x + 2 * h]), __uint_as_float(r[4 * x + 2 * h + 1])), k[h]);
               if constexpr (CAP) {
                 float a, b;
                 unpack2(z, a, b);
@@ -360,19 +379,25 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
           }
           int e = 0;
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            float a, b;
-            unpack2(y[x], a, b);
-            const float2 v = reinterpret_cast<const float2*>(vs)[x];
-            const int ea = static_cast<int>(__float_as_uint(v.x) >> 23 & 255);
-            const int eb = static_cast<int>(__float_as_uint(v.y) >> 23 & 255);
-            if (a > -INFINITY && ea < 255) e = max(e, ea);
-            if (b > -INFINITY && eb < 255) e = max(e, eb);
+          for (int x = 0; x < 8; ++x) {
+            uint64_t v[2];
+            lds_pairs(v, vs + x * 16);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float a, b, va, vb;
+              unpack2(y[2 * x + h], a, b);
+              unpack2(v[h], va, vb);
+              const int ea = static_cast<int>(__float_as_uint(va) >> 23 & 255);
+              const int eb = static_cast<int>(__float_as_uint(vb) >> 23 & 255);
+              if (a > -INFINITY && ea < 255) e = max(e, ea);
+              if (b > -INFINITY && eb < 255) e = max(e, eb);
+            }
           }
           float f = 1.0f;  // of what the row has so far
           if (top > ref) {
-            f = exp2_fast(ref - top);
-            ref = top;
+            const float now = top + 2.0f;  // room, so that it need not move again soon
+            f = exp2_fast(ref - now);
+            ref = now;
           }
           if (e > 0) {
             const float now = 10.0f - static_cast<float>(min(max(e, 37), 197) - 127);
@@ -417,7 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         uint32_t weights[16];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          const float4 v = vs[x];
+          uint64_t v[2];
+          lds_pairs(v, vs + x * 16);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float a, b;
@@ -425,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
             const uint64_t e2 = pack2(exp2_fast(a), exp2_fast(b));
             sum = add2(sum, e2);
             float wa, wb;
-            unpack2(mul2(e2, h ? pack2(v.z, v.w) : pack2(v.x, v.y)), wa, wb);
+            unpack2(mul2(e2, v[h]), wa, wb);
             if constexpr (!kOpen) {  // a token that is not seen may have any scale
               if (a == -INFINITY) wa = 0.0f;
               if (b == -INFINITY) wb = 0.0f;
@@ -445,8 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, ab,
                                                kErrSoftmaxWait)) && ok;
         tc_fence_after();
-        key_scales = reinterpret_cast<const float*>(smem + L::kScales) + (j % kScaleSlots) * 2 * kTokens;
-        value_scales = key_scales + kTokens;
+        key_scales = base + L::kScales + (j % kScaleSlots) * 2 * kTokens * 4;
+        value_scales = key_scales + kTokens * 4;
         const float* most4 = bars.most[j % kScaleSlots];
         const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
         token0 = (work.lo + j) * kTokens;
@@ -473,23 +499,33 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       unpack2(sum, s0, s1);
       s0 += s1;
       const float over = s0 > 0.0f || s0 != s0 ? 1.0f / s0 : 0.0f;
-      __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.a.out) +
-                          static_cast<int64_t>(work.seq.first + i) * p.a.out_token + static_cast<int64_t>(q_head) * p.a.out_head;
+      // the row's values to the query tile's room (its last product is done), from
+      // where DP / 8 lanes store each row
+      uint8_t* room = smem + L::kQuery + w * L::kMatrix + (warp & 3) * 32 * DP * 2;
 #pragma unroll 1
-      for (int d = 0; d < dim; d += 16) {
+      for (int d = 0; d < DP; d += 16) {
         uint32_t o[16];
         if (tiles > 0) {
           tmem_ld_x16(result + d, o);
           tmem_wait_ld();
         }
-        if (!there || !ok) continue;
+        uint32_t v[8];
 #pragma unroll
-        for (int x = 0; x < 16; x += 4) {
-          float v[4];
+        for (int x = 0; x < 8; ++x)
+          v[x] = tiles > 0 ? pack_bf16(__uint_as_float(o[2 * x]) * over, __uint_as_float(o[2 * x + 1]) * over) : 0;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) v[y] = tiles > 0 ? __uint_as_float(o[x + y]) * over : 0.0f;
-          Vec<__nv_bfloat16, 4>::store(to + d + x, v);
-        }
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<uint4*>(room + lane * DP * 2 + (((d / 8 + h) ^ (lane & 7)) << 4)) =
+              make_uint4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < kSteps; ++x) {
+        const int r = x * kWarpRows + sub;
+        const int64_t at = row_at(x, p.a.out_token, p.a.out_head);
+        if (at >= 0 && ok)
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + at) =
+              *reinterpret_cast<const uint4*>(room + r * DP * 2 + ((part ^ (r & 7)) << 4));
       }
       tc_fence_before();
       if (issuer && *ab.flag) {
@@ -499,48 +535,64 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         mbar_wait_drain(&bars.drain[w], 0, 500000000ull);
       }
     }
-  } else if (warp < 12) {
+  } else {
     // ------------------------------------------------------------- converting
-    const int me = threadIdx.x - 256, wv = warp - 8;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
+    const bool keys = warp < 12;
+    const int me = threadIdx.x & 127, wv = warp & 3;
+    const int8_t* data = keys ? cache.k : cache.v;
+    const float* data_scales = keys ? cache.k_scale : cache.v_scale;
+    uint8_t* matrices = smem + (keys ? L::kKeys : L::kValues);
+    uint64_t* full = keys ? bars.k_full : bars.v_full;
+    uint64_t* empty = keys ? bars.k_empty : bars.v_empty;
     constexpr int kChunks = DP / 16;               // 16-byte chunks of an int8 row
     constexpr int kAtOnce = 128 / kChunks;         // rows that the 128 threads take at once
     constexpr int kTurns = kTokens / kAtOnce;
     // lanes so that a quarter of a warp stores to eight different bank groups
     const int chunk = DP == 128 ? (lane & 3) | (lane >> 3 & 1) << 2 : lane & 3;
     const int my_row = DP == 128 ? wv * 4 + ((lane >> 2 & 1) | (lane >> 4 & 1) << 1) : wv * 8 + (lane >> 2);
-    int64_t from[kTurns];  // offset of the thread's chunk of each of its rows; -1: zeros
-    int4 k[kTurns], v[kTurns];
-    bool ok = true;
+    int4 x[kTurns];
+    float scale = 0.0f;  // of the thread's own token: 0 behind the end, NaN of a bad page
 
-    auto line_of = [&](int token, int& row) -> int64_t {  // (page, head) of a token; -1: none, -2: a bad page
-      if (token >= work.seq.length) return -1;
-      const int index = p.page_div.quot(token);
-      row = token - index * cache.page;
-      const int id = work.table[index];
-      if (id < 0 || id >= cache.pages) {
-        atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
-        return -2;
-      }
-      return static_cast<int64_t>(id) * cache.heads + work.head;
+    // page of a token: -1: none, -2: outside the cache
+    auto page_of = [&](int token) {
+      return token < work.seq.length ? work.table[p.page_div.quot(token)] : -1;
     };
-    auto look_up = [&](int j) {
+    auto checked = [&](int id, int token) {
+      if (token >= work.seq.length) return -1;
+      if (id >= 0 && id < cache.pages) return id;
+      atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
+      return -2;
+    };
+    auto fetch = [&](int j) {
+      const int token0 = (work.lo + j) * kTokens;
+      int id[kTurns];
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) id[i] = page_of(token0 + i * kAtOnce + my_row);
+      int mine = page_of(token0 + me);
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
-        int row = 0;
-        const int64_t line = line_of((work.lo + j) * kTokens + i * kAtOnce + my_row, row);
-        from[i] = line < 0 || chunk * 16 >= dim ? -1 : (line * cache.page + row) * dim + chunk * 16;
+        const int token = token0 + i * kAtOnce + my_row;
+        id[i] = checked(id[i], token);
+        const int64_t line = static_cast<int64_t>(id[i]) * cache.heads + work.head;
+        const int row = token - p.page_div.quot(token) * cache.page;
+        x[i] = make_int4(0, 0, 0, 0);
+        if (id[i] >= 0 && chunk * 16 < dim)
+          x[i] = *reinterpret_cast<const int4*>(data + (line * cache.page + row) * dim + chunk * 16);
       }
+      mine = checked(mine, token0 + me);
+      const int row = token0 + me - p.page_div.quot(token0 + me) * cache.page;
+      const int64_t line = static_cast<int64_t>(mine) * cache.heads + work.head;
+      scale = mine >= 0 ? data_scales[line * p.blocks + p.block_div.quot(row)] : mine == -1 ? 0.0f : __int_as_float(0x7fc00000);
     };
-    auto fetch = [&](const int8_t* base, int4 (&to)[kTurns]) {
-#pragma unroll
-      for (int i = 0; i < kTurns; ++i)
-        to[i] = from[i] < 0 ? make_int4(0, 0, 0, 0) : *reinterpret_cast<const int4*>(base + from[i]);
-    };
-    auto convert = [&](uint8_t* matrix, const int4 (&x)[kTurns]) {
+    if (tiles > 0) fetch(0);
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j & 1;
+      if (!mbar_wait_warp(&empty[stage], ((j >> 1) & 1) ^ 1, ab, kErrConvertWait)) break;
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
         const int row = i * kAtOnce + my_row;
-        uint8_t* to = matrix + chunk / 4 * L::kHalf + row * 128;
+        uint8_t* to = matrices + stage * L::kMatrix + chunk / 4 * L::kHalf + row * 128;
         const uint32_t u[4] = {static_cast<uint32_t>(x[i].x) ^ 0x80808080u, static_cast<uint32_t>(x[i].y) ^ 0x80808080u,
                                static_cast<uint32_t>(x[i].z) ^ 0x80808080u, static_cast<uint32_t>(x[i].w) ^ 0x80808080u};
 #pragma unroll
@@ -549,56 +601,24 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
               make_uint4(bytes_to_half2<kLow>(u[2 * h]), bytes_to_half2<kHigh>(u[2 * h]),
                          bytes_to_half2<kLow>(u[2 * h + 1]), bytes_to_half2<kHigh>(u[2 * h + 1]));
       }
-    };
-    // the scales of the thread's own token (0 behind the end, NaN of a bad page)
-    float ks = 0.0f, vs = 0.0f;
-    auto fetch_scales = [&](int j) {
-      int row = 0;
-      const int64_t line = line_of((work.lo + j) * kTokens + me, row);
-      const int64_t at = line * p.blocks + p.block_div.quot(row);
-      ks = line >= 0 ? cache.k_scale[at] : line == -1 ? 0.0f : __int_as_float(0x7fc00000);
-      vs = line >= 0 ? cache.v_scale[at] : line == -1 ? 0.0f : __int_as_float(0x7fc00000);
-    };
-    if (tiles > 0) {
-      look_up(0);
-      fetch(cache.k, k);
-      fetch(cache.v, v);
-      fetch_scales(0);
-    }
-    for (int j = 0; j < tiles; ++j) {
-      const int stage = j & 1;
-      const uint32_t phase = (j >> 1) & 1;
-      ok = mbar_wait_warp(&bars.k_empty[stage], phase ^ 1, ab, kErrConvertWait);
-      if (!ok) break;
-      convert(smem + L::kKeys + stage * L::kMatrix, k);
       fence_proxy_async_smem();
-      mbar_arrive(&bars.k_full[stage]);
-      // a slot's softmax is done: the scores of tile j - 2, whose stage this was, came behind it
-      float* scales = reinterpret_cast<float*>(smem + L::kScales) + (j % kScaleSlots) * 2 * kTokens;
-      scales[me] = ks;
-      scales[kTokens + me] = vs;
-      float most = vs < INFINITY ? vs : 0.0f;
+      mbar_arrive(&full[stage]);
+      // a slot's softmax is done: the products of tile j - 2, whose stage this was, came behind it
+      const int slot = j % kScaleSlots;
+      reinterpret_cast<float*>(smem + L::kScales)[slot * 2 * kTokens + (keys ? 0 : kTokens) + me] = scale;
+      if (!keys) {
+        float most = scale < INFINITY ? scale : 0.0f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (lane == 0) bars.most[j % kScaleSlots][wv] = most;
-      __syncwarp();
-      mbar_arrive(&bars.scales_full[j % kScaleSlots]);
-      const bool more = j + 1 < tiles;
-      if (more) {
-        look_up(j + 1);
-        fetch(cache.k, k);
-        fetch_scales(j + 1);
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (lane == 0) bars.most[slot][wv] = most;
+        __syncwarp();
       }
-      ok = mbar_wait_warp(&bars.v_empty[stage], phase ^ 1, ab, kErrConvertWait);
-      if (!ok) break;
-      convert(smem + L::kValues + stage * L::kMatrix, v);
-      fence_proxy_async_smem();
-      mbar_arrive(&bars.v_full[stage]);
-      if (more) fetch(cache.v, v);
+      mbar_arrive(&bars.scales_full[slot]);
+      if (j + 1 < tiles) fetch(j + 1);
     }
   }
   __syncthreads();
-  if (warp == 11) {
+  if (warp == 15) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
