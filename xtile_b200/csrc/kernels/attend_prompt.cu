@@ -98,6 +98,34 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+// Waits for a phase as mbar_wait does, but suspended in hardware for up to
+// ``kSuspendNs`` at a time: 16 polling warps took a fifth of the SM's issue
+// slots.  A whole warp calls.
+constexpr uint32_t kSuspendNs = 20000;
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const Abort& ab, uint32_t code) {
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if (*ab.flag) return false;
+    const uint64_t now = clock64();
+    if (t0 == 0) {
+      t0 = now;
+    } else if (now - t0 > ab.limit) {
+      *ab.flag = 1;
+      atomicCAS(ab.error_word, 0u, code);
+      return false;
+    }
+  }
+}
+
 // D[tmem] (+)= A[tmem] * B[smem], f16 inputs, f32 accumulate.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -278,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       constexpr uint32_t kOutDesc = instr_desc(1, 0, 0, 0, 1, 128, DP);
       const uint32_t base = smem_addr(smem);
       auto score = [&](int j) {  // S = Q K^T of token tile j; false: a wait gave up
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars.k_full[j & 1], (j >> 1) & 1, ab, kErrSoftmaxWait))) return false;
+        if (!wait_phase(&bars.k_full[j & 1], (j >> 1) & 1, ab, kErrSoftmaxWait)) return false;
         tc_fence_after();
         if (elect_sync()) {
 #pragma unroll
@@ -295,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         return true;
       };
       auto output = [&](int j) {  // O += P V of token tile j
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars.v_full[j & 1], (j >> 1) & 1, ab, kErrSoftmaxWait))) return false;
+        if (!wait_phase(&bars.v_full[j & 1], (j >> 1) & 1, ab, kErrSoftmaxWait)) return false;
         tc_fence_after();
         if (elect_sync()) {
           const uint64_t c = smem_desc_sw128(base + L::kValues + (j & 1) * L::kMatrix, L::kHalf, 1024);
@@ -337,13 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         tmem_wait_ld();
         const uint32_t ks = key_scales + c * 128, vs = value_scales + c * 128;
         uint64_t y[16];
-        float less = up - ref;
-        // The reference follows a row's maximum only when that has risen by
-        // more than 2^4, and the values' exponent only when a weight could
-        // leave f16's range, so the first turn is mostly the only one; the
-        // second takes the scores themselves.
-#pragma unroll 1
-        for (int turn = 0;; ++turn) {
+        auto exponents = [&](float less) {  // the largest of y = score + less
           const uint64_t by = pack2(factor, factor), add = pack2(less, less);
           float top = -INFINITY;
 #pragma unroll
@@ -371,12 +393,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
               y[2 * x + h] = z;
             }
           }
-          if (turn == 2) break;
-          if (turn == 0) {
-            if (!__any_sync(0xffffffffu, top > up + 4.0f || most > value_limit)) break;
-            less = 0.0f;
-            continue;
-          }
+          return top;
+        };
+        // The reference follows a row's maximum only when that has risen by
+        // more than 2^4, and the values' exponent only when a weight could
+        // leave f16's range.
+        float top = exponents(up - ref);
+        if (__any_sync(0xffffffffu, top > up + 4.0f || most > value_limit)) {
+          top = exponents(0.0f);
           int e = 0;
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
@@ -437,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
               tmem_st_x16(scores + d * 16, o);
             }
           }
-          less = up - ref;
+          exponents(up - ref);
         }
         uint32_t weights[16];
 #pragma unroll
@@ -467,9 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       for (int j = 0; j < tiles; ++j) {
         // A wait that gives up leaves the rest of the loop to run on whatever is
         // there, without another long wait: the barriers below stay whole.
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[w], j & 1, ab, kErrSoftmaxWait)) && ok;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, ab,
-                                               kErrSoftmaxWait)) && ok;
+        ok = wait_phase(&bars.s_full[w], j & 1, ab, kErrSoftmaxWait) && ok;
+        ok = wait_phase(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, ab, kErrSoftmaxWait) && ok;
         tc_fence_after();
         key_scales = base + L::kScales + (j % kScaleSlots) * 2 * kTokens * 4;
         value_scales = key_scales + kTokens * 4;
@@ -493,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       }
 
       // --- the result: output over the sum
-      if (tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[w], 0, ab, kErrSoftmaxWait)) && ok;
+      if (tiles > 0) ok = wait_phase(&bars.o_full[w], 0, ab, kErrSoftmaxWait) && ok;
       tc_fence_after();
       float s0, s1;
       unpack2(sum, s0, s1);
@@ -554,41 +577,52 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
     int4 x[kTurns];
     float scale = 0.0f;  // of the thread's own token: 0 behind the end, NaN of a bad page
 
-    // page of a token: -1: none, -2: outside the cache
-    auto page_of = [&](int token) {
-      return token < work.seq.length ? work.table[p.page_div.quot(token)] : -1;
+    // A token's page and row, from those of kAtOnce tokens before it.
+    auto step = [&](int& index, int& row) {
+      row += kAtOnce;
+      if (row < cache.page) return;
+      const int pages = cache.page >= kAtOnce ? 1 : p.page_div.quot(row);
+      index += pages;
+      row -= pages * cache.page;
     };
-    auto checked = [&](int id, int token) {
+    // (page, head) of a token as looked up: -1: behind the end, -2: a page outside the cache
+    auto line_of = [&](int id, int token) {
       if (token >= work.seq.length) return -1;
-      if (id >= 0 && id < cache.pages) return id;
+      if (id >= 0 && id < cache.pages) return id * cache.heads + work.head;
       atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
       return -2;
     };
+    const uint32_t line_bytes = static_cast<uint32_t>(cache.page) * dim;
     auto fetch = [&](int j) {
       const int token0 = (work.lo + j) * kTokens;
-      int id[kTurns];
-#pragma unroll
-      for (int i = 0; i < kTurns; ++i) id[i] = page_of(token0 + i * kAtOnce + my_row);
-      int mine = page_of(token0 + me);
+      const int first = p.page_div.quot(token0 + my_row), first_row = token0 + my_row - first * cache.page;
+      const int own = p.page_div.quot(token0 + me), own_row = token0 + me - own * cache.page;
+      int id[kTurns], index = first, row = first_row;
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
-        const int token = token0 + i * kAtOnce + my_row;
-        id[i] = checked(id[i], token);
-        const int64_t line = static_cast<int64_t>(id[i]) * cache.heads + work.head;
-        const int row = token - p.page_div.quot(token) * cache.page;
-        x[i] = make_int4(0, 0, 0, 0);
-        if (id[i] >= 0 && chunk * 16 < dim)
-          x[i] = *reinterpret_cast<const int4*>(data + (line * cache.page + row) * dim + chunk * 16);
+        id[i] = token0 + i * kAtOnce + my_row < work.seq.length ? work.table[index] : 0;
+        step(index, row);
       }
-      mine = checked(mine, token0 + me);
-      const int row = token0 + me - p.page_div.quot(token0 + me) * cache.page;
-      const int64_t line = static_cast<int64_t>(mine) * cache.heads + work.head;
-      scale = mine >= 0 ? data_scales[line * p.blocks + p.block_div.quot(row)] : mine == -1 ? 0.0f : __int_as_float(0x7fc00000);
+      const int own_id = token0 + me < work.seq.length ? work.table[own] : 0;
+      index = first, row = first_row;
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int line = line_of(id[i], token0 + i * kAtOnce + my_row);
+        x[i] = make_int4(0, 0, 0, 0);
+        if (line >= 0 && chunk * 16 < dim)
+          x[i] = *reinterpret_cast<const int4*>(data + static_cast<uint64_t>(static_cast<uint32_t>(line)) * line_bytes +
+                                                static_cast<uint32_t>(row * dim + chunk * 16));
+        step(index, row);
+      }
+      const int line = line_of(own_id, token0 + me);
+      scale = line >= 0 ? data_scales[static_cast<uint64_t>(static_cast<uint32_t>(line)) * static_cast<uint32_t>(p.blocks) +
+                                      p.block_div.quot(own_row)]
+                        : line == -1 ? 0.0f : __int_as_float(0x7fc00000);
     };
     if (tiles > 0) fetch(0);
     for (int j = 0; j < tiles; ++j) {
       const int stage = j & 1;
-      if (!mbar_wait_warp(&empty[stage], ((j >> 1) & 1) ^ 1, ab, kErrConvertWait)) break;
+      if (!wait_phase(&empty[stage], ((j >> 1) & 1) ^ 1, ab, kErrConvertWait)) break;
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
         const int row = i * kAtOnce + my_row;

@@ -35,8 +35,8 @@ int finish(const char* who, cudaError_t e) {
 int check_cache(const char* who, const xt_cache& c) {
   if (!c.k || !c.v || !c.k_scale || !c.v_scale) return bad(who, "null cache array");
   if (c.pages < 1 || c.heads < 1 || c.page < 1 || c.block < 1) return bad(who, "the cache's extents must be positive");
-  if (c.pages > kMaxInt) return bad(who, "the cache has too many pages");
-  if (c.heads > 65535) return bad(who, "the cache has too many heads");
+  if (c.heads > 65535 || c.pages > kMaxInt / c.heads) return bad(who, "the cache has too many heads or pages");
+  if (c.page > kMaxInt / 256) return bad(who, "the cache's pages are too long");
   if (c.page % c.block != 0) return bad(who, "a cache page must hold whole blocks");
   if (c.dim < 16 || c.dim > 256 || c.dim % 16 != 0) return bad(who, "the cache's dim must be a multiple of 16 up to 256");
   if (!aligned(c.k, 16) || !aligned(c.v, 16)) return bad(who, "the cache is not 16-byte aligned");
