@@ -592,6 +592,79 @@ def test_attention_prompts(new, total, dim, group, window, softcap):
     assert y.isfinite().all()
 
 
+@pytest.mark.parametrize("new, total", [([700, 64, 900], [700, 300, 2500]), ([1700], [1700]), ([33] * 50, [33 + 40 * i for i in range(50)])])
+@pytest.mark.parametrize("dim, heads, group, page", [(128, 2, 4, 64), (128, 8, 1, 40), (64, 2, 8, 16), (96, 1, 10, 48), (80, 2, 7, 1),
+                                                     (16, 1, 32, 128)])
+@pytest.mark.parametrize("window, softcap", [(0, 0.0), (130, 0.0), (0, 20.0), (7, 3.0)])
+def test_attention_long_prompts(new, total, dim, heads, group, page, window, softcap):
+    """Enough query rows for the kernel that long prompts run in, at every layout it has."""
+    g = generator(dim)
+    batch = Batch(new, total, page, seed=3)
+    cache = filled_cache(g, batch.pages_held, heads, dim, page, 8 if page % 8 == 0 else 1)
+    packed = normal(g, batch.tokens, (heads * group + 1) * dim, std=1.5, dtype=torch.bfloat16)
+    q = packed[:, :heads * group * dim].view(batch.tokens, heads * group, dim)
+    check_attention(cache, batch, q, window=window, softcap=softcap, max_new=max(new))
+
+
+def test_attention_long_prompt_edges():
+    """Rows that see nothing, garbage that no row sees, NaN that one sequence's rows see, zero scales, wrong tables."""
+    g = generator(16)
+    batch = Batch([900, 900, 300], [400, 900, 1500], 64, seed=3)  # the first 500 queries of sequence 0 see nothing
+    cache = filled_cache(g, batch.pages_held, 2, 64, 64, 1)
+    q = normal(g, batch.tokens, 16, 64, std=1.5, dtype=torch.bfloat16)
+    good = check_attention(cache, batch, q)
+    assert (good[:500] == 0).all() and torch.equal(good, xt.cache_attention(cache, q, *batch.args))
+    used = torch.zeros_like(cache.k_scale, dtype=torch.bool)
+    for b, t in enumerate(batch.total):
+        for j in range(t):
+            used[batch.table[b][j // 64], :, j % 64] = True
+    for bad in (float("nan"), float("inf"), 3e38):
+        for s in (cache.k_scale, cache.v_scale):
+            s[~used] = bad
+        assert torch.equal(xt.cache_attention(cache, q, *batch.args), good)
+    windowed = check_attention(cache, batch, q, window=50)
+    cache.v_scale[batch.table[2][0], 0, 10] = 1e30  # before the window of sequence 2's rows
+    cache.k_scale[batch.table[2][0], 0, 11] = float("nan")
+    assert torch.equal(xt.cache_attention(cache, q, *batch.args, window=50), windowed)
+    y = xt.cache_attention(cache, q, *batch.args)
+    assert y[1800:, :8].isnan().all() and torch.equal(y[:1800], good[:1800]) and torch.equal(y[:, 8:], good[:, 8:])
+    cache.k_scale[~used] = 0.02
+    cache.k_scale[batch.table[2][0], 0, 11] = 0.02
+    cache.v_scale.zero_()
+    assert (xt.cache_attention(cache, q, *batch.args) == 0).all()
+    cache = filled_cache(g, batch.pages_held, 2, 64, 64, 1)
+    good = xt.cache_attention(cache, q, *batch.args)
+    starts, lengths, table = batch.args
+    for fault in ("page", "length", "starts"):
+        s, n, t = starts.clone(), lengths.clone(), table.clone()
+        if fault == "page":
+            t[1, 3] = batch.pages_held
+        elif fault == "length":
+            n[1] = 1 << 20
+        else:
+            s[3] = batch.tokens + 5
+        y = xt.cache_attention(cache, q, s, n, t)
+        assert xt.device_error() == 0x303
+        rows = slice(1800, 2100) if fault == "starts" else slice(900 + 3 * 64, 1800) if fault == "page" else slice(900, 1800)
+        assert y[rows].isnan().all(), fault
+        assert torch.equal(y[:900], good[:900])
+
+
+def test_attention_long_prompt_scales_and_signs():
+    """Value scales of 1e-6 to 1e3 beside each other, a negative and a zero score scale, queries of very different sizes."""
+    g = generator(17)
+    batch = Batch([800, 600], [1000, 600], 64, seed=3)
+    cache = filled_cache(g, batch.pages_held, 2, 128, 64, 16)
+    q = normal(g, batch.tokens, 8, 128, dtype=torch.bfloat16)
+    q[:, ::2] *= 1e-20
+    q[:, 1::4] *= 8
+    check_attention(cache, batch, q, scale=-0.1)
+    check_attention(cache, batch, q, scale=0.0)
+    spread = torch.empty_like(cache.v_scale).uniform_(math.log(1e-6), math.log(1e3), generator=g)
+    cache.v_scale.copy_(spread.exp())
+    check_attention(cache, batch, q)
+
+
 def test_attention_hint_does_not_change_what_is_computed():
     g = generator(12)
     batch = Batch([200, 3], [400, 90], 64, seed=3)

@@ -852,13 +852,19 @@ int new_tokens(const AttendDev& p) {
   return p.a.max_new > 0 ? (p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens) : mean;
 }
 
-// Whether the tcgen05 kernel for many query rows runs the call.
+// Whether the tcgen05 kernel for many query rows runs the call.  Its CTAs take
+// about 3.7 us for 256 rows and 128 tokens, however few of the rows there are
+// and however few CTAs; attend_units spreads any work over the GPU, at 3.1 us
+// for a million (row, token) pairs of 128 dims.  They meet near 10000 rows
+// (us, attend_units and this one): 8192 rows of one sequence 123 and 126 at 4096
+// tokens, 16384 221 and 125; 64 sequences of 32 rows each and 8 heads 82 and
+// 113, of 64 rows 128 and 115.
 bool for_prompt(const AttendDev& p) {
   const int64_t rows = static_cast<int64_t>(new_tokens(p)) * p.group;
-  const int64_t ctas = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads / 256;
+  const int64_t all = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
   const bool vectors = reinterpret_cast<uintptr_t>(p.a.q) % 16 == 0 && reinterpret_cast<uintptr_t>(p.a.out) % 16 == 0 &&
                        p.a.q_token % 8 == 0 && p.a.q_head % 8 == 0 && p.a.out_token % 8 == 0 && p.a.out_head % 8 == 0;
-  return p.a.elem == kBF16 && p.a.cache.dim <= 128 && vectors && rows >= 128 && ctas >= 1;
+  return p.a.elem == kBF16 && p.a.cache.dim <= 128 && vectors && rows >= 64 && all >= 10240;
 }
 
 // Query rows of a segment: 8, 16 or 32, by the rows that a sequence's new

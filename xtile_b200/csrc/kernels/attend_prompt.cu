@@ -98,27 +98,32 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// Waits for a phase as mbar_wait does, but suspended in hardware for up to
-// ``kSuspendNs`` at a time: 16 polling warps took a fifth of the SM's issue
-// slots.  A whole warp calls.
-constexpr uint32_t kSuspendNs = 20000;
+// Waits for a phase as mbar_wait does; a whole warp calls.  The limit is
+// looked at once in 256 polls, each of which the hardware may suspend.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const Abort& ab, uint32_t code) {
+  const uint32_t at = smem_addr(bar);
   uint64_t t0 = 0;
   while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(kSuspendNs)
-        : "memory");
-    if (__all_sync(0xffffffffu, ok)) return true;
-    if (*ab.flag) return false;
+#pragma unroll 1
+    for (int poll = 0; poll < 256; ++poll) {
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(at), "r"(parity)
+          : "memory");
+      if (__any_sync(0xffffffffu, ok)) return true;  // the phase is over for every lane, then
+    }
+    if (__any_sync(0xffffffffu, *ab.flag != 0)) return false;
     const uint64_t now = clock64();
-    if (t0 == 0) {
+    bool late = false;
+    if (t0 == 0)
       t0 = now;
-    } else if (now - t0 > ab.limit) {
+    else
+      late = now - t0 > ab.limit;
+    if (__any_sync(0xffffffffu, late)) {
       *ab.flag = 1;
       atomicCAS(ab.error_word, 0u, code);
       return false;
@@ -246,57 +251,81 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int w = warp >> 2;
     if (w < queries) {
-      const int local = (threadIdx.x & 127), row = w * kTileRows + local;  // TMEM lane = local
+      const int local = w * kTileRows + (threadIdx.x & 127);  // the thread's row; its TMEM lane modulo 128
       const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;      // lane offset 32 * (warp & 3)
-      const int packed = work.row0 + row;
+      const int packed = work.row0 + local;
       const int i = p.group_div.quot(packed);
       const int pos = work.seq.length - work.seq.count + i;
       const float cap = p.a.softcap;
 
       // --- the query rows as f16 times 2^(10 - exponent of the row's largest
-      // magnitude).  DP / 8 lanes have a row, 16 bytes each, and all of a warp's
-      // loads are under way at once (a row a thread, its stores below likewise,
-      // took 9 us of a CTA's time).
+      // magnitude).  DP / 8 lanes have a row, 16 bytes each: asynchronous copies
+      // to where the row's f16 will be, turned there.  The loops here and at the
+      // end stay short: they run once a CTA, and straight code that is not in the
+      // instruction cache took 12 cycles an instruction (9000 for this part).
       constexpr int kRowLanes = DP / 8, kWarpRows = 32 / kRowLanes, kSteps = 32 / kWarpRows;
       const int part = lane % kRowLanes, sub = lane / kRowLanes;
       const int warp_row = w * kTileRows + (warp & 3) * 32;  // the warp's first row
-      auto row_at = [&](int step, int64_t token_stride, int64_t head_stride) {  // offset of the lane's part of row step; -1: none
-        const int r = warp_row + step * kWarpRows + sub;
-        const int at = work.row0 + r, token = p.group_div.quot(at);
-        if (r >= work.rows || part * 8 >= dim) return static_cast<int64_t>(-1);
-        return static_cast<int64_t>(work.seq.first + token) * token_stride +
-               static_cast<int64_t>(work.head * p.group + at - token * p.group) * head_stride + part * 8;
+      // the lane's part of the warp's rows, kWarpRows apart
+      struct Rows {
+        int at, token, head;  // packed row (of the CTA), its new token and head of the group
       };
+      const bool part_there = part * 8 < dim;
+      auto first_row = [&] {
+        const int at = warp_row + sub, token = p.group_div.quot(work.row0 + at);
+        return Rows{at, token, work.row0 + at - token * p.group};
+      };
+      auto next_row = [&](Rows& row) {
+        row.at += kWarpRows;
+        row.head += kWarpRows;
+        if (row.head < p.group) return;
+        const int tokens = p.group >= kWarpRows ? 1 : p.group_div.quot(row.head);
+        row.token += tokens;
+        row.head -= tokens * p.group;
+      };
+      auto offset = [&](const Rows& row, int64_t token_stride, int64_t head_stride) {
+        return static_cast<int64_t>(work.seq.first + row.token) * token_stride +
+               static_cast<int64_t>(work.head * p.group + row.head) * head_stride + part * 8;
+      };
+      const uint32_t base = smem_addr(smem);
       float row_scale = 0.0f;
       {
-        uint4 raw[kSteps];
-#pragma unroll
+        auto place = [&](int x) {
+          const int r = (warp & 3) * 32 + x * kWarpRows + sub;
+          return base + L::kQuery + w * L::kMatrix + part / 8 * L::kHalf + r * 128 + (((part & 7) ^ (r & 7)) << 4);
+        };
+        Rows row = first_row();
+#pragma unroll 2
         for (int x = 0; x < kSteps; ++x) {
-          const int64_t at = row_at(x, p.a.q_token, p.a.q_head);
-          raw[x] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.a.q) + at)
-                           : make_uint4(0, 0, 0, 0);
+          const bool there = row.at < work.rows && part_there;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place(x)),
+                       "l"(static_cast<const __nv_bfloat16*>(p.a.q) + (there ? offset(row, p.a.q_token, p.a.q_head) : 0)),
+                       "r"(there ? 16 : 0)
+                       : "memory");
+          next_row(row);
         }
-#pragma unroll
+        asm volatile("cp.async.wait_all;" ::: "memory");  // each lane reads back what it copied itself
+#pragma unroll 4
         for (int x = 0; x < kSteps; ++x) {
-          const uint32_t v[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+          uint32_t v[4];
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(place(x)));
           float top = 0.0f;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[y])), fabsf(bf16_hi(v[y]))));
+          for (int y = 0; y < 4; ++y) top = max3(top, fabsf(bf16_lo(v[y])), fabsf(bf16_hi(v[y])));
 #pragma unroll
           for (int o = kRowLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 243);
           const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23 | (p.a.scale < 0.0f ? 0x80000000u : 0u));
           const float down = __uint_as_float(static_cast<uint32_t>(e - 10) << 23) * fabsf(p.a.scale) *
-                             (cap > 0.0f ? 1.0f / cap : kLog2e);
+                             (CAP ? 1.0f / cap : kLog2e);
           // to the thread that has the row
           const float mine = __shfl_sync(0xffffffffu, down, lane % kWarpRows * kRowLanes);
           if (lane / kWarpRows == x) row_scale = mine;
-          const int r = (warp & 3) * 32 + x * kWarpRows + sub;
           uint32_t h[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) h[y] = pack_half2(bf16_lo(v[y]) * up, bf16_hi(v[y]) * up);
-          *reinterpret_cast<uint4*>(smem + L::kQuery + w * L::kMatrix + part / 8 * L::kHalf + r * 128 +
-                                    (((part & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(x)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                       : "memory");
         }
         fence_proxy_async_smem();
       }
@@ -304,7 +333,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       // --- the tile's products, issued by its first warp
       constexpr uint32_t kScoreDesc = instr_desc(1, 0, 0, 0, 0, 128, kTokens);
       constexpr uint32_t kOutDesc = instr_desc(1, 0, 0, 0, 1, 128, DP);
-      const uint32_t base = smem_addr(smem);
       auto score = [&](int j) {  // S = Q K^T of token tile j; false: a wait gave up
         if (!wait_phase(&bars.k_full[j & 1], (j >> 1) & 1, ab, kErrSoftmaxWait)) return false;
         tc_fence_after();
@@ -401,9 +429,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         float top = exponents(up - ref);
         if (__any_sync(0xffffffffu, top > up + 4.0f || most > value_limit)) {
           top = exponents(0.0f);
-          int e = 0;
+          int e = kOpen ? static_cast<int>(__float_as_uint(most) >> 23) : 0;  // an open tile's tokens are all seen
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
+          for (int x = 0; x < (kOpen ? 0 : 8); ++x) {
             uint64_t v[2];
             lds_pairs(v, vs + x * 16);
 #pragma unroll
@@ -526,29 +554,30 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       // where DP / 8 lanes store each row
       uint8_t* room = smem + L::kQuery + w * L::kMatrix + (warp & 3) * 32 * DP * 2;
 #pragma unroll 1
-      for (int d = 0; d < DP; d += 16) {
-        uint32_t o[16];
+      for (int d = 0; d < DP; d += 32) {
+        uint32_t r[32];
         if (tiles > 0) {
-          tmem_ld_x16(result + d, o);
+          tmem_ld_32x32b_x32(result + d, r);
           tmem_wait_ld();
         }
-        uint32_t v[8];
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          v[x] = tiles > 0 ? pack_bf16(__uint_as_float(o[2 * x]) * over, __uint_as_float(o[2 * x + 1]) * over) : 0;
+        for (int h = 0; h < 4; ++h) {
+          uint32_t v[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint4*>(room + lane * DP * 2 + (((d / 8 + h) ^ (lane & 7)) << 4)) =
-              make_uint4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+          for (int x = 0; x < 4; ++x)
+            v[x] = tiles > 0 ? pack_bf16(__uint_as_float(r[8 * h + 2 * x]) * over, __uint_as_float(r[8 * h + 2 * x + 1]) * over) : 0;
+          *reinterpret_cast<uint4*>(room + lane * DP * 2 + (((d / 8 + h) ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
       }
       __syncwarp();
-#pragma unroll
+      Rows row = first_row();
+#pragma unroll 4
       for (int x = 0; x < kSteps; ++x) {
-        const int r = x * kWarpRows + sub;
-        const int64_t at = row_at(x, p.a.out_token, p.a.out_head);
-        if (at >= 0 && ok)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + at) =
-              *reinterpret_cast<const uint4*>(room + r * DP * 2 + ((part ^ (r & 7)) << 4));
+        const int at = x * kWarpRows + sub;
+        const uint4 v = *reinterpret_cast<const uint4*>(room + at * DP * 2 + ((part ^ (at & 7)) << 4));
+        if (row.at < work.rows && part_there && ok)
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + offset(row, p.a.out_token, p.a.out_head)) = v;
+        next_row(row);
       }
       tc_fence_before();
       if (issuer && *ab.flag) {
