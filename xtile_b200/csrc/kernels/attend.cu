@@ -13,9 +13,10 @@
 // line, and each warp of a grid that fills the GPU takes an equal run of it:
 // ragged lengths, a single long sequence and many short ones all load every SM
 // alike.  A warp works alone, without a CTA barrier: it streams its own tiles
-// with cp.async through its own ring in shared memory, runs the two products
-// on mma.sync m16n8k16 in f16 and keeps the running reference, sum and output
-// of its rows in registers.  Segments that several warps share are joined by a
+// through its own ring in shared memory (TMA boxes of 16 rows where pages hold
+// whole tiles, cp.async rows where they do not), runs the two products on
+// mma.sync m16n8k16 in f16 and keeps the running reference, sum and output of
+// its rows in registers.  Segments that several warps share are joined by a
 // second kernel from f32 partial results.
 //
 // Tokens (and the output's dims) are the products' m, query rows their n: the
@@ -30,6 +31,7 @@
 // products: the key's multiplies the score in f32, the value's the weight,
 // which is rounded once to f16 (11 bits) on its way into the second product.
 // f32 queries go in as two f16 terms, and so do their weights: 22 bits.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -38,30 +40,35 @@
 #include "attend.cuh"
 #include "batch.cuh"
 #include "pdl.cuh"
+#include "sm100.cuh"
 #include "vec.cuh"
 
 namespace xt {
 namespace dev {
 namespace {
 
+constexpr int kTile = 16;  // tokens of a unit: the products' m
+constexpr uint32_t kErrUnitWait = 0x307;
+
 // How one instance of the kernel is laid out.  DP: dims, padded; NR: n8 tiles
 // of query rows.
 template <int DP, bool F32, int NR>
 struct Shape {
   static constexpr int kRows = 8 * NR;  // query rows of a segment
-  static constexpr int kMTiles = 1;     // m16 tiles of tokens in a unit
-  static constexpr int kTile = 16 * kMTiles;
   static constexpr int kWarps = DP <= 128 ? 4 : 2;
   static constexpr bool kHeavy = F32 || NR == 4 || DP > 128;
-  static constexpr int kCtas = DP > 128 ? (F32 && NR > 1 ? 2 : 3) : kHeavy ? 2 : NR == 2 ? 3 : 4;  // CTAs an SM
-  static constexpr int kStageBytes = 2 * kTile * DP + 2 * kTile * 4;  // keys, values, their scales
-  static constexpr bool kQueryInSmem = kHeavy;                        // else its fragments stay in registers
+  static constexpr int kCtas = DP > 128 ? (F32 && NR > 1 ? 2 : 3) : kHeavy || (NR == 2 && DP == 128) ? 2 : NR == 2 ? 3 : 4;  // CTAs an SM
+  static constexpr int kMatrix = kTile * DP;             // a stage holds keys and values
+  static constexpr bool kQueryInSmem = kHeavy;           // else its fragments stay in registers
   static constexpr int kQueryBytes = kQueryInSmem ? (DP / 16) * NR * 256 * (F32 ? 2 : 1) : 0;
-  static constexpr int kSpare = 226 * 1024 / kCtas - 1024;            // shared memory of a CTA
-  static constexpr int kFit = (kSpare / kWarps - kQueryBytes) / kStageBytes;
-  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  // shared memory of a CTA: 1 KB is the system's, 1 KB alignment, 256 bytes barriers
+  static constexpr int kSpare = 227 * 1024 / kCtas - 2 * 1024 - 256;
+  static constexpr int kFit = (kSpare / kWarps - kQueryBytes) / (2 * kMatrix);
+  static constexpr int kStages = kFit < 4 ? kFit : 4;
   static_assert(kStages >= 3, "a warp's ring holds three stages at least");
-  static constexpr int kWarpBytes = kStages * kStageBytes + kQueryBytes;
+  static constexpr int kWarpBytes = kStages * 2 * kMatrix + kQueryBytes;
+  static_assert(kWarpBytes % 1024 == 0, "a ring starts on a swizzle atom");
+  static constexpr int kBytes = kWarps * kWarpBytes + 256 + 1024;
 };
 
 // The units of sequence b: kv heads x row tiles x token tiles [lo, hi).
@@ -73,17 +80,23 @@ struct Segments {
   }
 };
 
-template <int ROWS, int TILE>
+template <int ROWS>
 __device__ __forceinline__ Segments load_segments(const AttendDev& p, int b) {
   Segments g;
   g.seq = load_sequence(p.a.batch, p.a.cache.page, b);
   if (!g.seq.ok) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
   g.row_tiles = static_cast<int>((static_cast<int64_t>(g.seq.count) * p.group + ROWS - 1) / ROWS);
   const int64_t first_seen = p.a.window > 0 ? static_cast<int64_t>(g.seq.length) - g.seq.count - p.a.window + 1 : 0;
-  g.lo = first_seen > 0 ? static_cast<int>(first_seen) / TILE : 0;
-  g.hi = (g.seq.length + TILE - 1) / TILE;
+  g.lo = first_seen > 0 ? static_cast<int>(first_seen) / kTile : 0;
+  g.hi = (g.seq.length + kTile - 1) / kTile;
   if (g.lo > g.hi) g.lo = g.hi;
   return g;
+}
+
+// a / b of positive values; 64-bit division took a third of a microsecond.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
 
 __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
@@ -93,11 +106,11 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 }
 
 // Units of all sequences, and of those before ``b``.  A whole warp calls.
-template <int ROWS, int TILE>
+template <int ROWS>
 __device__ __forceinline__ int64_t count_units(const AttendDev& p, int b, int64_t* before) {
   int64_t total = 0, front = 0;
   for (int i = threadIdx.x & 31; i < p.a.batch.seqs; i += 32) {
-    const int64_t u = load_segments<ROWS, TILE>(p, i).units(p.a.cache.heads);
+    const int64_t u = load_segments<ROWS>(p, i).units(p.a.cache.heads);
     total += u;
     if (i < b) front += u;
   }
@@ -106,7 +119,7 @@ __device__ __forceinline__ int64_t count_units(const AttendDev& p, int b, int64_
 }
 
 // A place in the line of units.
-template <int ROWS, int TILE>
+template <int ROWS>
 struct Cursor {
   Segments seg;
   int b, head, row_tile, tile;
@@ -117,7 +130,7 @@ struct Cursor {
     b = 0;
     for (int base = 0; base < p.a.batch.seqs; base += 32) {
       const int i = base + lane;
-      const int64_t mine = i < p.a.batch.seqs ? load_segments<ROWS, TILE>(p, i).units(heads) : 0;
+      const int64_t mine = i < p.a.batch.seqs ? load_segments<ROWS>(p, i).units(heads) : 0;
       int64_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -133,11 +146,11 @@ struct Cursor {
       }
       front += __shfl_sync(0xffffffffu, upto, 31);
     }
-    seg = load_segments<ROWS, TILE>(p, b);
+    seg = load_segments<ROWS>(p, b);
     const int tiles = seg.hi - seg.lo;
-    const int64_t at = u - front, line = at / tiles;
+    const int64_t at = u - front, line = divide(at, tiles);
     tile = seg.lo + static_cast<int>(at - line * tiles);
-    head = static_cast<int>(line / seg.row_tiles);
+    head = static_cast<int>(divide(line, seg.row_tiles));
     row_tile = static_cast<int>(line - static_cast<int64_t>(head) * seg.row_tiles);
   }
 
@@ -151,7 +164,7 @@ struct Cursor {
     head = 0;
     do {
       ++b;
-      seg = load_segments<ROWS, TILE>(p, b);
+      seg = load_segments<ROWS>(p, b);
     } while (seg.units(1) == 0 && b + 1 < p.a.batch.seqs);
     tile = seg.lo;
   }
@@ -160,14 +173,9 @@ struct Cursor {
 __device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-// 4 bytes, or 4 zero bytes where ``bytes`` is 0.
-__device__ __forceinline__ void cp_async4(uint32_t to, const void* from, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrives on ``bar`` once the calling lane's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(sm100::smem_addr(bar)) : "memory");
 }
 
 // c += a b for 16 x 16 f16 a, 16 x 8 f16 b, f32 c.
@@ -192,17 +200,22 @@ __device__ __forceinline__ uint32_t rest_half2(float lo, float hi, uint32_t roun
   return pack_half2(lo - r.x, hi - r.y);
 }
 
-// Shared-memory places of 16-byte chunk ``c`` of a tile's token ``row``,
-// permuted so that the eight lanes of each quarter of a warp-wide 16-byte read
-// meet eight different bank groups: key reads take chunk 4 j + t of tokens g
-// (two tokens a quarter), value reads chunk g of tokens 2 t.
+// Shared-memory places of 16-byte chunk ``c`` of a tile's token ``row``: TMA's
+// swizzle of 128-byte rows (two halves of 16 rows at 256 dims) or 64-byte rows.
 template <int DP>
-__device__ __forceinline__ uint32_t key_place(int row, int c) {
-  return row * DP + ((DP >= 128 ? c ^ ((row & 1) << 2) : c) << 4);
+__device__ __forceinline__ uint32_t place(int row, int c) {
+  if constexpr (DP == 64) return row * 64 + ((c ^ (row >> 1 & 3)) << 4);
+  return (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
+
+// The token of a tile that row r (of 8) of the score product stands for; row
+// r + 8 is the one 8 behind it.  With that order the eight lanes of each
+// quarter of a 16-byte read meet eight different bank groups, both where keys
+// are read (chunks t .. of rows 2 q and 2 q + 1) and values (chunk 2 q or 2 q + 1
+// of rows 0, 2, 4, 6 or 1, 3, 5, 7).
 template <int DP>
-__device__ __forceinline__ uint32_t value_place(int row, int c) {
-  return row * DP + ((DP >= 128 ? c ^ (((row >> 1) & 3) << 1) : c ^ (((row >> 1) & 1) << 1)) << 4);
+__device__ __forceinline__ int token_of_row(int r) {
+  return DP == 64 ? r ^ (r >> 1 & 1) : r ^ ((r & 1) << 2);
 }
 
 __device__ __forceinline__ void lds128(uint32_t (&w)[4], uint32_t at) {
@@ -211,50 +224,65 @@ __device__ __forceinline__ void lds128(uint32_t (&w)[4], uint32_t at) {
 
 template <int DP, bool F32, int NR>
 __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32, NR>::kCtas)
-    attend_units(const __grid_constant__ AttendDev p) {
+    attend_units(const __grid_constant__ AttendDev p, const __grid_constant__ CUtensorMap key_map,
+                 const __grid_constant__ CUtensorMap value_map) {
   using S = Shape<DP, F32, NR>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-  constexpr int kTile = S::kTile, kMTiles = S::kMTiles, kRows = S::kRows;
+  constexpr int kRows = S::kRows, kStages = S::kStages;
   constexpr int kSteps = DP / 16;    // k16 steps of the score product
   constexpr int kOut = DP / 16;      // m16 tiles of the output
   constexpr int kChunks = DP / 16;   // 16-byte chunks of a token
   constexpr int kRowsAtOnce = 32 / kChunks;
   constexpr int kSpan = DP >= 128 ? 16 : 8;  // consecutive dims that a lane reads of a value row
-  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int kBox = DP < 128 ? DP : 128;  // bytes of a row in a TMA box
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   unsigned char* ring = smem + warp * S::kWarpBytes;
-  const uint32_t ring_addr = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  uint2* query = reinterpret_cast<uint2*>(ring + S::kStages * S::kStageBytes);
+  const uint32_t ring_addr = sm100::smem_addr(ring);
+  uint2* query = reinterpret_cast<uint2*>(ring + kStages * 2 * S::kMatrix);
+  uint64_t* landed = reinterpret_cast<uint64_t*>(smem + S::kWarps * S::kWarpBytes) + warp * kStages;  // a stage's data
+  int* abort_flag = reinterpret_cast<int*>(smem + S::kWarps * S::kWarpBytes + 128) + warp;
   const CacheView& cache = p.a.cache;
   const int dim = cache.dim;
+  // where pages hold whole tiles, a tile is one run of rows and comes by TMA
+  const bool one_page = p.by_tma;
 
-  // chunks behind dim are never loaded; they stay zero
-  if (dim < DP) {
-    for (int i = lane; i < S::kStages * S::kStageBytes / 16; i += 32)
+  if (!one_page && dim < DP) {
+    // chunks behind dim are never loaded by cp.async; they stay zero
+    for (int i = lane; i < kStages * 2 * S::kMatrix / 16; i += 32)
       reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
-    __syncwarp();
   }
-  griddep_launch_dependents();
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&landed[i], one_page ? 1 : 32);
+    *abort_flag = 0;
+    sm100::fence_barrier_init();
+  }
+  __syncwarp();
   griddep_wait();
+  // behind the wait: what the join reads before its own wait is final, then
+  griddep_launch_dependents();
 
   int64_t unused;
-  const int64_t total = count_units<kRows, kTile>(p, 0, &unused);
-  const int64_t per = (total + p.workers - 1) / p.workers;
+  const int64_t total = count_units<kRows>(p, 0, &unused);
+  const int64_t per = divide(total + p.workers - 1, p.workers);
   const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
   const int64_t begin = worker * per;
   if (begin >= total) return;
   int left = static_cast<int>(total - begin < per ? total - begin : per);  // units to do, and to issue
   int to_issue = left;
 
-  Cursor<kRows, kTile> at;
+  Cursor<kRows> at;
   at.seek(p, begin);
-  Cursor<kRows, kTile> ahead = at;
+  Cursor<kRows> ahead = at;
 
-  // --- loading.  Where pages hold whole tiles (page a multiple of kTile) a tile
-  // is one run of rows; else lane l % kTile looks up token l of the tile.
-  const bool one_page = cache.page % kTile == 0;
+  // --- loading.  Lane l looks up the page of token l % 16 of the tile to come
+  // (of its first token where pages hold whole tiles), and holds the scale of
+  // that token's keys (lanes 0 to 15) or values of each tile under way.
   const int my_chunk = lane % kChunks, my_row = lane / kChunks;
+  const float* my_scales = lane < kTile ? cache.k_scale : cache.v_scale;
+  float scale[kStages - 1];  // oldest first
   int page_id = 0, page_row = 0;
   auto look_up = [&] {
     const int token = ahead.tile * kTile + (one_page ? 0 : lane % kTile);
@@ -263,67 +291,63 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
     page_id = token < ahead.seg.seq.length ? p.a.batch.table[ahead.b * p.a.batch.table_stride + index] : 0;
   };
   auto issue = [&](int stage) {
+    float s = 0.0f;
     if (to_issue > 0) {
-      const uint32_t base = ring_addr + stage * S::kStageBytes;
-      const int there = min(ahead.seg.seq.length - ahead.tile * kTile, kTile);  // tokens of the tile
+      const uint32_t base = ring_addr + stage * 2 * S::kMatrix;
+      const int there = ahead.seg.seq.length - ahead.tile * kTile;  // tokens of the tile: 16 of them, or fewer
       const bool bad = page_id < 0 || page_id >= cache.pages;
-      const int64_t line = static_cast<int64_t>(bad ? 0 : page_id) * cache.heads + ahead.head;
-      const int64_t row_at = line * cache.page + page_row;
-      // the scales: a lane a token, keys' and values'
-#pragma unroll
-      for (int i = 0; i < 2 * kTile / 32; ++i) {
-        const int slot = i * 32 + lane, token = slot % kTile;
-        const int row = page_row + (one_page ? token : 0);
-        const int64_t scale_at = line * p.blocks + p.block_div.quot(row);
-        const uint32_t to = base + 2 * kTile * DP + slot * 4;
-        const bool mine = token < there;
-        if (mine && bad) {
+      const int line = (bad ? 0 : page_id) * cache.heads + ahead.head;
+      if (lane % kTile < there) {
+        if (bad) {
           // a page outside the cache: recorded, and NaN for whoever attends to it
           atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(0x7fc00000u) : "memory");
+          s = __int_as_float(0x7fc00000);
         } else {
-          cp_async4(to, (slot < kTile ? cache.k_scale : cache.v_scale) + (mine ? scale_at : 0), mine ? 4 : 0);
+          const int row = page_row + (one_page ? lane % kTile : 0);
+          s = my_scales[static_cast<uint64_t>(static_cast<uint32_t>(line)) * static_cast<uint32_t>(p.blocks) + p.block_div.quot(row)];
         }
       }
-      // Rows behind the sequence's end, and of a bad page, are left as they are:
-      // finite int8, and their weight is 0 or NaN.
+      // Rows behind the sequence's end are whatever the page or the ring holds:
+      // finite int8, and their weight is 0.  So are a bad page's, with NaN.
       if (one_page) {
-        const int rows = bad || my_chunk * 16 >= dim ? 0 : there;
-        const int64_t from = (row_at + my_row) * dim + my_chunk * 16;
-        const int8_t* k = cache.k + from;
-        const int8_t* v = cache.v + from;
+        if (lane == 0) {
+          if (bad) {
+            sm100::mbar_arrive(&landed[stage]);
+          } else {
+            const int row = line * cache.page + page_row;
+            sm100::mbar_arrive_expect_tx(&landed[stage], 2 * S::kMatrix);
+            unsigned char* to = ring + stage * 2 * S::kMatrix;
 #pragma unroll
-        for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-          const int row = i * kRowsAtOnce + my_row;
-          if (row < rows) {
-            cp_async16(base + key_place<DP>(row, my_chunk), k);
-            cp_async16(base + kTile * DP + value_place<DP>(row, my_chunk), v);
+            for (int h = 0; h < DP / kBox; ++h) {
+              sm100::tma_load_2d(to + h * kTile * kBox, &key_map, &landed[stage], h * kBox, row);
+              sm100::tma_load_2d(to + S::kMatrix + h * kTile * kBox, &value_map, &landed[stage], h * kBox, row);
+            }
           }
-          k += kRowsAtOnce * dim;
-          v += kRowsAtOnce * dim;
         }
       } else {
+        const int64_t row_at = static_cast<int64_t>(line) * cache.page + page_row;
         const unsigned rows_there = __ballot_sync(0xffffffffu, lane % kTile < there && !bad);
 #pragma unroll
         for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
           const int row = i * kRowsAtOnce + my_row;
           const int64_t from = __shfl_sync(0xffffffffu, row_at, row) * dim + my_chunk * 16;
           if (my_chunk * 16 < dim && (rows_there >> row & 1)) {
-            cp_async16(base + key_place<DP>(row, my_chunk), cache.k + from);
-            cp_async16(base + kTile * DP + value_place<DP>(row, my_chunk), cache.v + from);
+            cp_async16(base + place<DP>(row, my_chunk), cache.k + from);
+            cp_async16(base + S::kMatrix + place<DP>(row, my_chunk), cache.v + from);
           }
         }
+        cp_async_arrive(&landed[stage]);
       }
       if (--to_issue > 0) {
         ahead.advance(p);
         look_up();
       }
     }
-    cp_async_commit();
+    return s;
   };
   look_up();
 #pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) issue(i);
+  for (int i = 0; i < kStages - 1; ++i) scale[i] = issue(i);
 
   // --- the segment at hand
   uint2 qf[S::kQueryInSmem ? 1 : NR][S::kQueryInSmem ? 1 : kSteps];
@@ -454,48 +478,57 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   };
 
   start_segment();
+  // what the lane reads of a tile: keys of tokens (row g) and 8 behind, values
+  // of tokens (rows 2 t and 2 t + 1) and 8 behind
+  const int key_row = token_of_row<DP>(g);
+  const uint32_t key_at = place<DP>(key_row, t);
+  const uint32_t value_at[2] = {place<DP>(token_of_row<DP>(2 * t), DP == 64 ? g >> 1 : g) + (DP == 64 ? (g & 1) * 8 : 0),
+                                place<DP>(token_of_row<DP>(2 * t + 1), DP == 64 ? g >> 1 : g) + (DP == 64 ? (g & 1) * 8 : 0)};
+  constexpr int kEight = 8 * kBox;  // eight rows on
+  const sm100::Abort ab{abort_flag, p.a.error_word, sm100::kWaitLimitCycles};
   int stage = 0;
+  uint32_t phase = 0;
   while (true) {
-    cp_async_wait<S::kStages - 2>();
-    __syncwarp();
-    issue(stage == 0 ? S::kStages - 1 : stage - 1);
-    const uint32_t keys = ring_addr + stage * S::kStageBytes;
-    const uint32_t values = keys + kTile * DP;
-    const float* scales = reinterpret_cast<const float*>(ring + stage * S::kStageBytes + 2 * kTile * DP);
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(&landed[stage], phase, ab, kErrUnitWait))) break;
+    __syncwarp();  // every lane has read the stage before this one
+    const float scales = scale[0];
+#pragma unroll
+    for (int i = 0; i < kStages - 2; ++i) scale[i] = scale[i + 1];
+    scale[kStages - 2] = issue(stage == 0 ? kStages - 1 : stage - 1);
+    const uint32_t keys = ring_addr + stage * 2 * S::kMatrix;
+    const uint32_t values = keys + S::kMatrix;
 
-    // --- scores: token rows g and g + 8 of each m16 tile
-    float z[kMTiles][NR][4];
+    // --- scores: rows g and g + 8 of the tile's tokens
+    float z[NR][4];
 #pragma unroll
-    for (int m = 0; m < kMTiles; ++m) {
+    for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
+      for (int e = 0; e < 4; ++e) z[nr][e] = start[nr][e & 1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[m][nr][e] = start[nr][e & 1];
+    for (int j = 0; j < DP / 64; ++j) {
+      uint32_t u[4], w[4];
+      const uint32_t from = keys + (key_at ^ ((j & 1) << 6)) + (j >> 1) * kTile * 128;
+      lds128(u, from);
+      lds128(w, from + kEight);
 #pragma unroll
-      for (int j = 0; j < DP / 64; ++j) {
-        uint32_t u[4], w[4];
-        lds128(u, keys + key_place<DP>(16 * m + g, 4 * j + t));
-        lds128(w, keys + key_place<DP>(16 * m + g + 8, 4 * j + t));
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t x = u[s] ^ 0x80808080u, y = w[s] ^ 0x80808080u;
+        const int step = 4 * j + s;
+        uint32_t a0, a1, a2, a3;
+        if constexpr (F32) {
+          a0 = bytes_to_half2<kLow>(x), a2 = bytes_to_half2<kHigh>(x);
+          a1 = bytes_to_half2<kLow>(y), a3 = bytes_to_half2<kHigh>(y);
+        } else {
+          a0 = __byte_perm(x, 0, kLow), a2 = __byte_perm(x, 0, kHigh);
+          a1 = __byte_perm(y, 0, kLow), a3 = __byte_perm(y, 0, kHigh);
+        }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const uint32_t x = u[s] ^ 0x80808080u, y = w[s] ^ 0x80808080u;
-          const int step = 4 * j + s;
-          uint32_t a0, a1, a2, a3;
-          if constexpr (F32) {
-            a0 = bytes_to_half2<kLow>(x), a2 = bytes_to_half2<kHigh>(x);
-            a1 = bytes_to_half2<kLow>(y), a3 = bytes_to_half2<kHigh>(y);
+        for (int nr = 0; nr < NR; ++nr) {
+          if constexpr (S::kQueryInSmem) {
+            mma_16816(z[nr], a0, a1, a2, a3, query[(nr * kSteps + step) * 32 + lane]);
+            if constexpr (F32) mma_16816(z[nr], a0, a1, a2, a3, query[((NR + nr) * kSteps + step) * 32 + lane]);
           } else {
-            a0 = __byte_perm(x, 0, kLow), a2 = __byte_perm(x, 0, kHigh);
-            a1 = __byte_perm(y, 0, kLow), a3 = __byte_perm(y, 0, kHigh);
-          }
-#pragma unroll
-          for (int nr = 0; nr < NR; ++nr) {
-            if constexpr (S::kQueryInSmem) {
-              mma_16816(z[m][nr], a0, a1, a2, a3, query[(nr * kSteps + step) * 32 + lane]);
-              if constexpr (F32) mma_16816(z[m][nr], a0, a1, a2, a3, query[((NR + nr) * kSteps + step) * 32 + lane]);
-            } else {
-              mma_16816(z[m][nr], a0, a1, a2, a3, qf[nr][step]);
-            }
+            mma_16816(z[nr], a0, a1, a2, a3, qf[nr][step]);
           }
         }
       }
@@ -506,66 +539,52 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
     const int token0 = at.tile * kTile;
     // every row sees all of the tile's tokens
     const bool open = token0 + kTile - 1 <= pos_min && (p.a.window == 0 || token0 > pos_max - p.a.window);
-    float vs[kMTiles][2], y[kMTiles][NR][4];
+    const float ks[2] = {__shfl_sync(0xffffffffu, scales, key_row), __shfl_sync(0xffffffffu, scales, key_row + 8)};
+    const float vs[2] = {__shfl_sync(0xffffffffu, scales, key_row + 16), __shfl_sync(0xffffffffu, scales, key_row + 24)};
+    float y[NR][4];
 #pragma unroll
-    for (int m = 0; m < kMTiles; ++m) {
-      const float k0 = scales[16 * m + g], k1 = scales[16 * m + g + 8];
-      vs[m][0] = scales[kTile + 16 * m + g], vs[m][1] = scales[kTile + 16 * m + g + 8];
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[nr][e] *= ks[e >> 1];
+    if (cap > 0.0f) {
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[m][nr][e] *= e < 2 ? k0 : k1;
-    }
-    if (cap > 0.0f) {
-#pragma unroll
-      for (int m = 0; m < kMTiles; ++m)
-#pragma unroll
-        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            z[m][nr][e] = tanhf(z[m][nr][e] * capped_scale[nr][e & 1]) * (cap * kLog2e);
+        for (int e = 0; e < 4; ++e) z[nr][e] = tanhf(z[nr][e] * capped_scale[nr][e & 1]) * (cap * kLog2e);
     }
     auto exponents = [&] {
       float top = -INFINITY;
 #pragma unroll
-      for (int m = 0; m < kMTiles; ++m)
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[m][nr][e] = fmaf(z[m][nr][e], row_scale[nr][e & 1], -ref[nr][e & 1]);
-            if (!open) {
-              const int j = token0 + 16 * m + g + 8 * (e >> 1), pos = row_pos[nr][e & 1];
-              if (j > pos || (p.a.window > 0 && j <= pos - p.a.window)) y[m][nr][e] = -INFINITY;
-            }
-            top = fmaxf(top, y[m][nr][e]);
+        for (int e = 0; e < 4; ++e) {
+          y[nr][e] = fmaf(z[nr][e], row_scale[nr][e & 1], -ref[nr][e & 1]);
+          if (!open) {
+            const int j = token0 + key_row + 8 * (e >> 1), pos = row_pos[nr][e & 1];
+            if (j > pos || (p.a.window > 0 && j <= pos - p.a.window)) y[nr][e] = -INFINITY;
           }
+          top = fmaxf(top, y[nr][e]);
+        }
       return top;
     };
     const float top = exponents();
     float shift = __uint_as_float(static_cast<uint32_t>(137 - value_exp) << 23);
-    float most = 0.0f;
-#pragma unroll
-    for (int m = 0; m < kMTiles; ++m) most = fmaxf(most, fmaxf(vs[m][0], vs[m][1]));
     // The reference of a row's exponents follows its maximum only when that has
     // risen by more than 2^4, and the values' scales enter the weights as
     // multiples of a power of two that the first scales seen set and that
     // changes only where a weight could leave f16's range: most units leave
     // the output as it is.  2^10 of room below the largest weights keeps f16's
     // subnormals (2^-24 apart) at 2^-34 of them.
-    if (__any_sync(0xffffffffu, top > 4.0f || most * shift > 2048.0f || !value_set)) {
+    if (__any_sync(0xffffffffu, top > 4.0f || fmaxf(vs[0], vs[1]) * shift > 2048.0f || !value_set)) {
       int e = 0;
 #pragma unroll
-      for (int m = 0; m < kMTiles; ++m)
+      for (int r = 0; r < 2; ++r) {
+        float seen = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float seen = -INFINITY;
-#pragma unroll
-          for (int nr = 0; nr < NR; ++nr)
-            seen = fmaxf(seen, fmaxf(y[m][nr][2 * r], y[m][nr][2 * r + 1]));
-          const int b = static_cast<int>(__float_as_uint(vs[m][r]) >> 23 & 255);
-          if (seen > -INFINITY && b < 255) e = max(e, b);
-        }
+        for (int nr = 0; nr < NR; ++nr) seen = fmaxf(seen, fmaxf(y[nr][2 * r], y[nr][2 * r + 1]));
+        const int b = static_cast<int>(__float_as_uint(vs[r]) >> 23 & 255);
+        if (seen > -INFINITY && b < 255) e = max(e, b);
+      }
       e = __reduce_max_sync(0xffffffffu, e);
       float fall = 1.0f;
       if (e > 0) {
@@ -583,20 +602,15 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float rise = -INFINITY;
-#pragma unroll
-          for (int m = 0; m < kMTiles; ++m) rise = fmaxf(rise, fmaxf(y[m][nr][c], y[m][nr][c + 2]));
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) rise = fmaxf(rise, __shfl_xor_sync(0xffffffffu, rise, x));
-          const float by = row_scale[nr][c];
+          float rise = fmaxf(y[nr][c], y[nr][c + 2]);
           float best = -INFINITY;
+          if (y[nr][c] > -INFINITY) best = fmaxf(best, z[nr][c] * row_scale[nr][c]);
+          if (y[nr][c + 2] > -INFINITY) best = fmaxf(best, z[nr][c + 2] * row_scale[nr][c]);
 #pragma unroll
-          for (int m = 0; m < kMTiles; ++m) {
-            if (y[m][nr][c] > -INFINITY) best = fmaxf(best, z[m][nr][c] * by);
-            if (y[m][nr][c + 2] > -INFINITY) best = fmaxf(best, z[m][nr][c + 2] * by);
+          for (int x = 4; x < 32; x <<= 1) {
+            rise = fmaxf(rise, __shfl_xor_sync(0xffffffffu, rise, x));
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
           }
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
           float f = 1.0f;
           if (rise > 0.0f) {
             f = exp2_fast(ref[nr][c] - best);
@@ -612,130 +626,133 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
         }
       exponents();
     }
-    uint2 wf[kMTiles][NR], wl[F32 ? kMTiles : 1][F32 ? NR : 1];
+    uint2 wf[NR], wl[F32 ? NR : 1];
+    const float v0 = vs[0] * shift, v1 = vs[1] * shift;
 #pragma unroll
-    for (int m = 0; m < kMTiles; ++m) {
-      const float v0 = vs[m][0] * shift, v1 = vs[m][1] * shift;
+    for (int nr = 0; nr < NR; ++nr) {
+      float w[4];
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float weight = exp2_fast(y[m][nr][e]);
-          sum[nr][e & 1] += weight;
-          w[e] = weight * (e < 2 ? v0 : v1);
-          // a token that is not seen may have any scale
-          if (!open && y[m][nr][e] == -INFINITY) w[e] = 0.0f;
-        }
-        const uint32_t a = pack_half2(w[0], w[1]), b = pack_half2(w[2], w[3]);
-        wf[m][nr] = make_uint2(transpose_8x8(a), transpose_8x8(b));
-        if constexpr (F32)
-          wl[m][nr] = make_uint2(transpose_8x8(rest_half2(w[0], w[1], a)), transpose_8x8(rest_half2(w[2], w[3], b)));
+      for (int e = 0; e < 4; ++e) {
+        const float weight = exp2_fast(y[nr][e]);
+        sum[nr][e & 1] += weight;
+        w[e] = weight * (e < 2 ? v0 : v1);
+        // a token that is not seen may have any scale
+        if (!open && y[nr][e] == -INFINITY) w[e] = 0.0f;
       }
+      const uint32_t a = pack_half2(w[0], w[1]), b = pack_half2(w[2], w[3]);
+      wf[nr] = make_uint2(transpose_8x8(a), transpose_8x8(b));
+      if constexpr (F32)
+        wl[nr] = make_uint2(transpose_8x8(rest_half2(w[0], w[1], a)), transpose_8x8(rest_half2(w[2], w[3], b)));
     }
 
-    // --- output: the lane's tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each m16 tile
+    // --- output
     constexpr int kWords = kSpan / 4;  // words of a token that one read brings
 #pragma unroll
     for (int h = 0; h < DP / (8 * kSpan); ++h) {
+      uint32_t v[4][4];
 #pragma unroll
-      for (int m = 0; m < kMTiles; ++m) {
-        uint32_t v[4][4];
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t from = values + value_at[i & 1] + (i >> 1) * kEight + h * kTile * 128;
+        if constexpr (DP >= 128)
+          lds128(v[i], from);
+        else
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[i][0]), "=r"(v[i][1]) : "r"(from));
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 16 * m + 2 * t + (i & 1) + 8 * (i >> 1);
-          if constexpr (DP >= 128) {
-            lds128(v[i], values + value_place<DP>(row, 8 * h + g));
-          } else {
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                         : "=r"(v[i][0]), "=r"(v[i][1])
-                         : "r"(values + value_place<DP>(row, g >> 1) + (g & 1) * 8));
-          }
-        }
+      for (int k = 0; k < kWords; ++k) {
 #pragma unroll
-        for (int k = 0; k < kWords; ++k) {
+        for (int half = 0; half < 2; ++half) {
+          // bytes 2 half and 2 half + 1 of two tokens, side by side
+          const uint32_t a = __byte_perm(v[0][k], v[1][k], half ? 0x7362u : 0x5140u) ^ 0x80808080u;
+          const uint32_t b = __byte_perm(v[2][k], v[3][k], half ? 0x7362u : 0x5140u) ^ 0x80808080u;
+          const uint32_t a0 = bytes_to_half2<kLow>(a), a1 = bytes_to_half2<kHigh>(a);
+          const uint32_t a2 = bytes_to_half2<kLow>(b), a3 = bytes_to_half2<kHigh>(b);
+          const int i = h * kSpan / 2 + 2 * k + half;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            // bytes 2 half and 2 half + 1 of two tokens, side by side
-            const uint32_t a = __byte_perm(v[0][k], v[1][k], half ? 0x7362u : 0x5140u) ^ 0x80808080u;
-            const uint32_t b = __byte_perm(v[2][k], v[3][k], half ? 0x7362u : 0x5140u) ^ 0x80808080u;
-            const uint32_t a0 = bytes_to_half2<kLow>(a), a1 = bytes_to_half2<kHigh>(a);
-            const uint32_t a2 = bytes_to_half2<kLow>(b), a3 = bytes_to_half2<kHigh>(b);
-            const int i = h * kSpan / 2 + 2 * k + half;
+          for (int nr = 0; nr < NR; ++nr) {
+            if constexpr (F32) {
+              // a fresh sum for the tile, added in f32: the tensor cores' own sums round toward zero
+              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma_16816(c, a0, a1, a2, a3, wl[nr]);
+              mma_16816(c, a0, a1, a2, a3, wf[nr]);
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-              if constexpr (F32) {
-                // a fresh sum for the tile, added in f32: the tensor cores' own sums round toward zero
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma_16816(c, a0, a1, a2, a3, wl[m][nr]);
-                mma_16816(c, a0, a1, a2, a3, wf[m][nr]);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[i][nr][x] += c[x];
-              } else {
-                mma_16816(o[i][nr], a0, a1, a2, a3, wf[m][nr]);
-              }
+              for (int x = 0; x < 4; ++x) o[i][nr][x] += c[x];
+            } else {
+              mma_16816(o[i][nr], a0, a1, a2, a3, wf[nr]);
             }
           }
         }
       }
     }
-    stage = stage == S::kStages - 1 ? 0 : stage + 1;
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
 
     const bool last_unit = at.tile + 1 == at.seg.hi;
     --left;
     if (last_unit || left == 0) {
       finish_segment(last_unit);
-      if (left == 0) break;
+      if (left == 0) return;
       at.advance(p);
       start_segment();
     } else {
       ++at.tile;
     }
   }
-  cp_async_wait<0>();
+  // a wait gave up: what is under way lands before the memory goes
+  for (int i = 0; i < kStages - 1 && left - to_issue > i; ++i) {
+    sm100::mbar_wait_drain(&landed[stage], phase, 500000000ull);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
 }
 
 // Joins the partial results of the segments that several workers had.  WARPS
 // warps have one (new token, query head): each takes every WARPS-th partial.
-template <class T, int DP, int ROWS, int TILE, int WARPS>
+template <class T, int DP, int ROWS, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(const __grid_constant__ AttendDev p) {
   constexpr int kPer = DP / 32;  // dims a lane
   __shared__ float shared_o[WARPS == 1 ? 1 : WARPS][WARPS == 1 ? 1 : DP];
   __shared__ float2 shared_ml[WARPS];
+  // The batch's tables were final before attend_units let this grid start, so
+  // they are read before the wait for its results.  Every thread waits, also
+  // those with nothing to join: what follows this grid counts on attend_units
+  // being done.
   griddep_launch_dependents();
-  griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t index = WARPS == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + warp : blockIdx.x;
-  if (index >= static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads) return;
-  const int token = static_cast<int>(index / p.a.q_heads), q_head = static_cast<int>(index % p.a.q_heads);
+  if (index >= static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads) {
+    griddep_wait();
+    return;
+  }
+  const int token = static_cast<int>(static_cast<uint32_t>(index) / static_cast<uint32_t>(p.a.q_heads));
+  const int q_head = static_cast<int>(index) - token * p.a.q_heads;
   const int b = last_at_most(p.a.batch.seqs, token, [&](int i) { return static_cast<int64_t>(p.a.batch.starts[i]); });
-  const Segments seg = load_segments<ROWS, TILE>(p, b);
-  const int i = token - seg.seq.first;
+  const Segments seg = load_segments<ROWS>(p, b);
+  const int i = token - seg.seq.first, tiles = seg.hi - seg.lo;
+  const int head = p.group_div.quot(q_head);
+  const int packed = i * p.group + q_head - head * p.group;
+  const bool mine_to_join = seg.seq.ok && i >= 0 && i < seg.seq.count && tiles > 0;
+  int64_t first = 0, last = 0;
+  if (mine_to_join) {
+    int64_t front;
+    const int64_t total = count_units<ROWS>(p, b, &front);
+    const int64_t per = divide(total + p.workers - 1, p.workers);
+    const int64_t u0 = front + (static_cast<int64_t>(head) * seg.row_tiles + packed / ROWS) * tiles;
+    first = divide(u0, per), last = divide(u0 + tiles - 1, per);
+  }
+  griddep_wait();
   T* out = static_cast<T*>(p.a.out) + static_cast<int64_t>(token) * p.a.out_token + static_cast<int64_t>(q_head) * p.a.out_head;
-  if (!seg.seq.ok) {
-    // its table is wrong: recorded, and its rows are NaN
-    for (int d = lane; d < p.a.cache.dim; d += 32) {
-      const float nan[1] = {__int_as_float(0x7fc00000)};
-      Vec<T, 1>::store(out + d, nan);
-    }
+  if (!mine_to_join) {
+    if (seg.seq.ok && (i < 0 || i >= seg.seq.count)) return;  // a row of no sequence
+    // no token at all: 0; a wrong table: recorded, and NaN
+    const float v[1] = {seg.seq.ok ? 0.0f : __int_as_float(0x7fc00000)};
+    for (int d = lane; d < p.a.cache.dim; d += 32) Vec<T, 1>::store(out + d, v);
     return;
   }
-  if (i < 0 || i >= seg.seq.count) return;  // a row of no sequence
-  int64_t front;
-  const int64_t total = count_units<ROWS, TILE>(p, b, &front);
-  const int64_t per = (total + p.workers - 1) / p.workers;
-  const int head = q_head / p.group;
-  const int packed = i * p.group + q_head % p.group;
-  const int tiles = seg.hi - seg.lo;
-  if (tiles == 0) {
-    for (int d = lane; d < p.a.cache.dim; d += 32) {
-      const float zero[1] = {0.0f};
-      Vec<T, 1>::store(out + d, zero);
-    }
-    return;
-  }
-  const int64_t u0 = front + (static_cast<int64_t>(head) * seg.row_tiles + packed / ROWS) * tiles;
-  const int64_t first = u0 / per, last = (u0 + tiles - 1) / per;
   if (first == last) return;  // one worker had it all, and has written it
   const int row = packed % ROWS, dim = p.a.cache.dim;
   auto slot_of = [&](int64_t c) { return (c * 2 + (c == first ? 1 : 0)) * ROWS + row; };
@@ -817,6 +834,23 @@ int sm_count() {
   return sms;
 }
 
+// A tensor map of ``lines`` rows of ``dim`` bytes whose boxes are 16 rows of up
+// to 128 bytes, swizzled as place() has it; bytes behind dim read as zeros.
+bool cache_map(CUtensorMap* map, const void* base, int dim, uint64_t lines, int padded) {
+  typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  auto encode = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(dim), lines};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(dim)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(padded < 128 ? padded : 128), kTile};
+  const cuuint32_t step[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, padded < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DP, bool F32, int NR>
 cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   using S = Shape<DP, F32, NR>;
@@ -829,21 +863,28 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   }
   p.part = static_cast<float*>(p.a.workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part + p.workers * 2 * S::kRows * dim);
-  constexpr int kSmem = S::kWarps * S::kWarpBytes;
+  // boxes of a tile's rows, as bytes
+  CUtensorMap maps[2] = {};
+  const uint64_t lines = static_cast<uint64_t>(p.a.cache.pages) * p.a.cache.heads * p.a.cache.page;
+  p.by_tma = p.a.cache.page % kTile == 0 && lines <= 0x7fffffff;  // a box's row is a 32-bit coordinate
+  if (p.by_tma) {
+    if (!cache_map(&maps[0], p.a.cache.k, dim, lines, DP) || !cache_map(&maps[1], p.a.cache.v, dim, lines, DP))
+      return cudaErrorInvalidValue;
+  }
   static std::atomic<bool> allowed[kMaxDevices];
-  cudaError_t e = allow_smem(attend_units<DP, F32, NR>, kSmem, allowed);
+  cudaError_t e = allow_smem(attend_units<DP, F32, NR>, S::kBytes, allowed);
   if (e != cudaSuccess) return e;
-  PdlLaunch launch(dim3(static_cast<unsigned>(sms * S::kCtas)), dim3(S::kWarps * 32), kSmem, stream);
-  e = launch(attend_units<DP, F32, NR>, p);
+  PdlLaunch launch(dim3(static_cast<unsigned>(sms * S::kCtas)), dim3(S::kWarps * 32), S::kBytes, stream);
+  e = launch(attend_units<DP, F32, NR>, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
   const int64_t rows = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
   // a row's partials are spread over eight warps where the rows alone would not fill the GPU
   if (rows <= 4 * sms) {
     PdlLaunch join(dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream);
-    return join(attend_join<T, DP, S::kRows, S::kTile, 8>, p);
+    return join(attend_join<T, DP, S::kRows, 8>, p);
   }
   PdlLaunch join(dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream);
-  return join(attend_join<T, DP, S::kRows, S::kTile, 1>, p);
+  return join(attend_join<T, DP, S::kRows, 1>, p);
 }
 
 // New tokens of a sequence, as far as the caller knows; else their mean.
