@@ -57,7 +57,9 @@ struct Shape {
   static constexpr int kRows = 8 * NR;  // query rows of a segment
   static constexpr int kWarps = DP <= 128 ? 4 : 2;
   static constexpr bool kHeavy = F32 || NR == 4 || DP > 128;
-  static constexpr int kCtas = DP > 128 ? (F32 && NR > 1 ? 2 : 3) : kHeavy || (NR == 2 && DP == 128) ? 2 : NR == 2 ? 3 : 4;  // CTAs an SM
+  static constexpr int kCtas = DP > 128               ? (F32 && NR > 1 ? 2 : 3)  // CTAs an SM, by the registers of a row and dim
+                               : DP * NR * (F32 ? 2 : 1) <= 128 ? (F32 || NR > 1 ? 3 : 4)
+                                                                : 2;
   static constexpr int kMatrix = kTile * DP;             // a stage holds keys and values
   static constexpr bool kQueryInSmem = kHeavy;           // else its fragments stay in registers
   static constexpr int kQueryBytes = kQueryInSmem ? (DP / 16) * NR * 256 * (F32 ? 2 : 1) : 0;
@@ -154,19 +156,20 @@ struct Cursor {
     row_tile = static_cast<int>(line - static_cast<int64_t>(head) * seg.row_tiles);
   }
 
-  // The next unit; there must be one.
-  __device__ __forceinline__ void advance(const AttendDev& p) {
-    if (++tile < seg.hi) return;
+  // The next unit; there must be one.  True if it is of the same segment.
+  __device__ __forceinline__ bool advance(const AttendDev& p) {
+    if (++tile < seg.hi) return true;
     tile = seg.lo;
-    if (++row_tile < seg.row_tiles) return;
+    if (++row_tile < seg.row_tiles) return false;
     row_tile = 0;
-    if (++head < p.a.cache.heads) return;
+    if (++head < p.a.cache.heads) return false;
     head = 0;
     do {
       ++b;
       seg = load_segments<ROWS>(p, b);
     } while (seg.units(1) == 0 && b + 1 < p.a.batch.seqs);
     tile = seg.lo;
+    return false;
   }
 };
 
@@ -222,7 +225,7 @@ __device__ __forceinline__ void lds128(uint32_t (&w)[4], uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
 }
 
-template <int DP, bool F32, int NR>
+template <int DP, bool F32, int NR, bool TMA>
 __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32, NR>::kCtas)
     attend_units(const __grid_constant__ AttendDev p, const __grid_constant__ CUtensorMap key_map,
                  const __grid_constant__ CUtensorMap value_map) {
@@ -231,8 +234,6 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   constexpr int kRows = S::kRows, kStages = S::kStages;
   constexpr int kSteps = DP / 16;    // k16 steps of the score product
   constexpr int kOut = DP / 16;      // m16 tiles of the output
-  constexpr int kChunks = DP / 16;   // 16-byte chunks of a token
-  constexpr int kRowsAtOnce = 32 / kChunks;
   constexpr int kSpan = DP >= 128 ? 16 : 8;  // consecutive dims that a lane reads of a value row
   constexpr int kBox = DP < 128 ? DP : 128;  // bytes of a row in a TMA box
   extern __shared__ unsigned char smem_raw[];
@@ -246,16 +247,14 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   int* abort_flag = reinterpret_cast<int*>(smem + S::kWarps * S::kWarpBytes + 128) + warp;
   const CacheView& cache = p.a.cache;
   const int dim = cache.dim;
-  // where pages hold whole tiles, a tile is one run of rows and comes by TMA
-  const bool one_page = p.by_tma;
 
-  if (!one_page && dim < DP) {
+  if (!TMA && dim < DP) {
     // chunks behind dim are never loaded by cp.async; they stay zero
     for (int i = lane; i < kStages * 2 * S::kMatrix / 16; i += 32)
       reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
   }
   if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&landed[i], one_page ? 1 : 32);
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&landed[i], TMA ? 1 : 32);
     *abort_flag = 0;
     sm100::fence_barrier_init();
   }
@@ -277,75 +276,92 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   at.seek(p, begin);
   Cursor<kRows> ahead = at;
 
-  // --- loading.  Lane l looks up the page of token l % 16 of the tile to come
-  // (of its first token where pages hold whole tiles), and holds the scale of
-  // that token's keys (lanes 0 to 15) or values of each tile under way.
-  const int my_chunk = lane % kChunks, my_row = lane / kChunks;
+  // --- loading.  By TMA a tile is one run of rows of a page: the next page is
+  // looked up as soon as the one at hand is entered.  Else lane l looks up the
+  // page of token l % 16 of the tile to come.  Lane l holds the scale of that
+  // token's keys (lanes 0 to 15) or values of each tile under way.
   const float* my_scales = lane < kTile ? cache.k_scale : cache.v_scale;
   float scale[kStages - 1];  // oldest first
-  int page_id = 0, page_row = 0;
-  auto look_up = [&] {
-    const int token = ahead.tile * kTile + (one_page ? 0 : lane % kTile);
-    const int index = p.page_div.quot(token);
-    page_row = token - index * cache.page;
-    page_id = token < ahead.seg.seq.length ? p.a.batch.table[ahead.b * p.a.batch.table_stride + index] : 0;
+  int page_id = 0, page_row = 0, next_id = 0, page_index = 0;
+  auto table_at = [&](int index) {
+    return index * cache.page < ahead.seg.seq.length ? p.a.batch.table[ahead.b * p.a.batch.table_stride + index] : 0;
+  };
+  auto look_up = [&](bool same_segment) {
+    if constexpr (TMA) {
+      if (same_segment) {
+        page_row += kTile;
+        if (page_row < cache.page) return;
+        page_row = 0;
+        ++page_index;
+        page_id = next_id;
+      } else {
+        page_index = p.page_div.quot(ahead.tile * kTile);
+        page_row = ahead.tile * kTile - page_index * cache.page;
+        page_id = table_at(page_index);
+      }
+      next_id = table_at(page_index + 1);
+    } else {
+      const int token = ahead.tile * kTile + lane % kTile;
+      const int index = p.page_div.quot(token);
+      page_row = token - index * cache.page;
+      page_id = token < ahead.seg.seq.length ? table_at(index) : 0;
+    }
   };
   auto issue = [&](int stage) {
     float s = 0.0f;
     if (to_issue > 0) {
-      const uint32_t base = ring_addr + stage * 2 * S::kMatrix;
       const int there = ahead.seg.seq.length - ahead.tile * kTile;  // tokens of the tile: 16 of them, or fewer
-      const bool bad = page_id < 0 || page_id >= cache.pages;
+      const bool bad = static_cast<uint32_t>(page_id) >= static_cast<uint32_t>(cache.pages);
       const int line = (bad ? 0 : page_id) * cache.heads + ahead.head;
+      const int row = page_row + (TMA ? lane % kTile : 0);
+      const uint64_t scale_at = static_cast<uint64_t>(static_cast<uint32_t>(line)) * static_cast<uint32_t>(p.blocks) +
+                                p.block_div.quot(row);
       if (lane % kTile < there) {
-        if (bad) {
-          // a page outside the cache: recorded, and NaN for whoever attends to it
-          atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
-          s = __int_as_float(0x7fc00000);
-        } else {
-          const int row = page_row + (one_page ? lane % kTile : 0);
-          s = my_scales[static_cast<uint64_t>(static_cast<uint32_t>(line)) * static_cast<uint32_t>(p.blocks) + p.block_div.quot(row)];
-        }
+        s = bad ? __int_as_float(0x7fc00000) : my_scales[scale_at];
+        // a page outside the cache: recorded, and NaN for whoever attends to it
+        if (bad) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
       }
       // Rows behind the sequence's end are whatever the page or the ring holds:
       // finite int8, and their weight is 0.  So are a bad page's, with NaN.
-      if (one_page) {
-        if (lane == 0) {
+      if constexpr (TMA) {
+        if (sm100::elect_sync()) {
           if (bad) {
             sm100::mbar_arrive(&landed[stage]);
           } else {
-            const int row = line * cache.page + page_row;
             sm100::mbar_arrive_expect_tx(&landed[stage], 2 * S::kMatrix);
             unsigned char* to = ring + stage * 2 * S::kMatrix;
 #pragma unroll
             for (int h = 0; h < DP / kBox; ++h) {
-              sm100::tma_load_2d(to + h * kTile * kBox, &key_map, &landed[stage], h * kBox, row);
-              sm100::tma_load_2d(to + S::kMatrix + h * kTile * kBox, &value_map, &landed[stage], h * kBox, row);
+              sm100::tma_load_2d(to + h * kTile * kBox, &key_map, &landed[stage], h * kBox, line * cache.page + page_row);
+              sm100::tma_load_2d(to + S::kMatrix + h * kTile * kBox, &value_map, &landed[stage], h * kBox,
+                                 line * cache.page + page_row);
             }
           }
         }
+        __syncwarp();
       } else {
+        constexpr int kChunks = DP / 16;  // 16-byte chunks of a token
+        constexpr int kRowsAtOnce = 32 / kChunks;
+        const int my_chunk = lane % kChunks, my_row = lane / kChunks;
+        const uint32_t base = ring_addr + stage * 2 * S::kMatrix;
         const int64_t row_at = static_cast<int64_t>(line) * cache.page + page_row;
         const unsigned rows_there = __ballot_sync(0xffffffffu, lane % kTile < there && !bad);
 #pragma unroll
         for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-          const int row = i * kRowsAtOnce + my_row;
-          const int64_t from = __shfl_sync(0xffffffffu, row_at, row) * dim + my_chunk * 16;
-          if (my_chunk * 16 < dim && (rows_there >> row & 1)) {
-            cp_async16(base + place<DP>(row, my_chunk), cache.k + from);
-            cp_async16(base + S::kMatrix + place<DP>(row, my_chunk), cache.v + from);
+          const int r = i * kRowsAtOnce + my_row;
+          const int64_t from = __shfl_sync(0xffffffffu, row_at, r) * dim + my_chunk * 16;
+          if (my_chunk * 16 < dim && (rows_there >> r & 1)) {
+            cp_async16(base + place<DP>(r, my_chunk), cache.k + from);
+            cp_async16(base + S::kMatrix + place<DP>(r, my_chunk), cache.v + from);
           }
         }
         cp_async_arrive(&landed[stage]);
       }
-      if (--to_issue > 0) {
-        ahead.advance(p);
-        look_up();
-      }
+      if (--to_issue > 0) look_up(ahead.advance(p));
     }
     return s;
   };
-  look_up();
+  look_up(false);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) scale[i] = issue(i);
 
@@ -866,16 +882,21 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   // boxes of a tile's rows, as bytes
   CUtensorMap maps[2] = {};
   const uint64_t lines = static_cast<uint64_t>(p.a.cache.pages) * p.a.cache.heads * p.a.cache.page;
-  p.by_tma = p.a.cache.page % kTile == 0 && lines <= 0x7fffffff;  // a box's row is a 32-bit coordinate
-  if (p.by_tma) {
+  // TMA where pages hold whole tiles (a box's row is a 32-bit coordinate) and
+  // the sequences may be long enough: encoding the maps costs 5 us on the host,
+  // and TMA wins 4 us of 134 at 670 MB
+  const int64_t tokens = static_cast<int64_t>(p.a.batch.seqs) * p.a.batch.table_width * p.a.cache.page;
+  const bool tma = p.a.cache.page % kTile == 0 && lines <= 0x7fffffff && tokens * p.a.cache.heads * dim >= (64 << 20);
+  if (tma) {
     if (!cache_map(&maps[0], p.a.cache.k, dim, lines, DP) || !cache_map(&maps[1], p.a.cache.v, dim, lines, DP))
       return cudaErrorInvalidValue;
   }
-  static std::atomic<bool> allowed[kMaxDevices];
-  cudaError_t e = allow_smem(attend_units<DP, F32, NR>, S::kBytes, allowed);
+  static std::atomic<bool> allowed[2][kMaxDevices];
+  auto kernel = tma ? attend_units<DP, F32, NR, true> : attend_units<DP, F32, NR, false>;
+  cudaError_t e = allow_smem(kernel, S::kBytes, allowed[tma]);
   if (e != cudaSuccess) return e;
   PdlLaunch launch(dim3(static_cast<unsigned>(sms * S::kCtas)), dim3(S::kWarps * 32), S::kBytes, stream);
-  e = launch(attend_units<DP, F32, NR>, p, maps[0], maps[1]);
+  e = launch(kernel, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
   const int64_t rows = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
   // a row's partials are spread over eight warps where the rows alone would not fill the GPU

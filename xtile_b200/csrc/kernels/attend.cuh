@@ -18,7 +18,6 @@ struct AttendDev {
   AttendArgs a;
   FastDiv page_div, block_div, group_div;
   int group, blocks;  // query heads a kv head, blocks a page
-  bool by_tma;        // tiles come by TMA
   float* part;        // [workers][2][rows][dim] partial outputs
   float2* part_ml;    // [workers][2][rows] (reference, sum)
   int64_t workers;
