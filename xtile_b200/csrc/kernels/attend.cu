@@ -57,9 +57,8 @@ struct Shape {
   static constexpr int kRows = 8 * NR;  // query rows of a segment
   static constexpr int kWarps = DP <= 128 ? 4 : 2;
   static constexpr bool kHeavy = F32 || NR == 4 || DP > 128;
-  static constexpr int kCtas = DP > 128               ? (F32 && NR > 1 ? 2 : 3)  // CTAs an SM, by the registers of a row and dim
-                               : DP * NR * (F32 ? 2 : 1) <= 128 ? (F32 || NR > 1 ? 3 : 4)
-                                                                : 2;
+  // CTAs an SM, by the registers of a row and dim
+  static constexpr int kCtas = DP > 128 ? (F32 && NR > 1 ? 2 : 3) : F32 || DP * NR > 128 ? 2 : NR == 2 ? 3 : 4;
   static constexpr int kMatrix = kTile * DP;             // a stage holds keys and values
   static constexpr bool kQueryInSmem = kHeavy;           // else its fragments stay in registers
   static constexpr int kQueryBytes = kQueryInSmem ? (DP / 16) * NR * 256 * (F32 ? 2 : 1) : 0;
