@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <cstring>
+
 #include "../serve.h"
 #include "pdl.cuh"
 #include "vec.cuh"
@@ -30,6 +32,7 @@ struct NormDev {
   int cols;
   float eps, inv_cols;
   uint8_t weight_elem, y_elem;
+  int shift, shift_step;  // SHIFT: elements that row 0 starts behind a vector's boundary, and each row more
 };
 
 // Sum (or largest, NaN kept) of ``v`` over the threads of a row: a warp, or
@@ -74,12 +77,34 @@ __device__ __forceinline__ void store_row(const NormDev& p, int64_t row, int at,
     Vec<float, V>::store(static_cast<float*>(p.y) + to, y);
 }
 
-// V elements as they lie in memory.
+// Those of V values that fall in a row's [0, cols).
+template <class U, int V>
+__device__ __forceinline__ void store_some(U* row, int at, int cols, const float (&x)[V], float inverse) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (at + j < 0 || at + j >= cols) continue;
+    if constexpr (sizeof(U) == 1) {
+      row[at + j] = static_cast<int8_t>(quantize(x[j], inverse));
+    } else {
+      const float one[1] = {x[j]};
+      Vec<U, 1>::store(row + at + j, one);
+    }
+  }
+}
+
+// V elements as they lie in memory.  load_some takes those of [at, at + V) that
+// lie in [0, cols), and zeros for the others.
 template <class T, int V>
 struct Raw {
   uint4 v;
   __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load_some(const T* row, int at, int cols) {
+    T x[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = at + j >= 0 && at + j < cols ? row[at + j] : static_cast<T>(0.0f);
+    memcpy(&v, x, sizeof v);
+  }
   __device__ __forceinline__ void values(float (&x)[V]) const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -98,14 +123,18 @@ struct Raw<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = *p; }
   __device__ __forceinline__ void zero() { v = static_cast<T>(0.0f); }
+  __device__ __forceinline__ void load_some(const T*, int, int) {}  // never partial
   __device__ __forceinline__ void values(float (&x)[1]) const { x[0] = static_cast<float>(v); }
 };
 
 // A row in a CTA's registers, or (CTA false) in a warp's: N vectors of V
-// elements a thread.  A CTA goes on to the row gridDim behind, whose loads are
+// elements a thread.  SHIFT: rows that start off a vector's boundary, all
+// arrays' alike (an odd number of columns); their vectors start on the
+// boundary before the row, and the first and last are partial.  Element by
+// element, 8192 x 4095 bf16 took 117 us.  A CTA goes on to the row gridDim behind, whose loads are
 // under way while this one is reduced, rounded and stored: with a CTA a row
 // 8192 x 4096 bf16 took 44.1 us.
-template <class T, int V, int N, bool CTA, int MAX_THREADS, int CTAS>
+template <class T, int V, int N, bool CTA, int MAX_THREADS, int CTAS, bool SHIFT = false>
 __global__ void __launch_bounds__(MAX_THREADS, CTAS) rms_norm_rows(const NormDev p) {
   __shared__ float part[2][2][32];
   const int threads = CTA ? blockDim.x : 32;
@@ -115,21 +144,33 @@ __global__ void __launch_bounds__(MAX_THREADS, CTAS) rms_norm_rows(const NormDev
   const int64_t step = static_cast<int64_t>(gridDim.x) * rows_at_once;
   griddep_launch_dependents();
   griddep_wait();
+  auto shift_of = [&](int64_t at_row) {
+    return SHIFT ? static_cast<int>((p.shift + at_row * p.shift_step) % V) : 0;
+  };
+  auto whole = [&](int at) { return !SHIFT ? at < p.cols : at >= 0 && at + V <= p.cols; };
+  auto some = [&](int at) { return SHIFT && at + V > 0 && at < p.cols; };
   Raw<T, V> x[N], res[N];
   auto fetch = [&](int64_t at_row) {
     const T* from = static_cast<const T*>(p.x) + at_row * p.x_stride;
     const T* also = static_cast<const T*>(p.residual) + at_row * p.residual_stride;
+    const int shift = shift_of(at_row);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = (i * threads + me) * V;
+      const int at = (i * threads + me) * V - shift;
       x[i].zero();
       res[i].zero();
-      if (at < p.cols) x[i].load(from + at);
-      if (at < p.cols && p.residual) res[i].load(also + at);
+      if (whole(at)) {
+        x[i].load(from + at);
+        if (p.residual) res[i].load(also + at);
+      } else if (some(at)) {
+        x[i].load_some(from, at, p.cols);
+        if (p.residual) res[i].load_some(also, at, p.cols);
+      }
     }
   };
   if (row < p.rows) fetch(row);
   for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    const int shift = shift_of(row);
     float h[N][V];
     float ss = 0.0f;
 #pragma unroll
@@ -148,8 +189,11 @@ __global__ void __launch_bounds__(MAX_THREADS, CTAS) rms_norm_rows(const NormDev
       T* sum = static_cast<T*>(p.sum) + row * p.sum_stride;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int at = (i * threads + me) * V;
-        if (at < p.cols) Vec<T, V>::store(sum + at, h[i]);
+        const int at = (i * threads + me) * V - shift;
+        if (whole(at))
+          Vec<T, V>::store(sum + at, h[i]);
+        else if (some(at))
+          store_some(sum, at, p.cols, h[i], 0.0f);
       }
     }
     ss = row_reduce<false, CTA>(ss, part[turn][0]);
@@ -157,10 +201,19 @@ __global__ void __launch_bounds__(MAX_THREADS, CTAS) rms_norm_rows(const NormDev
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = (i * threads + me) * V;
-      if (at >= p.cols) continue;
+      const int at = (i * threads + me) * V - shift;
+      if (!whole(at) && !some(at)) continue;
       float w[V];
-      load_weight<T, V>(p, at, w);
+      if constexpr (SHIFT) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float one[1] = {0.0f};
+          if (at + j >= 0 && at + j < p.cols) load_weight<T, 1>(p, at + j, one);
+          w[j] = one[0];
+        }
+      } else {
+        load_weight<T, V>(p, at, w);
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         h[i][j] = h[i][j] * r * w[j];
@@ -176,8 +229,17 @@ __global__ void __launch_bounds__(MAX_THREADS, CTAS) rms_norm_rows(const NormDev
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = (i * threads + me) * V;
-      if (at < p.cols) store_row<V>(p, row, at, h[i], inverse);
+      const int at = (i * threads + me) * V - shift;
+      if (whole(at)) {
+        store_row<V>(p, row, at, h[i], inverse);
+      } else if (some(at)) {
+        if (p.y_elem == kI8)
+          store_some(static_cast<int8_t*>(p.y) + row * p.y_stride, at, p.cols, h[i], inverse);
+        else if (p.y_elem == kBF16)
+          store_some(static_cast<__nv_bfloat16*>(p.y) + row * p.y_stride, at, p.cols, h[i], inverse);
+        else
+          store_some(static_cast<float*>(p.y) + row * p.y_stride, at, p.cols, h[i], inverse);
+      }
     }
   }
 }
@@ -229,10 +291,11 @@ __global__ void __launch_bounds__(1024) rms_norm_wide(const NormDev p) {
   }
 }
 
-template <class T, int V>
+template <class T, int V, bool SHIFT = false>
 cudaError_t launch_typed(const NormDev& p, cudaStream_t stream) {
   constexpr int kSms = 148;
-  const int vectors = (p.cols + V - 1) / V;  // V divides cols unless it is 1
+  // V divides cols unless it is 1; a shifted row may take two vectors more than its elements
+  const int vectors = SHIFT ? (p.cols + 2 * V - 2) / V : (p.cols + V - 1) / V;
   // as many CTAs as the SMs hold by the kernel's registers, and no more than there are rows for
   auto go = [&](auto kernel, int regs, int threads, int64_t groups) {
     const int ctas = 65536 / (regs * threads) < 2048 / threads ? 65536 / (regs * threads) : 2048 / threads;
@@ -243,11 +306,11 @@ cudaError_t launch_typed(const NormDev& p, cudaStream_t stream) {
   auto threads_for = [&](int n) { return ((vectors + n - 1) / n + 31) / 32 * 32; };
   // narrow rows: a warp each, no barrier
   const int64_t eights = (p.rows + 7) / 8;
-  if (vectors <= 32) return go(rms_norm_rows<T, V, 1, false, 256, 5>, 48, 256, eights);
-  if (vectors <= 128) return go(rms_norm_rows<T, V, 4, false, 256, 2>, 128, 256, eights);
-  if (vectors <= 512) return go(rms_norm_rows<T, V, 2, true, 256, 4>, 64, threads_for(2), p.rows);
-  if (vectors <= 1024) return go(rms_norm_rows<T, V, 2, true, 512, 2>, 64, threads_for(2), p.rows);
-  if (vectors <= 4096) return go(rms_norm_rows<T, V, 4, true, 1024, 1>, 64, threads_for(4), p.rows);
+  if (vectors <= 32) return go(rms_norm_rows<T, V, 1, false, 256, 5, SHIFT>, 48, 256, eights);
+  if (vectors <= 128) return go(rms_norm_rows<T, V, 4, false, 256, 2, SHIFT>, 128, 256, eights);
+  if (vectors <= 512) return go(rms_norm_rows<T, V, 2, true, 256, 4, SHIFT>, 64, threads_for(2), p.rows);
+  if (vectors <= 1024) return go(rms_norm_rows<T, V, 2, true, 512, 2, SHIFT>, 64, threads_for(2), p.rows);
+  if (vectors <= 4096) return go(rms_norm_rows<T, V, 4, true, 1024, 1, SHIFT>, 64, threads_for(4), p.rows);
   PdlLaunch launch(dim3(static_cast<unsigned>(p.rows)), dim3(1024), 0, stream);
   return launch(rms_norm_wide<T>, p);
 }
@@ -260,7 +323,7 @@ cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
   NormDev p{a.x,        a.residual, a.weight,     a.y,  a.sum, a.scales, a.x_stride, a.residual_stride,
             a.y_stride, a.sum_stride, a.rows, static_cast<int>(a.cols), a.eps, 1.0f / static_cast<float>(a.cols),
-            a.weight_elem, a.y_elem};
+            a.weight_elem, a.y_elem, 0, 0};
   // 16-byte vectors of x's type where every row of every array starts on its vector's boundary
   const int v = a.elem == kF32 ? 4 : 8;
   auto fits = [&](const void* ptr, int64_t stride, int bytes) {
@@ -271,8 +334,22 @@ cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t stream) {
   const bool vec = multiple(a.cols, v) && fits(a.x, a.x_stride, v * size) && fits(a.residual, a.residual_stride, v * size) &&
                    fits(a.sum, a.sum_stride, v * size) && fits(a.y, a.y_stride, v * y_size) &&
                    reinterpret_cast<uintptr_t>(a.weight) % 16 == 0;
-  if (a.elem == kF32) return vec ? launch_typed<float, 4>(p, stream) : launch_typed<float, 1>(p, stream);
-  return vec ? launch_typed<__nv_bfloat16, 8>(p, stream) : launch_typed<__nv_bfloat16, 1>(p, stream);
+  // or where every row of every array starts equally far behind one
+  auto shift_of = [&](const void* ptr, int bytes) { return static_cast<int>(reinterpret_cast<uintptr_t>(ptr) / bytes % v); };
+  p.shift = shift_of(a.x, size);
+  p.shift_step = static_cast<int>(a.x_stride % v);
+  auto alike = [&](const void* ptr, int64_t stride, int bytes) {
+    return !ptr || (shift_of(ptr, bytes) == p.shift && stride % v == p.shift_step);
+  };
+  const bool shifted = a.x_stride >= 0 && alike(a.residual, a.residual_stride, size) && alike(a.sum, a.sum_stride, size) &&
+                       alike(a.y, a.y_stride, y_size);
+  if (a.elem == kF32)
+    return vec       ? launch_typed<float, 4>(p, stream)
+           : shifted ? launch_typed<float, 4, true>(p, stream)
+                     : launch_typed<float, 1>(p, stream);
+  return vec       ? launch_typed<__nv_bfloat16, 8>(p, stream)
+         : shifted ? launch_typed<__nv_bfloat16, 8, true>(p, stream)
+                   : launch_typed<__nv_bfloat16, 1>(p, stream);
 }
 
 }  // namespace dev
