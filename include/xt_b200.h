@@ -301,7 +301,7 @@ int xt_cache_attention_workspace(const xt_cache_attention_args* args, size_t* ou
 int xt_cache_attention(const xt_cache_attention_args* args, void* stream);
 
 /* out[i] = q[i] * scales[i / run]: int8 data (rows, or a cache's blocks) back
- * as f32 or bf16 values.  q and out are 16-byte aligned. */
+ * as f32 or bf16 values; n is a multiple of run.  q and out are 16-byte aligned. */
 int xt_dequantize(const int8_t* q, const float* scales, void* out, int64_t n, int64_t run, int elem, void* stream);
 
 #ifdef __cplusplus

@@ -79,10 +79,46 @@ cudaError_t launch_rope_typed(const RopeArgs& a, cudaStream_t stream) {
   return threads >= 4 * 148 * 1024 ? go(rope_heads<T, U, V, 4>, 4) : go(rope_heads<T, U, V, 1>, 1);
 }
 
-// 16 int8 values a thread, whose scales are one or (RUNS) several.
-template <class U, bool ONE>
-__global__ void __launch_bounds__(kThreads) dequantize_flat(const int8_t* __restrict__ q, const float* __restrict__ scales,
-                                                            U* __restrict__ out, int64_t n, int64_t run) {
+// 16 int8 values as f32 or bf16, one scale.
+template <class U>
+__device__ __forceinline__ void dequantize_16(const int4& w, float s, U* out) {
+  const int words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      y[e] = static_cast<float>(static_cast<int8_t>(words[2 * j + e / 4] >> (8 * (e % 4)))) * s;
+    Vec<U, 8>::store(out + 8 * j, y);
+  }
+}
+
+// Runs of whole 16-byte vectors: two a thread, both loads under way at once.
+template <class U>
+__global__ void __launch_bounds__(kThreads) dequantize_runs(const int8_t* __restrict__ q, const float* __restrict__ scales,
+                                                            U* __restrict__ out, int64_t vectors, int64_t run) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int4* q4 = reinterpret_cast<const int4*>(q);
+  const int64_t run_vectors = run / 16;
+  auto scale_of = [&](int64_t i) {
+    return scales[(i | run_vectors) >> 32 ? i / run_vectors : static_cast<uint32_t>(i) / static_cast<uint32_t>(run_vectors)];
+  };
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * (2 * kThreads);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (2 * kThreads) + threadIdx.x; i < vectors; i += stride) {
+    const int64_t k = i + kThreads;
+    const bool two = k < vectors;
+    const int4 a = q4[i], b = two ? q4[k] : make_int4(0, 0, 0, 0);
+    const float sa = scale_of(i), sb = two ? scale_of(k) : 0.0f;
+    dequantize_16(a, sa, out + 16 * i);
+    if (two) dequantize_16(b, sb, out + 16 * k);
+  }
+}
+
+// Any runs: 16 values a thread, whose scales may change anywhere.
+template <class U>
+__global__ void __launch_bounds__(kThreads) dequantize_any(const int8_t* __restrict__ q, const float* __restrict__ scales,
+                                                           U* __restrict__ out, int64_t n, int64_t run) {
   griddep_launch_dependents();
   griddep_wait();
   const int64_t vectors = (n + 15) / 16;
@@ -90,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_flat(const int8_t* __rest
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
     const int64_t at = i * 16;
     int64_t r = (at | run) >> 32 ? at / run : static_cast<uint32_t>(at) / static_cast<uint32_t>(run);
-    if (ONE || at + 16 <= n) {
+    if (at + 16 <= n) {
       const int4 w = *reinterpret_cast<const int4*>(q + at);
       const int words[4] = {w.x, w.y, w.z, w.w};
       float s = scales[r];
@@ -100,11 +136,11 @@ __global__ void __launch_bounds__(kThreads) dequantize_flat(const int8_t* __rest
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (!ONE && left == 0) {
+          if (left == 0) {
             s = scales[++r];
             left = run;
           }
-          if (!ONE) --left;
+          --left;
           y[e] = static_cast<float>(static_cast<int8_t>(words[2 * j + e / 4] >> (8 * (e % 4)))) * s;
         }
         Vec<U, 8>::store(out + at + 8 * j, y);
@@ -116,6 +152,19 @@ __global__ void __launch_bounds__(kThreads) dequantize_flat(const int8_t* __rest
       }
     }
   }
+}
+
+template <class U>
+cudaError_t launch_dequantize_typed(const DequantArgs& a, cudaStream_t stream) {
+  U* out = static_cast<U*>(a.out);
+  const int64_t vectors = (a.n + 15) / 16;
+  auto grid = [](int64_t blocks) { return dim3(static_cast<unsigned>(blocks < (1 << 30) ? blocks : (1 << 30))); };
+  if (a.run % 16 == 0) {
+    PdlLaunch launch(grid((vectors + 2 * kThreads - 1) / (2 * kThreads)), dim3(kThreads), 0, stream);
+    return launch(dequantize_runs<U>, a.q, a.scales, out, vectors, a.run);
+  }
+  PdlLaunch launch(grid((vectors + kThreads - 1) / kThreads), dim3(kThreads), 0, stream);
+  return launch(dequantize_any<U>, a.q, a.scales, out, a.n, a.run);
 }
 
 }  // namespace
@@ -142,17 +191,7 @@ cudaError_t launch_rope(const RopeArgs& a, cudaStream_t stream) {
 
 cudaError_t launch_dequantize(const DequantArgs& a, cudaStream_t stream) {
   if (a.n <= 0) return cudaSuccess;
-  const int64_t blocks = ((a.n + 15) / 16 + kThreads - 1) / kThreads;
-  PdlLaunch launch(dim3(static_cast<unsigned>(blocks < (1 << 30) ? blocks : (1 << 30))), dim3(kThreads), 0, stream);
-  const bool one = a.run % 16 == 0 && a.n % 16 == 0;
-  if (a.elem == kF32) {
-    float* out = static_cast<float*>(a.out);
-    return one ? launch(dequantize_flat<float, true>, a.q, a.scales, out, a.n, a.run)
-               : launch(dequantize_flat<float, false>, a.q, a.scales, out, a.n, a.run);
-  }
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
-  return one ? launch(dequantize_flat<__nv_bfloat16, true>, a.q, a.scales, out, a.n, a.run)
-             : launch(dequantize_flat<__nv_bfloat16, false>, a.q, a.scales, out, a.n, a.run);
+  return a.elem == kF32 ? launch_dequantize_typed<float>(a, stream) : launch_dequantize_typed<__nv_bfloat16>(a, stream);
 }
 
 }  // namespace dev

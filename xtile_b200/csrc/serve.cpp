@@ -170,6 +170,7 @@ int xt_dequantize(const int8_t* q, const float* scales, void* out, int64_t n, in
   const char* who = "xt_dequantize";
   if (n < 0 || run < 1) return bad(who, "n must not be negative and run must be positive");
   if (!is_float(elem)) return bad(who, "out must be f32 or bf16");
+  if (n % run != 0) return bad(who, "n must be whole runs");
   if (n == 0) return XT_OK;
   if (!q || !scales || !out) return bad(who, "null array");
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(scales, 4)) return bad(who, "q and out must be 16-byte aligned");
