@@ -579,6 +579,101 @@ def test_attention_many_sequences():
     check_attention(cache, batch, normal(g, 1500, 2, 64, dtype=torch.bfloat16))
 
 
+def widened(batch, cache, form):
+    """The batch with a page table so wide that, as far as the host can tell, its sequences may be very long: their
+    tokens are shared out over the whole GPU then, and come as single rows ("rows") or as boxes of rows ("boxes")."""
+    starts, lengths, table = batch.args
+    tokens = (40 if form == "boxes" else 1) * 16400 * 16 // (cache.heads * max(len(batch.total), 1)) + 1
+    if form == "rows":  # but not so long that boxes pay
+        assert tokens * len(batch.total) * cache.heads * cache.dim < 64 << 20 or cache.page % 16
+    extra = torch.full((table.shape[0], -(-tokens // cache.page)), -9, dtype=torch.int32, device="cuda")
+    batch.args = (starts, lengths, torch.cat([table, extra], 1))
+    return batch
+
+
+@pytest.mark.parametrize("form", ["rows", "boxes"])
+@pytest.mark.parametrize("new, total", LENGTHS)
+@pytest.mark.parametrize("dim, heads, group", [(128, 2, 4), (64, 3, 1), (256, 1, 8), (80, 2, 5), (16, 1, 16), (96, 2, 7),
+                                               (128, 1, 32), (192, 2, 2)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_shapes_shared_out(form, new, total, dim, heads, group, dtype):
+    g = generator(dim + group)
+    page, block = {128: (64, 16), 64: (48, 8), 256: (16, 16), 80: (40, 20), 16: (32, 1)}.get(dim, (64, 64))
+    if form == "rows" and dim > 128:
+        page, block = 24, 8
+    batch = Batch(new, total, page, seed=dim)
+    cache = filled_cache(g, batch.pages_held, heads, dim, page, block)
+    widened(batch, cache, form)
+    q = normal(g, batch.tokens, heads * group, dim, std=1.5, dtype=dtype)
+    y = check_attention(cache, batch, q)
+    assert torch.equal(y, xt.cache_attention(cache, q, *batch.args))  # no order of arrival in it
+
+
+@pytest.mark.parametrize("form", ["rows", "boxes"])
+@pytest.mark.parametrize("window, softcap", [(0, 4.0), (1, 0.0), (100, 0.0), (5000, 20.0)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_long_shared_out(form, window, softcap, dtype):
+    g = generator(window)
+    batch = Batch([1, 2, 30, 1], [9000, 777, 500, 20000], 64, seed=3)
+    cache = filled_cache(g, batch.pages_held, 2, 128, 64, 16)
+    widened(batch, cache, form)
+    check_attention(cache, batch, normal(g, batch.tokens, 8, 128, std=2.0, dtype=dtype), window=window, softcap=softcap)
+
+
+@pytest.mark.parametrize("form", ["rows", "boxes"])
+def test_attention_edges_shared_out(form):
+    """Garbage that nothing sees, NaN that is seen, and wrong tables."""
+    g = generator(6)
+    batch = Batch([1, 2, 3], [70, 33, 2000], 16, seed=3)
+    cache = filled_cache(g, batch.pages_held, 2, 64, 16, 1)
+    widened(batch, cache, form)
+    q = normal(g, batch.tokens, 4, 64, dtype=torch.bfloat16)
+    good = check_attention(cache, batch, q, window=20)
+    used = torch.zeros_like(cache.k_scale, dtype=torch.bool)
+    for b, (n, t) in enumerate(zip(batch.new, batch.total)):
+        for j in range(max(0, t - n - 20 + 1), t):
+            used[batch.table[b][j // 16], :, j % 16] = True
+    for bad in (float("nan"), float("inf"), 3e38):
+        for s in (cache.k_scale, cache.v_scale):
+            s[~used] = bad
+        for c in (cache.k, cache.v):
+            c[~used] = -128
+        assert torch.equal(xt.cache_attention(cache, q, *batch.args, window=20), good)
+    cache.v_scale[batch.table[0][69 // 16], 0, 69 % 16] = float("nan")
+    y = xt.cache_attention(cache, q, *batch.args, window=20)
+    assert y[0, :2].isnan().all() and torch.equal(y[0, 2:], good[0, 2:]) and torch.equal(y[1:], good[1:])
+
+    cache = filled_cache(g, batch.pages_held, 2, 64, 16, 1)
+    starts, lengths, table = batch.args
+    good = xt.cache_attention(cache, q, starts, lengths, table)
+    for fault in ("page", "length", "starts"):
+        s, n, t = starts.clone(), lengths.clone(), table.clone()
+        if fault == "page":
+            t[1, 1] = batch.pages_held
+        elif fault == "length":
+            n[1] = -3
+        else:
+            s[3] = 9
+        y = xt.cache_attention(cache, q, s, n, t)
+        assert xt.device_error() == 0x303
+        wrong = slice(3, 6) if fault == "starts" else slice(1, 3)
+        assert y[wrong].isnan().all(), fault
+        assert torch.equal(y[0], good[0])
+
+
+@pytest.mark.parametrize("seqs, heads, new", [(1, 1, 1), (3, 2, 1), (40, 4, 1), (300, 2, 1), (5, 8, 3), (1, 16, 40)])
+@pytest.mark.parametrize("dim, group", [(128, 8), (64, 2), (256, 3)])
+def test_attention_clusters(seqs, heads, new, dim, group):
+    """Few and many small segments: clusters of every size, rows over several tiles."""
+    g = generator(seqs + new)
+    total = [max(new, 1 + (97 * i) % 200) for i in range(seqs)]
+    batch = Batch([new] * seqs, total, 16, seed=3)
+    cache = filled_cache(g, batch.pages_held, heads, dim, 16, 4)
+    for dtype in TYPES:
+        q = normal(g, batch.tokens, heads * group, dim, dtype=dtype)
+        check_attention(cache, batch, q, max_new=new)
+
+
 @pytest.mark.parametrize("new, total", [([300], [300]), ([257, 64, 500], [1000, 64, 777]), ([128, 1, 129], [2048, 900, 129])])
 @pytest.mark.parametrize("dim, group", [(128, 4), (64, 8), (128, 1), (96, 5), (256, 2), (80, 7)])
 @pytest.mark.parametrize("window, softcap", [(0, 0.0), (100, 0.0), (0, 20.0)])

@@ -115,7 +115,7 @@ def test_cache_attention_refuses(kw, word):
 
 
 def test_cache_attention_needs_its_workspace():
-    args = Attend(**parts({}), q=AT, out=AT, q_heads=2, scale=0.125, elem=BF16)
+    args = Attend(**parts(dict(table_width=1 << 16, table_stride=1 << 16)), q=AT, out=AT, q_heads=2, scale=0.125, elem=BF16)
     need = ctypes.c_size_t()
     assert LIB.xt_cache_attention_workspace(ctypes.byref(args), ctypes.byref(need)) == 0
     args.workspace, args.workspace_bytes = AT, max(need.value, 1) - 1

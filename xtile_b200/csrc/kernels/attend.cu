@@ -17,7 +17,9 @@
 // whole tiles, cp.async rows where they do not), runs the two products on
 // mma.sync m16n8k16 in f16 and keeps the running reference, sum and output of
 // its rows in registers.  Segments that several warps share are joined by a
-// second kernel from f32 partial results.
+// second kernel from f32 partial results.  That kernel costs 4.5 us, so small
+// calls give each segment to a cluster instead, whose warps split its tokens
+// and join in shared memory.
 //
 // Tokens (and the output's dims) are the products' m, query rows their n: the
 // converted cache bytes are A operands that all of a segment's rows share, and
@@ -35,6 +37,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "../serve.h"
 #include "attend.cuh"
@@ -70,7 +74,12 @@ struct Shape {
   static constexpr int kWarpBytes = kStages * 2 * kMatrix + kQueryBytes;
   static_assert(kWarpBytes % 1024 == 0, "a ring starts on a swizzle atom");
   static constexpr int kBytes = kWarps * kWarpBytes + 256 + 1024;
+  static_assert(kRows * DP * 4 + kRows * 16 <= kWarpBytes, "a warp's partial result fits its ring");
 };
+
+// How tiles come: rows by cp.async or boxes by TMA, units shared out over the
+// grid; or rows by cp.async, a cluster a segment.
+enum class Form { kRows, kBoxes, kCluster };
 
 // The units of sequence b: kv heads x row tiles x token tiles [lo, hi).
 struct Segments {
@@ -180,6 +189,24 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(sm100::smem_addr(bar)) : "memory");
 }
 
+// What lies at this address in the shared memory of CTA ``rank`` of the cluster.
+__device__ __forceinline__ float2 cluster_load2(const float2* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(sm100::mapa_shared(sm100::smem_addr(p), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(sm100::mapa_shared(sm100::smem_addr(p), rank))
+               : "memory");
+  return v;
+}
+
 // c += a b for 16 x 16 f16 a, 16 x 8 f16 b, f32 c.
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
   asm volatile(
@@ -224,12 +251,13 @@ __device__ __forceinline__ void lds128(uint32_t (&w)[4], uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
 }
 
-template <int DP, bool F32, int NR, bool TMA>
+template <int DP, bool F32, int NR, Form FORM>
 __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32, NR>::kCtas)
     attend_units(const __grid_constant__ AttendDev p, const __grid_constant__ CUtensorMap key_map,
                  const __grid_constant__ CUtensorMap value_map) {
   using S = Shape<DP, F32, NR>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+  constexpr bool TMA = FORM == Form::kBoxes, kCluster = FORM == Form::kCluster;
   constexpr int kRows = S::kRows, kStages = S::kStages;
   constexpr int kSteps = DP / 16;    // k16 steps of the score product
   constexpr int kOut = DP / 16;      // m16 tiles of the output
@@ -262,17 +290,37 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   // behind the wait: what the join reads before its own wait is final, then
   griddep_launch_dependents();
 
-  int64_t unused;
-  const int64_t total = count_units<kRows>(p, 0, &unused);
-  const int64_t per = divide(total + p.workers - 1, p.workers);
-  const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
-  const int64_t begin = worker * per;
-  if (begin >= total) return;
-  int left = static_cast<int>(total - begin < per ? total - begin : per);  // units to do, and to issue
-  int to_issue = left;
-
   Cursor<kRows> at;
-  at.seek(p, begin);
+  int64_t worker = 0;
+  int left;  // units to do
+  if constexpr (kCluster) {
+    const int rank = blockIdx.x % p.cluster, index = blockIdx.x / p.cluster, slot = index / cache.heads;
+    auto base = [&](int i) { return first_slot(p.a.batch.starts[i], i, p.group, kRows); };
+    at.b = last_at_most(p.a.batch.seqs, slot, base);
+    at.head = index - slot * cache.heads;
+    at.seg = load_segments<kRows>(p, at.b);
+    const int64_t row_tile = slot - base(at.b);
+    // the cluster's CTAs return together
+    if (!at.seg.seq.ok) {
+      if (row_tile == 0 && rank == 0) refuse_sequence<T>(p, at.b, at.head, threadIdx.x, S::kWarps * 32);
+      return;
+    }
+    if (row_tile < 0 || row_tile >= at.seg.row_tiles) return;
+    at.row_tile = static_cast<int>(row_tile);
+    const int64_t tiles = at.seg.hi - at.seg.lo, of = p.cluster * S::kWarps, mine = rank * S::kWarps + warp;
+    at.tile = at.seg.lo + static_cast<int>(divide(tiles * mine, of));
+    left = at.seg.lo + static_cast<int>(divide(tiles * (mine + 1), of)) - at.tile;
+  } else {
+    int64_t unused;
+    const int64_t total = count_units<kRows>(p, 0, &unused);
+    const int64_t per = divide(total + p.workers - 1, p.workers);
+    worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
+    const int64_t begin = worker * per;
+    if (begin >= total) return;
+    left = static_cast<int>(total - begin < per ? total - begin : per);
+    at.seek(p, begin);
+  }
+  int to_issue = left;
   Cursor<kRows> ahead = at;
 
   // --- loading.  By TMA a tile is one run of rows of a page: the next page is
@@ -360,7 +408,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
     }
     return s;
   };
-  look_up(false);
+  if (to_issue > 0) look_up(false);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) scale[i] = issue(i);
 
@@ -503,7 +551,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   const sm100::Abort ab{abort_flag, p.a.error_word, sm100::kWaitLimitCycles};
   int stage = 0;
   uint32_t phase = 0;
-  while (true) {
+  while (!kCluster || left > 0) {
     if (!__all_sync(0xffffffffu, sm100::mbar_wait(&landed[stage], phase, ab, kErrUnitWait))) break;
     __syncwarp();  // every lane has read the stage before this one
     const float scales = scale[0];
@@ -704,8 +752,12 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       phase ^= 1;
     }
 
-    const bool last_unit = at.tile + 1 == at.seg.hi;
     --left;
+    if constexpr (kCluster) {
+      ++at.tile;
+      continue;
+    }
+    const bool last_unit = at.tile + 1 == at.seg.hi;
     if (last_unit || left == 0) {
       finish_segment(last_unit);
       if (left == 0) return;
@@ -722,6 +774,83 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       stage = 0;
       phase ^= 1;
     }
+  }
+  if constexpr (kCluster) {
+    // --- the warps' results, over their rings: [rows][dim], then (reference, sum) of each row
+    __syncwarp();
+    const float up = __uint_as_float(static_cast<uint32_t>(value_exp + 117) << 23);
+    auto part_of = [&](int w) { return reinterpret_cast<float*>(smem + w * S::kWarpBytes); };
+    auto sums_of = [&](int w) { return reinterpret_cast<float2*>(part_of(w) + kRows * DP); };
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float s = sum[nr][c];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        const int row = 8 * nr + 2 * t + c;
+#pragma unroll
+        for (int x = 0; x < kOut * 2; x += 4) {
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = o[(x + e) / 2][nr][2 * ((x + e) % 2) + c] * up;
+          const int d = x / kSpan * 8 * kSpan + g * kSpan + x % kSpan;
+          *reinterpret_cast<float4*>(part_of(warp) + row * DP + d) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+        if (g == 0) sums_of(warp)[row] = make_float2(ref[nr][c], s);
+      }
+    __syncthreads();
+    // --- the CTA's, four dims a thread, over warp 0's (its sums behind them)
+    constexpr int kThreads = S::kWarps * 32, kItems = kRows * DP / 4;
+    float2* cta_sums = sums_of(0) + kRows;
+    for (int item = threadIdx.x; item < kItems; item += kThreads) {
+      const int row = item / (DP / 4), d = item % (DP / 4) * 4;
+      float2 ml[S::kWarps];
+      float top = kNone;
+#pragma unroll
+      for (int w = 0; w < S::kWarps; ++w) {
+        ml[w] = sums_of(w)[row];
+        top = fmaxf(top, ml[w].x);
+      }
+      float s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < S::kWarps; ++w) {
+        const float by = exp2_fast(ml[w].x - top);
+        const float4 v = *reinterpret_cast<const float4*>(part_of(w) + row * DP + d);
+        s += ml[w].y * by;
+        y[0] += v.x * by, y[1] += v.y * by, y[2] += v.z * by, y[3] += v.w * by;
+      }
+      *reinterpret_cast<float4*>(part_of(0) + row * DP + d) = make_float4(y[0], y[1], y[2], y[3]);
+      if (d == 0) cta_sums[row] = make_float2(top, s);
+    }
+    // --- the cluster's: each CTA has a share of the items
+    if (p.cluster > 1)
+      sm100::cluster_sync();
+    else
+      __syncthreads();
+    const int rank = blockIdx.x % p.cluster;
+    for (int item = rank * kThreads + threadIdx.x; item < kItems; item += p.cluster * kThreads) {
+      const int row = item / (DP / 4), d = item % (DP / 4) * 4;
+      int i;
+      const int head = row_of(row, &i);
+      if (head < 0 || d >= dim) continue;
+      float top = kNone;
+      for (int c = 0; c < p.cluster; ++c) top = fmaxf(top, cluster_load2(cta_sums + row, c).x);
+      float s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int c = 0; c < p.cluster; ++c) {
+        const float2 ml = cluster_load2(cta_sums + row, c);
+        const float4 v = cluster_load4(part_of(0) + row * DP + d, c);
+        const float by = exp2_fast(ml.x - top);
+        s += ml.y * by;
+        y[0] += v.x * by, y[1] += v.y * by, y[2] += v.z * by, y[3] += v.w * by;
+      }
+      const float over = s > 0.0f || s != s ? 1.0f / s : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] *= over;
+      Vec<T, 4>::store(static_cast<T*>(p.a.out) + static_cast<int64_t>(at.seg.seq.first + i) * p.a.out_token +
+                           static_cast<int64_t>(head) * p.a.out_head + d, y);
+    }
+    if (p.cluster > 1) sm100::cluster_sync();  // no CTA goes while another reads its memory
   }
 }
 
@@ -866,35 +995,61 @@ bool cache_map(CUtensorMap* map, const void* base, int dim, uint64_t lines, int 
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// New tokens of a sequence, as far as the caller knows; else their mean.
+int new_tokens(const AttendDev& p) {
+  const int mean = (p.a.batch.tokens + p.a.batch.seqs - 1) / p.a.batch.seqs;
+  return p.a.max_new > 0 ? (p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens) : mean;
+}
+
 template <int DP, bool F32, int NR>
 cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   using S = Shape<DP, F32, NR>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-  const int sms = sm_count(), dim = p.a.cache.dim;
-  p.workers = static_cast<int64_t>(sms) * S::kCtas * S::kWarps;
+  const int sms = sm_count(), dim = p.a.cache.dim, resident = sms * S::kCtas;
+  static std::atomic<bool> allowed[3][kMaxDevices];
+  // At most this many tokens of a sequence are seen, as far as the host knows.
+  int64_t longest = static_cast<int64_t>(p.a.batch.table_width) * p.a.cache.page;
+  if (p.a.window > 0) longest = std::min<int64_t>(longest, static_cast<int64_t>(p.a.window) + new_tokens(p));
+  const int64_t tiles = (longest + kTile - 1) / kTile;
+  const int64_t segments = static_cast<int64_t>(p.a.batch.seqs) * p.a.cache.heads *
+                           ((static_cast<int64_t>(new_tokens(p)) * p.group + S::kRows - 1) / S::kRows);
+  // A cluster a segment where the whole is small: 1.3 units a nanosecond make
+  // 16384 of them 12 us, of which an uneven share loses less than the join.
+  if (segments * tiles <= 16384) {
+    if (bytes) {
+      *bytes = 0;
+      return cudaSuccess;
+    }
+    p.cluster = 8;
+    while (p.cluster > 1 && (segments * p.cluster > resident || p.cluster * S::kWarps > tiles)) p.cluster /= 2;
+    auto kernel = attend_units<DP, F32, NR, Form::kCluster>;
+    const cudaError_t e = allow_smem(kernel, S::kBytes, allowed[2]);
+    if (e != cudaSuccess) return e;
+    const int64_t slots = first_slot(p.a.batch.tokens, p.a.batch.seqs, p.group, S::kRows);
+    PdlLaunch launch(dim3(static_cast<unsigned>(slots * p.a.cache.heads * p.cluster)), dim3(S::kWarps * 32), S::kBytes, stream,
+                     p.cluster);
+    return launch(kernel, p, CUtensorMap{}, CUtensorMap{});
+  }
+  p.workers = static_cast<int64_t>(resident) * S::kWarps;
   if (bytes) {
     *bytes = static_cast<size_t>(p.workers) * 2 * S::kRows * (dim + 2) * sizeof(float);
     return cudaSuccess;
   }
   p.part = static_cast<float*>(p.a.workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part + p.workers * 2 * S::kRows * dim);
-  // boxes of a tile's rows, as bytes
+  // Boxes of a tile's rows by TMA where pages hold whole tiles (a box's row is a
+  // 32-bit coordinate) and the sequences may be long enough: encoding the maps
+  // costs 5 us on the host, and TMA wins 12 us of 134 at 670 MB.
   CUtensorMap maps[2] = {};
   const uint64_t lines = static_cast<uint64_t>(p.a.cache.pages) * p.a.cache.heads * p.a.cache.page;
-  // TMA where pages hold whole tiles (a box's row is a 32-bit coordinate) and
-  // the sequences may be long enough: encoding the maps costs 5 us on the host,
-  // and TMA wins 4 us of 134 at 670 MB
-  const int64_t tokens = static_cast<int64_t>(p.a.batch.seqs) * p.a.batch.table_width * p.a.cache.page;
-  const bool tma = p.a.cache.page % kTile == 0 && lines <= 0x7fffffff && tokens * p.a.cache.heads * dim >= (64 << 20);
-  if (tma) {
-    if (!cache_map(&maps[0], p.a.cache.k, dim, lines, DP) || !cache_map(&maps[1], p.a.cache.v, dim, lines, DP))
-      return cudaErrorInvalidValue;
-  }
-  static std::atomic<bool> allowed[2][kMaxDevices];
-  auto kernel = tma ? attend_units<DP, F32, NR, true> : attend_units<DP, F32, NR, false>;
+  const bool tma = p.a.cache.page % kTile == 0 && lines <= 0x7fffffff &&
+                   longest * p.a.batch.seqs * p.a.cache.heads * dim >= (64 << 20);
+  if (tma && (!cache_map(&maps[0], p.a.cache.k, dim, lines, DP) || !cache_map(&maps[1], p.a.cache.v, dim, lines, DP)))
+    return cudaErrorInvalidValue;
+  auto kernel = tma ? attend_units<DP, F32, NR, Form::kBoxes> : attend_units<DP, F32, NR, Form::kRows>;
   cudaError_t e = allow_smem(kernel, S::kBytes, allowed[tma]);
   if (e != cudaSuccess) return e;
-  PdlLaunch launch(dim3(static_cast<unsigned>(sms * S::kCtas)), dim3(S::kWarps * 32), S::kBytes, stream);
+  PdlLaunch launch(dim3(static_cast<unsigned>(resident)), dim3(S::kWarps * 32), S::kBytes, stream);
   e = launch(kernel, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
   const int64_t rows = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
@@ -905,12 +1060,6 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   }
   PdlLaunch join(dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream);
   return join(attend_join<T, DP, S::kRows, 1>, p);
-}
-
-// New tokens of a sequence, as far as the caller knows; else their mean.
-int new_tokens(const AttendDev& p) {
-  const int mean = (p.a.batch.tokens + p.a.batch.seqs - 1) / p.a.batch.seqs;
-  return p.a.max_new > 0 ? (p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens) : mean;
 }
 
 // Whether the tcgen05 kernel for many query rows runs the call.  Its CTAs take

@@ -21,6 +21,7 @@ struct AttendDev {
   float* part;        // [workers][2][rows][dim] partial outputs
   float2* part_ml;    // [workers][2][rows] (reference, sum)
   int64_t workers;
+  int cluster;        // CTAs of a segment, where each has a cluster
 };
 
 // 2^x, at most 2^-22 of it off; 0 for -inf.
@@ -59,6 +60,23 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[kMaxDevice
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess && keep) done[device] = true;
   return e;
+}
+
+// Segments without a scan: sequence b's row tiles of ROWS packed rows stand at
+// slots starts[b] * group / ROWS + b on, which leaves room for all of them.
+__host__ __device__ inline int64_t first_slot(int64_t start, int b, int group, int rows) { return start * group / rows + b; }
+
+// A sequence whose table is wrong: recorded, and its rows of a kv head are NaN.
+template <class T>
+__device__ __forceinline__ void refuse_sequence(const AttendDev& p, int b, int head, int thread, int threads) {
+  if (thread == 0) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
+  const int dim = p.a.cache.dim;
+  const int64_t first = max(p.a.batch.starts[b], 0), end = min(p.a.batch.starts[b + 1], p.a.batch.tokens);
+  const int64_t each = static_cast<int64_t>(p.group) * dim;
+  for (int64_t i = thread; i < (end - first) * each; i += threads) {
+    const int64_t token = first + i / each, h = head * p.group + i % each / dim;
+    static_cast<T*>(p.a.out)[token * p.a.out_token + h * p.a.out_head + i % dim] = static_cast<T>(__int_as_float(0x7fc00000));
+  }
 }
 
 // The tcgen05 kernel for many query rows (attend_prompt.cu): bf16, dim <= 128.

@@ -181,28 +181,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
   griddep_launch_dependents();
   griddep_wait();
 
-  // --- which rows.  Sequence b's row tiles stand from slot starts[b] * group /
-  // 256 + b on; the last slots, which see the most tokens, come first.
+  // --- which rows.  The last slots, which see the most tokens, come first.
   Work work;
   {
     const int slot = slots - 1 - static_cast<int>(blockIdx.x) / cache.heads;
     work.head = static_cast<int>(blockIdx.x) % cache.heads;
-    auto base = [&](int i) { return static_cast<int64_t>(p.a.batch.starts[i]) * p.group / kRows + i; };
+    auto base = [&](int i) { return first_slot(p.a.batch.starts[i], i, p.group, kRows); };
     const int b = last_at_most(p.a.batch.seqs, slot, base);
     work.seq = load_sequence(p.a.batch, cache.page, b);
     work.table = p.a.batch.table + b * p.a.batch.table_stride;
     const int64_t index = slot - base(b);
     if (!work.seq.ok) {
-      // its table is wrong: recorded, and its rows are NaN
-      if (index != 0) return;
-      if (threadIdx.x == 0) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
-      const int64_t first = max(p.a.batch.starts[b], 0), end = min(p.a.batch.starts[b + 1], p.a.batch.tokens);
-      const int64_t each = static_cast<int64_t>(p.group) * dim;
-      for (int64_t i = threadIdx.x; i < (end - first) * each; i += kThreads) {
-        const int64_t token = first + i / each, h = work.head * p.group + i % each / dim;
-        static_cast<__nv_bfloat16*>(p.a.out)[token * p.a.out_token + h * p.a.out_head + i % dim] =
-            __float2bfloat16(__int_as_float(0x7fc00000));
-      }
+      if (index == 0) refuse_sequence<__nv_bfloat16>(p, b, work.head, threadIdx.x, kThreads);
       return;
     }
     const int64_t row0 = index * kRows, all = static_cast<int64_t>(work.seq.count) * p.group;
@@ -692,7 +682,7 @@ cudaError_t launch_dims(const AttendDev& p, cudaStream_t stream) {
   static std::atomic<bool> allowed[kMaxDevices];
   const cudaError_t e = allow_smem(attend_prompt<DP, CAP>, Layout<DP>::kBytes, allowed);
   if (e != cudaSuccess) return e;
-  const int64_t slots = static_cast<int64_t>(p.a.batch.tokens) * p.group / kRows + p.a.batch.seqs;
+  const int64_t slots = first_slot(p.a.batch.tokens, p.a.batch.seqs, p.group, kRows);
   PdlLaunch launch(dim3(static_cast<unsigned>(slots * p.a.cache.heads)), dim3(kThreads), Layout<DP>::kBytes, stream);
   return launch(attend_prompt<DP, CAP>, p, static_cast<int>(slots));
 }
