@@ -39,6 +39,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../serve.h"
 #include "attend.cuh"
@@ -270,8 +271,9 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   unsigned char* ring = smem + warp * S::kWarpBytes;
   const uint32_t ring_addr = sm100::smem_addr(ring);
   uint2* query = reinterpret_cast<uint2*>(ring + kStages * 2 * S::kMatrix);
-  uint64_t* landed = reinterpret_cast<uint64_t*>(smem + S::kWarps * S::kWarpBytes) + warp * kStages;  // a stage's data
-  int* abort_flag = reinterpret_cast<int*>(smem + S::kWarps * S::kWarpBytes + 128) + warp;
+  const int warps = kCluster ? blockDim.x >> 5 : S::kWarps;
+  uint64_t* landed = reinterpret_cast<uint64_t*>(smem + warps * S::kWarpBytes) + warp * kStages;  // a stage's data
+  int* abort_flag = reinterpret_cast<int*>(smem + warps * S::kWarpBytes + 128) + warp;
   const CacheView& cache = p.a.cache;
   const int dim = cache.dim;
 
@@ -302,12 +304,12 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
     const int64_t row_tile = slot - base(at.b);
     // the cluster's CTAs return together
     if (!at.seg.seq.ok) {
-      if (row_tile == 0 && rank == 0) refuse_sequence<T>(p, at.b, at.head, threadIdx.x, S::kWarps * 32);
+      if (row_tile == 0 && rank == 0) refuse_sequence<T>(p, at.b, at.head, threadIdx.x, blockDim.x);
       return;
     }
     if (row_tile < 0 || row_tile >= at.seg.row_tiles) return;
     at.row_tile = static_cast<int>(row_tile);
-    const int64_t tiles = at.seg.hi - at.seg.lo, of = p.cluster * S::kWarps, mine = rank * S::kWarps + warp;
+    const int64_t tiles = at.seg.hi - at.seg.lo, of = p.cluster * warps, mine = rank * warps + warp;
     at.tile = at.seg.lo + static_cast<int>(divide(tiles * mine, of));
     left = at.seg.lo + static_cast<int>(divide(tiles * (mine + 1), of)) - at.tile;
   } else {
@@ -776,6 +778,10 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
     }
   }
   if constexpr (kCluster) {
+    if (p.cluster * warps == 1) {
+      finish_segment(true);
+      return;
+    }
     // --- the warps' results, over their rings: [rows][dim], then (reference, sum) of each row
     __syncwarp();
     const float up = __uint_as_float(static_cast<uint32_t>(value_exp + 117) << 23);
@@ -801,55 +807,61 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       }
     __syncthreads();
     // --- the CTA's, four dims a thread, over warp 0's (its sums behind them)
-    constexpr int kThreads = S::kWarps * 32, kItems = kRows * DP / 4;
-    float2* cta_sums = sums_of(0) + kRows;
-    for (int item = threadIdx.x; item < kItems; item += kThreads) {
-      const int row = item / (DP / 4), d = item % (DP / 4) * 4;
-      float2 ml[S::kWarps];
-      float top = kNone;
+    auto join = [&](auto count) {
+      constexpr int kWarps = count.value, kThreads = kWarps * 32, kItems = kRows * DP / 4;
+      float2* cta_sums = sums_of(0) + kRows;
+      for (int item = threadIdx.x; item < kItems; item += kThreads) {
+        const int row = item / (DP / 4), d = item % (DP / 4) * 4;
+        float2 ml[kWarps];
+        float top = kNone;
 #pragma unroll
-      for (int w = 0; w < S::kWarps; ++w) {
-        ml[w] = sums_of(w)[row];
-        top = fmaxf(top, ml[w].x);
-      }
-      float s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < kWarps; ++w) {
+          ml[w] = sums_of(w)[row];
+          top = fmaxf(top, ml[w].x);
+        }
+        float s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < S::kWarps; ++w) {
-        const float by = exp2_fast(ml[w].x - top);
-        const float4 v = *reinterpret_cast<const float4*>(part_of(w) + row * DP + d);
-        s += ml[w].y * by;
-        y[0] += v.x * by, y[1] += v.y * by, y[2] += v.z * by, y[3] += v.w * by;
+        for (int w = 0; w < kWarps; ++w) {
+          const float by = exp2_fast(ml[w].x - top);
+          const float4 v = *reinterpret_cast<const float4*>(part_of(w) + row * DP + d);
+          s += ml[w].y * by;
+          y[0] += v.x * by, y[1] += v.y * by, y[2] += v.z * by, y[3] += v.w * by;
+        }
+        *reinterpret_cast<float4*>(part_of(0) + row * DP + d) = make_float4(y[0], y[1], y[2], y[3]);
+        if (d == 0) cta_sums[row] = make_float2(top, s);
       }
-      *reinterpret_cast<float4*>(part_of(0) + row * DP + d) = make_float4(y[0], y[1], y[2], y[3]);
-      if (d == 0) cta_sums[row] = make_float2(top, s);
-    }
-    // --- the cluster's: each CTA has a share of the items
-    if (p.cluster > 1)
-      sm100::cluster_sync();
+      // --- the cluster's: each CTA has a share of the items
+      if (p.cluster > 1)
+        sm100::cluster_sync();
+      else
+        __syncthreads();
+      const int rank = blockIdx.x % p.cluster;
+      for (int item = rank * kThreads + threadIdx.x; item < kItems; item += p.cluster * kThreads) {
+        const int row = item / (DP / 4), d = item % (DP / 4) * 4;
+        int i;
+        const int head = row_of(row, &i);
+        if (head < 0 || d >= dim) continue;
+        float top = kNone;
+        for (int c = 0; c < p.cluster; ++c) top = fmaxf(top, cluster_load2(cta_sums + row, c).x);
+        float s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < p.cluster; ++c) {
+          const float2 ml = cluster_load2(cta_sums + row, c);
+          const float4 v = cluster_load4(part_of(0) + row * DP + d, c);
+          const float by = exp2_fast(ml.x - top);
+          s += ml.y * by;
+          y[0] += v.x * by, y[1] += v.y * by, y[2] += v.z * by, y[3] += v.w * by;
+        }
+        const float over = s > 0.0f || s != s ? 1.0f / s : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= over;
+        Vec<T, 4>::store(static_cast<T*>(p.a.out) + static_cast<int64_t>(at.seg.seq.first + i) * p.a.out_token +
+                             static_cast<int64_t>(head) * p.a.out_head + d, y);
+      }
+    };
+    if (warps == S::kWarps)
+      join(std::integral_constant<int, S::kWarps>{});
     else
-      __syncthreads();
-    const int rank = blockIdx.x % p.cluster;
-    for (int item = rank * kThreads + threadIdx.x; item < kItems; item += p.cluster * kThreads) {
-      const int row = item / (DP / 4), d = item % (DP / 4) * 4;
-      int i;
-      const int head = row_of(row, &i);
-      if (head < 0 || d >= dim) continue;
-      float top = kNone;
-      for (int c = 0; c < p.cluster; ++c) top = fmaxf(top, cluster_load2(cta_sums + row, c).x);
-      float s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int c = 0; c < p.cluster; ++c) {
-        const float2 ml = cluster_load2(cta_sums + row, c);
-        const float4 v = cluster_load4(part_of(0) + row * DP + d, c);
-        const float by = exp2_fast(ml.x - top);
-        s += ml.y * by;
-        y[0] += v.x * by, y[1] += v.y * by, y[2] += v.z * by, y[3] += v.w * by;
-      }
-      const float over = s > 0.0f || s != s ? 1.0f / s : 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] *= over;
-      Vec<T, 4>::store(static_cast<T*>(p.a.out) + static_cast<int64_t>(at.seg.seq.first + i) * p.a.out_token +
-                           static_cast<int64_t>(head) * p.a.out_head + d, y);
-    }
+      join(std::integral_constant<int, 2>{});
     if (p.cluster > 1) sm100::cluster_sync();  // no CTA goes while another reads its memory
   }
 }
@@ -1001,18 +1013,27 @@ int new_tokens(const AttendDev& p) {
   return p.a.max_new > 0 ? (p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens) : mean;
 }
 
+// Tokens that a query tile of a sequence sees, at most, as far as the host knows.
+int64_t longest_seen(const AttendDev& p) {
+  const int64_t room = static_cast<int64_t>(p.a.batch.table_width) * p.a.cache.page;
+  if (p.a.window <= 0) return room;
+  // a window starts and ends inside a tile
+  return std::min<int64_t>(room, static_cast<int64_t>(p.a.window) + new_tokens(p) + kTile - 1);
+}
+
+// Segments of ``rows`` query rows.
+int64_t segments_of(const AttendDev& p, int rows) {
+  const int64_t tiles = (static_cast<int64_t>(new_tokens(p)) * p.group + rows - 1) / rows;
+  return static_cast<int64_t>(p.a.batch.seqs) * p.a.cache.heads * tiles;
+}
+
 template <int DP, bool F32, int NR>
 cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   using S = Shape<DP, F32, NR>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
   const int sms = sm_count(), dim = p.a.cache.dim, resident = sms * S::kCtas;
   static std::atomic<bool> allowed[3][kMaxDevices];
-  // At most this many tokens of a sequence are seen, as far as the host knows.
-  int64_t longest = static_cast<int64_t>(p.a.batch.table_width) * p.a.cache.page;
-  if (p.a.window > 0) longest = std::min<int64_t>(longest, static_cast<int64_t>(p.a.window) + new_tokens(p));
-  const int64_t tiles = (longest + kTile - 1) / kTile;
-  const int64_t segments = static_cast<int64_t>(p.a.batch.seqs) * p.a.cache.heads *
-                           ((static_cast<int64_t>(new_tokens(p)) * p.group + S::kRows - 1) / S::kRows);
+  const int64_t longest = longest_seen(p), tiles = (longest + kTile - 1) / kTile, segments = segments_of(p, S::kRows);
   // A cluster a segment where the whole is small: 1.3 units a nanosecond make
   // 16384 of them 12 us, of which an uneven share loses less than the join.
   if (segments * tiles <= 16384) {
@@ -1020,15 +1041,39 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
       *bytes = 0;
       return cudaSuccess;
     }
-    p.cluster = 8;
-    while (p.cluster > 1 && (segments * p.cluster > resident || p.cluster * S::kWarps > tiles)) p.cluster /= 2;
     auto kernel = attend_units<DP, F32, NR, Form::kCluster>;
     const cudaError_t e = allow_smem(kernel, S::kBytes, allowed[2]);
     if (e != cudaSuccess) return e;
-    const int64_t slots = first_slot(p.a.batch.tokens, p.a.batch.seqs, p.group, S::kRows);
-    PdlLaunch launch(dim3(static_cast<unsigned>(slots * p.a.cache.heads * p.cluster)), dim3(S::kWarps * 32), S::kBytes, stream,
-                     p.cluster);
-    return launch(kernel, p, CUtensorMap{}, CUtensorMap{});
+    const int64_t slots = first_slot(p.a.batch.tokens, p.a.batch.seqs, p.group, S::kRows) * p.a.cache.heads;
+    auto launch = [&](int warps, int cluster) {
+      return PdlLaunch(dim3(static_cast<unsigned>(slots * cluster)), dim3(warps * 32),
+                       S::kBytes - (S::kWarps - warps) * S::kWarpBytes, stream, cluster);
+    };
+    // A segment's warps: as many as it has tiles and the GPU has room for, so
+    // that many short segments stand side by side, each with a warp (50 sequences
+    // of 5 new tokens, 56 f32 heads and 28 tokens: 30.7 us with four warps for
+    // each segment, 10.8 with one).  A cluster's SMs are neighbours: how many fit
+    // is less than their CTAs would.
+    static std::atomic<int> fitting[2][kMaxDevices];  // 8 and 4 CTAs a cluster
+    auto fit = [&](int cluster) {
+      if (cluster <= 2) return resident / cluster;
+      int device = 0, n = 0;
+      cudaGetDevice(&device);
+      const bool keep = device >= 0 && device < kMaxDevices;
+      if (keep && fitting[cluster == 4][device]) return fitting[cluster == 4][device].load();
+      auto l = launch(S::kWarps, cluster);
+      l.attrs[0] = l.attrs[1], l.cfg.numAttrs = 1;  // the question knows no other attribute
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess) cudaGetLastError();
+      if (keep) fitting[cluster == 4][device] = n;
+      return n;
+    };
+    int warps = S::kWarps;
+    p.cluster = 8;
+    while (p.cluster > 1 && (p.cluster * warps > tiles || segments > fit(p.cluster))) p.cluster /= 2;
+    // alone, a CTA has fewer warps only where there is no room: one without a tile still helps with the join
+    if (tiles == 1) warps = 1;
+    while (p.cluster == 1 && warps > 1 && segments * warps > resident * S::kWarps) warps /= 2;
+    return launch(warps, p.cluster)(kernel, p, CUtensorMap{}, CUtensorMap{});
   }
   p.workers = static_cast<int64_t>(resident) * S::kWarps;
   if (bytes) {
@@ -1079,12 +1124,17 @@ bool for_prompt(const AttendDev& p) {
 
 // Query rows of a segment: 8, 16 or 32, by the rows that a sequence's new
 // tokens and the group make.  Registers hold 16 at dims over 128 and in f32.
+// Where the GPU has a warp for each unit of fewer rows (2368 of them run at
+// once at best), sharing units would only leave warps idle: 21 new tokens of 4
+// heads behind a window of 5 took 11.8 us with 32 rows and 5.6 with 8.
 template <int DP, bool F32>
 cudaError_t launch_rows_for(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   const int64_t rows = static_cast<int64_t>(new_tokens(p)) * p.group;
-  if (rows <= 8) return launch_shape<DP, F32, 1>(p, stream, bytes);
+  const int64_t tiles = (longest_seen(p) + kTile - 1) / kTile;
+  auto spread = [&](int fewer) { return segments_of(p, fewer) * tiles <= 16 * sm_count(); };
+  if (rows <= 8 || spread(8)) return launch_shape<DP, F32, 1>(p, stream, bytes);
   if constexpr (DP <= 128 && !F32) {
-    if (rows > 16) return launch_shape<DP, F32, 4>(p, stream, bytes);
+    if (rows > 16 && !spread(16)) return launch_shape<DP, F32, 4>(p, stream, bytes);
   }
   return launch_shape<DP, F32, 2>(p, stream, bytes);
 }
