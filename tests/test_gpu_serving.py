@@ -701,6 +701,45 @@ def test_attention_long_prompts(new, total, dim, heads, group, page, window, sof
     check_attention(cache, batch, q, window=window, softcap=softcap, max_new=max(new))
 
 
+@pytest.mark.parametrize("new, total", [([64], [2000]), ([128], [1600]), ([512], [1600]), ([70, 3, 90], [4000, 70, 2500])])
+@pytest.mark.parametrize("dim, heads, group, page", [(128, 8, 4, 64), (64, 8, 8, 48), (96, 10, 5, 40)])
+@pytest.mark.parametrize("window, softcap", [(0, 0.0), (1300, 0.0), (0, 20.0)])
+def test_attention_prompt_clusters(new, total, dim, heads, group, page, window, softcap):
+    """Few segments of many rows: clusters of two, four and eight that share the tokens of a segment."""
+    g = generator(dim + len(new))
+    batch = Batch(new, total, page, seed=3)
+    cache = filled_cache(g, batch.pages_held, heads, dim, page, 8)
+    q = normal(g, batch.tokens, heads * group, dim, std=1.5, dtype=torch.bfloat16)
+    y = check_attention(cache, batch, q, window=window, softcap=softcap, max_new=max(new))
+    assert torch.equal(y, xt.cache_attention(cache, q, *batch.args, window=window, softcap=softcap, max_new=max(new)))
+
+
+def test_attention_prompt_cluster_edges():
+    """Rows that see nothing, CTAs of a cluster that have no token, NaN in one CTA's share, wrong tables."""
+    g = generator(18)
+    batch = Batch([128], [1600], 64, seed=3)
+    cache = filled_cache(g, batch.pages_held, 8, 128, 64, 1)
+    q = normal(g, batch.tokens, 32, 128, std=1.5, dtype=torch.bfloat16)
+    starts, lengths, table = batch.args
+    good = check_attention(cache, batch, q)
+    short = torch.tensor([100], dtype=torch.int32, device="cuda")  # 28 queries before the first token, one tile at most
+    y = xt.cache_attention(cache, q, starts, short, table)
+    batch.total, batch.args = [100], (starts, short, table)
+    assert (y[:28] == 0).all() and torch.equal(y, check_attention(cache, batch, q))
+    none = torch.tensor([0], dtype=torch.int32, device="cuda")
+    assert (xt.cache_attention(cache, q, starts, none, table) == 0).all()
+    where = batch.table[0][700 // 64], 2, 700 % 64
+    cache.v_scale[where] = float("nan")
+    y = xt.cache_attention(cache, q, starts, lengths, table)
+    assert y[:, 8:12].isnan().all() and torch.equal(y[:, :8], good[:, :8]) and torch.equal(y[:, 12:], good[:, 12:])
+    cache.v_scale[where] = 0.02
+    wrong = table.clone()
+    wrong[0, 20] = -1
+    assert xt.cache_attention(cache, q, starts, lengths, wrong).isnan().all() and xt.device_error() == 0x303
+    over = torch.tensor([1 << 20], dtype=torch.int32, device="cuda")
+    assert xt.cache_attention(cache, q, starts, over, table).isnan().all() and xt.device_error() == 0x303
+
+
 def test_attention_long_prompt_edges():
     """Rows that see nothing, garbage that no row sees, NaN that one sequence's rows see, zero scales, wrong tables."""
     g = generator(16)

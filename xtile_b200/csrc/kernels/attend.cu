@@ -39,6 +39,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "../serve.h"
@@ -188,24 +189,6 @@ __device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
 // Arrives on ``bar`` once the calling lane's copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(sm100::smem_addr(bar)) : "memory");
-}
-
-// What lies at this address in the shared memory of CTA ``rank`` of the cluster.
-__device__ __forceinline__ float2 cluster_load2(const float2* p, int rank) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-               : "=f"(v.x), "=f"(v.y)
-               : "r"(sm100::mapa_shared(sm100::smem_addr(p), rank))
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(sm100::mapa_shared(sm100::smem_addr(p), rank))
-               : "memory");
-  return v;
 }
 
 // c += a b for 16 x 16 f16 a, 16 x 8 f16 b, f32 c.
@@ -615,7 +598,10 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[nr][e] = tanhf(z[nr][e] * capped_scale[nr][e & 1]) * (cap * kLog2e);
+        for (int e = 0; e < 4; ++e) {
+          const float x = z[nr][e] * capped_scale[nr][e & 1];
+          z[nr][e] = (F32 ? tanhf(x) : tanh_fast(x)) * (cap * kLog2e);
+        }
     }
     auto exponents = [&] {
       float top = -INFINITY;
@@ -1007,33 +993,13 @@ bool cache_map(CUtensorMap* map, const void* base, int dim, uint64_t lines, int 
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// New tokens of a sequence, as far as the caller knows; else their mean.
-int new_tokens(const AttendDev& p) {
-  const int mean = (p.a.batch.tokens + p.a.batch.seqs - 1) / p.a.batch.seqs;
-  return p.a.max_new > 0 ? (p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens) : mean;
-}
-
-// Tokens that a query tile of a sequence sees, at most, as far as the host knows.
-int64_t longest_seen(const AttendDev& p) {
-  const int64_t room = static_cast<int64_t>(p.a.batch.table_width) * p.a.cache.page;
-  if (p.a.window <= 0) return room;
-  // a window starts and ends inside a tile
-  return std::min<int64_t>(room, static_cast<int64_t>(p.a.window) + new_tokens(p) + kTile - 1);
-}
-
-// Segments of ``rows`` query rows.
-int64_t segments_of(const AttendDev& p, int rows) {
-  const int64_t tiles = (static_cast<int64_t>(new_tokens(p)) * p.group + rows - 1) / rows;
-  return static_cast<int64_t>(p.a.batch.seqs) * p.a.cache.heads * tiles;
-}
-
 template <int DP, bool F32, int NR>
 cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   using S = Shape<DP, F32, NR>;
   using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
   const int sms = sm_count(), dim = p.a.cache.dim, resident = sms * S::kCtas;
   static std::atomic<bool> allowed[3][kMaxDevices];
-  const int64_t longest = longest_seen(p), tiles = (longest + kTile - 1) / kTile, segments = segments_of(p, S::kRows);
+  const int64_t longest = longest_seen(p, kTile), tiles = (longest + kTile - 1) / kTile, segments = segments_of(p, S::kRows);
   // A cluster a segment where the whole is small: 1.3 units a nanosecond make
   // 16384 of them 12 us, of which an uneven share loses less than the join.
   if (segments * tiles <= 16384) {
@@ -1057,15 +1023,7 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
     static std::atomic<int> fitting[2][kMaxDevices];  // 8 and 4 CTAs a cluster
     auto fit = [&](int cluster) {
       if (cluster <= 2) return resident / cluster;
-      int device = 0, n = 0;
-      cudaGetDevice(&device);
-      const bool keep = device >= 0 && device < kMaxDevices;
-      if (keep && fitting[cluster == 4][device]) return fitting[cluster == 4][device].load();
-      auto l = launch(S::kWarps, cluster);
-      l.attrs[0] = l.attrs[1], l.cfg.numAttrs = 1;  // the question knows no other attribute
-      if (cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess) cudaGetLastError();
-      if (keep) fitting[cluster == 4][device] = n;
-      return n;
+      return clusters_at_once(kernel, launch(S::kWarps, cluster), fitting[cluster == 4]);
     };
     int warps = S::kWarps;
     p.cluster = 8;
@@ -1107,19 +1065,38 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   return join(attend_join<T, DP, S::kRows, 1>, p);
 }
 
-// Whether the tcgen05 kernel for many query rows runs the call.  Its CTAs take
-// about 3.7 us for 256 rows and 128 tokens, however few of the rows there are
-// and however few CTAs; attend_units spreads any work over the GPU, at 3.1 us
-// for a million (row, token) pairs of 128 dims.  They meet near 10000 rows
-// (us, attend_units and this one): 8192 rows of one sequence 123 and 126 at 4096
-// tokens, 16384 221 and 125; 64 sequences of 32 rows each and 8 heads 82 and
-// 113, of 64 rows 128 and 115.
-bool for_prompt(const AttendDev& p) {
+// Whether the tcgen05 kernel for many query rows runs the call, and the CTAs
+// that share a segment's tokens in it, by what the two kernels would take as far
+// as the host knows (us; fitted to 1 to 89 sequences of 1024 to 65536 tokens,
+// 4 to 512 of them new, within a third of what was measured):
+//   that one    6.5, 6.5 a wave of CTAs (7.5 where clusters join), and 2.2 or 2.7
+//               a tile of 128 tokens with 64 or 128 dims and up to 128 rows, 2.8
+//               or 3.4 with up to 256
+//   this one    4 to 20, and 1.7 or 3.0 for a million (row, token) pairs
+// 16384 rows of one sequence and 4096 tokens: 240 here, 79 there; 256 rows 25 and
+// 24; 64 sequences of 32 rows, 8 heads and up to 1024 tokens 85 and 112.
+bool for_prompt(AttendDev& p) {
   const int64_t rows = static_cast<int64_t>(new_tokens(p)) * p.group;
-  const int64_t all = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
   const bool vectors = reinterpret_cast<uintptr_t>(p.a.q) % 16 == 0 && reinterpret_cast<uintptr_t>(p.a.out) % 16 == 0 &&
                        p.a.q_token % 8 == 0 && p.a.q_head % 8 == 0 && p.a.out_token % 8 == 0 && p.a.out_head % 8 == 0;
-  return p.a.elem == kBF16 && p.a.cache.dim <= 128 && vectors && rows >= 64 && all >= 10240;
+  if (p.a.elem != kBF16 || p.a.cache.dim > 128 || !vectors || rows <= 16) return false;
+  const bool small = p.a.cache.dim <= 64;
+  const int64_t longest = longest_seen(p, 128), tiles = (longest + 127) / 128, segments = segments_of(p, 256);
+  const float tile_us = small ? (rows <= 128 ? 2.2f : 2.8f) : rows <= 128 ? 2.7f : 3.4f;
+  float best = 0.0f;
+  for (int cluster = 1; cluster <= 8 && cluster <= tiles; cluster *= 2) {
+    const int64_t at_once = cluster == 1 ? sm_count() : prompt_clusters(cluster);
+    if (at_once == 0) break;
+    // ragged or many segments fill each other's gaps
+    float waves = std::max(static_cast<float>(segments) / at_once, 1.0f);
+    if (p.a.batch.seqs == 1 && waves < 2.0f) waves = std::ceil(waves);
+    const float us = 6.5f + waves * (tile_us * ((tiles + cluster - 1) / cluster) + (cluster > 1 ? 7.5f : 6.5f));
+    if (cluster > 1 && us >= best) continue;
+    best = us;
+    p.cluster = cluster;
+  }
+  const float pairs = static_cast<float>(segments_of(p, 32)) * 32e-6f * longest;
+  return best < 4.0f + std::min(16.0f, longest / 160.0f) + (small ? 1.7f : 3.0f) * pairs;
 }
 
 // Query rows of a segment: 8, 16 or 32, by the rows that a sequence's new
@@ -1130,7 +1107,7 @@ bool for_prompt(const AttendDev& p) {
 template <int DP, bool F32>
 cudaError_t launch_rows_for(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   const int64_t rows = static_cast<int64_t>(new_tokens(p)) * p.group;
-  const int64_t tiles = (longest_seen(p) + kTile - 1) / kTile;
+  const int64_t tiles = (longest_seen(p, kTile) + kTile - 1) / kTile;
   auto spread = [&](int fewer) { return segments_of(p, fewer) * tiles <= 16 * sm_count(); };
   if (rows <= 8 || spread(8)) return launch_shape<DP, F32, 1>(p, stream, bytes);
   if constexpr (DP <= 128 && !F32) {

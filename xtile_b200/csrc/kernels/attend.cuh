@@ -4,9 +4,12 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../serve.h"
+#include "pdl.cuh"
+#include "sm100.cuh"
 
 namespace xt {
 namespace dev {
@@ -21,7 +24,7 @@ struct AttendDev {
   float* part;        // [workers][2][rows][dim] partial outputs
   float2* part_ml;    // [workers][2][rows] (reference, sum)
   int64_t workers;
-  int cluster;        // CTAs of a segment, where each has a cluster
+  int cluster;        // CTAs of a segment, which then has a cluster
 };
 
 // 2^x, at most 2^-22 of it off; 0 for -inf.
@@ -48,6 +51,35 @@ __device__ __forceinline__ uint32_t bytes_to_half2(uint32_t biased) {
 }
 constexpr uint32_t kLow = 0x4140u, kHigh = 0x4342u;  // bytes 0, 1 and bytes 2, 3
 
+// What lies at this address in the shared memory of CTA ``rank`` of the cluster.
+__device__ __forceinline__ float2 cluster_load2(const float2* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(sm100::mapa_shared(sm100::smem_addr(p), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(sm100::mapa_shared(sm100::smem_addr(p), rank))
+               : "memory");
+  return v;
+}
+
+// tanh(x) for scores whose weights are rounded to f16: 1 - 2 / (1 + e^2x), at
+// most 2^-22 off, and the first terms of its series near 0, where that would
+// cancel; 2^-18 of the value at most.  Two chunks of 2048 new tokens behind 2048
+// with capped scores took 441 us with tanhf and 405 with this.
+__device__ __forceinline__ float tanh_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(x * (2.0f * kLog2e))));
+  const float s = x * x;
+  return s < 0.0225f ? x * fmaf(s, fmaf(s, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f) : fmaf(-2.0f, r, 1.0f);
+}
+
 constexpr int kMaxDevices = 64;
 
 // Grants ``kernel`` its shared memory, once a device.
@@ -62,9 +94,47 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[kMaxDevice
   return e;
 }
 
+// Clusters of a launch that the GPU runs at once, asked once a device.
+template <class K>
+int clusters_at_once(K kernel, PdlLaunch launch, std::atomic<int> (&known)[kMaxDevices]) {
+  int device = 0, n = 0;
+  cudaGetDevice(&device);
+  const bool keep = device >= 0 && device < kMaxDevices;
+  if (keep && known[device]) return known[device];
+  launch.attrs[0] = launch.attrs[1];  // the question knows no other attribute
+  launch.cfg.attrs = launch.attrs;
+  launch.cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &launch.cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (keep) known[device] = n;
+  return n;
+}
+
 // Segments without a scan: sequence b's row tiles of ROWS packed rows stand at
 // slots starts[b] * group / ROWS + b on, which leaves room for all of them.
 __host__ __device__ inline int64_t first_slot(int64_t start, int b, int group, int rows) { return start * group / rows + b; }
+
+// New tokens of a sequence, as far as the caller knows; else their mean.
+inline int new_tokens(const AttendDev& p) {
+  const int mean = (p.a.batch.tokens + p.a.batch.seqs - 1) / p.a.batch.seqs;
+  return p.a.max_new > 0 ? (p.a.max_new < p.a.batch.tokens ? p.a.max_new : p.a.batch.tokens) : mean;
+}
+
+// Tokens that a query tile of a sequence sees, at most, as far as the host knows.
+inline int64_t longest_seen(const AttendDev& p, int tile) {
+  const int64_t room = static_cast<int64_t>(p.a.batch.table_width) * p.a.cache.page;
+  if (p.a.window <= 0) return room;
+  // a window starts and ends inside a tile
+  return std::min<int64_t>(room, static_cast<int64_t>(p.a.window) + new_tokens(p) + tile - 1);
+}
+
+// Segments of ``rows`` query rows.
+inline int64_t segments_of(const AttendDev& p, int rows) {
+  const int64_t tiles = (static_cast<int64_t>(new_tokens(p)) * p.group + rows - 1) / rows;
+  return static_cast<int64_t>(p.a.batch.seqs) * p.a.cache.heads * tiles;
+}
 
 // A sequence whose table is wrong: recorded, and its rows of a kv head are NaN.
 template <class T>
@@ -80,7 +150,9 @@ __device__ __forceinline__ void refuse_sequence(const AttendDev& p, int b, int h
 }
 
 // The tcgen05 kernel for many query rows (attend_prompt.cu): bf16, dim <= 128.
+// Each segment of 256 rows has p.cluster CTAs.
 cudaError_t launch_attend_prompt(const AttendDev& p, cudaStream_t stream);
+int prompt_clusters(int cluster);  // clusters of 2, 4 or 8 CTAs that run at once
 
 }  // namespace dev
 }  // namespace xt

@@ -15,6 +15,11 @@
 //                    turn them into f16 in shared memory (128-byte swizzle,
 //                    two stages); one such group for both was the bottleneck
 //
+// Where there are few segments a cluster of up to eight CTAs has each: they share
+// out its token tiles, leave their f32 sums in shared memory and join a share of
+// the rows each (16384 rows of one sequence and 4096 tokens: 124 us alone, 79 in
+// clusters of two; 2048 rows 122 and 32).
+//
 // Registers go where the rows are: 168 a softmax thread, 88 a converting one.
 // While one query tile's softmax runs, the tensor cores work for the other.
 // The scores of the next token tile go to the same columns as the weights that
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
   Bars& bars = *reinterpret_cast<Bars*>(smem + L::kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const CacheView& cache = p.a.cache;
-  const int dim = cache.dim;
+  const int dim = cache.dim, rank = static_cast<int>(blockIdx.x) % p.cluster;
 
   griddep_launch_dependents();
   griddep_wait();
@@ -184,8 +189,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
   // --- which rows.  The last slots, which see the most tokens, come first.
   Work work;
   {
-    const int slot = slots - 1 - static_cast<int>(blockIdx.x) / cache.heads;
-    work.head = static_cast<int>(blockIdx.x) % cache.heads;
+    const int index_of = static_cast<int>(blockIdx.x) / p.cluster;
+    const int slot = slots - 1 - index_of / cache.heads;
+    work.head = index_of % cache.heads;
     auto base = [&](int i) { return first_slot(p.a.batch.starts[i], i, p.group, kRows); };
     const int b = last_at_most(p.a.batch.seqs, slot, base);
     work.seq = load_sequence(p.a.batch, cache.page, b);
@@ -205,6 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
     const int seen_from = p.a.window > 0 ? pos_first - p.a.window + 1 : 0;
     work.lo = seen_from > 0 ? seen_from / kTokens : 0;
     work.hi = pos_last < 0 ? work.lo : max(pos_last / kTokens + 1, work.lo);
+    // a cluster's CTAs share them out (and returned together above)
+    const int all_tiles = work.hi - work.lo, first = all_tiles * rank / p.cluster;
+    work.hi = work.lo + all_tiles * (rank + 1) / p.cluster;
+    work.lo += first;
   }
   const int tiles = work.hi - work.lo;
   const int queries = work.rows > kTileRows ? 2 : 1;  // query tiles that have rows
@@ -235,6 +245,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
   // TMEM columns: scores and weights of the two query tiles, then outputs
   auto score_at = [&](int w) { return tmem + w * 128; };
   auto out_at = [&](int w) { return tmem + 256 + w * 128; };
+
+  // Where a cluster shares the tokens: a query tile's f32 sums in the rooms of the
+  // keys (tile 0) and of the values (tile 1), and in its own room each row's
+  // (exponent of the sums, sum of the weights)
+  auto part_at = [&](int row, int chunk) {  // four dims
+    return reinterpret_cast<float*>(smem + L::kKeys + (row >> 7) * 2 * L::kMatrix + (row & 127) * DP * 4 + ((chunk ^ (row & 7)) << 4));
+  };
+  auto part_sum = [&](int row) { return reinterpret_cast<float2*>(smem + L::kQuery + (row >> 7) * L::kMatrix) + (row & 127); };
 
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
@@ -396,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
               if constexpr (CAP) {
                 float a, b;
                 unpack2(z, a, b);
-                z = pack2(tanhf(a * row_scale) * (cap * kLog2e), tanhf(b * row_scale) * (cap * kLog2e));
+                z = pack2(tanh_fast(a * row_scale) * (cap * kLog2e), tanh_fast(b * row_scale) * (cap * kLog2e));
               }
               z = fma2(z, by, add);
               float a, b;
@@ -539,35 +557,53 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       float s0, s1;
       unpack2(sum, s0, s1);
       s0 += s1;
-      const float over = s0 > 0.0f || s0 != s0 ? 1.0f / s0 : 0.0f;
-      // the row's values to the query tile's room (its last product is done), from
-      // where DP / 8 lanes store each row
-      uint8_t* room = smem + L::kQuery + w * L::kMatrix + (warp & 3) * 32 * DP * 2;
+      if (p.cluster > 1) {
+        named_barrier_sync(3, queries * 128);  // the products of both tiles are done
 #pragma unroll 1
-      for (int d = 0; d < DP; d += 32) {
-        uint32_t r[32];
-        if (tiles > 0) {
-          tmem_ld_32x32b_x32(result + d, r);
-          tmem_wait_ld();
-        }
+        for (int d = 0; d < DP; d += 32) {
+          uint32_t r[32];
+          if (tiles > 0) {
+            tmem_ld_32x32b_x32(result + d, r);
+            tmem_wait_ld();
+          }
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t v[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            v[x] = tiles > 0 ? pack_bf16(__uint_as_float(r[8 * h + 2 * x]) * over, __uint_as_float(r[8 * h + 2 * x + 1]) * over) : 0;
-          *reinterpret_cast<uint4*>(room + lane * DP * 2 + (((d / 8 + h) ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+          for (int h = 0; h < 8; ++h)
+            *reinterpret_cast<uint4*>(part_at(local, d / 4 + h)) =
+                tiles > 0 ? make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]) : make_uint4(0, 0, 0, 0);
         }
-      }
-      __syncwarp();
-      Rows row = first_row();
+        // the weights carry 2^(up - ref); a wait that gave up leaves NaN
+        *part_sum(local) = make_float2(ref - up, ok ? s0 : __int_as_float(0x7fc00000));
+      } else {
+        const float over = s0 > 0.0f || s0 != s0 ? 1.0f / s0 : 0.0f;
+        // the row's values to the query tile's room (its last product is done), from
+        // where DP / 8 lanes store each row
+        uint8_t* room = smem + L::kQuery + w * L::kMatrix + (warp & 3) * 32 * DP * 2;
+#pragma unroll 1
+        for (int d = 0; d < DP; d += 32) {
+          uint32_t r[32];
+          if (tiles > 0) {
+            tmem_ld_32x32b_x32(result + d, r);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t v[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              v[x] = tiles > 0 ? pack_bf16(__uint_as_float(r[8 * h + 2 * x]) * over, __uint_as_float(r[8 * h + 2 * x + 1]) * over) : 0;
+            *reinterpret_cast<uint4*>(room + lane * DP * 2 + (((d / 8 + h) ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        __syncwarp();
+        Rows row = first_row();
 #pragma unroll 4
-      for (int x = 0; x < kSteps; ++x) {
-        const int at = x * kWarpRows + sub;
-        const uint4 v = *reinterpret_cast<const uint4*>(room + at * DP * 2 + ((part ^ (at & 7)) << 4));
-        if (row.at < work.rows && part_there && ok)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + offset(row, p.a.out_token, p.a.out_head)) = v;
-        next_row(row);
+        for (int x = 0; x < kSteps; ++x) {
+          const int at = x * kWarpRows + sub;
+          const uint4 v = *reinterpret_cast<const uint4*>(room + at * DP * 2 + ((part ^ (at & 7)) << 4));
+          if (row.at < work.rows && part_there && ok)
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + offset(row, p.a.out_token, p.a.out_head)) = v;
+          next_row(row);
+        }
       }
       tc_fence_before();
       if (issuer && *ab.flag) {
@@ -576,6 +612,32 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         __syncwarp();
         mbar_wait_drain(&bars.drain[w], 0, 500000000ull);
       }
+    }
+    if (p.cluster > 1) {
+      cluster_sync();
+      // --- each CTA joins a share of the rows, four dims a thread
+      for (int item = rank * 256 + threadIdx.x; item < work.rows * (DP / 4); item += p.cluster * 256) {
+        const int row = item / (DP / 4), part = item % (DP / 4);
+        if (part * 4 >= dim) continue;
+        float top = 2.0f * kNone;
+        for (int c = 0; c < p.cluster; ++c) top = fmaxf(top, cluster_load2(part_sum(row), c).x);
+        float s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < p.cluster; ++c) {
+          const float2 sums = cluster_load2(part_sum(row), c);
+          const float4 v = cluster_load4(part_at(row, part), c);
+          const float by = exp2_fast(sums.x - top);
+          s += sums.y * by;
+          y[0] += v.x * by, y[1] += v.y * by, y[2] += v.z * by, y[3] += v.w * by;
+        }
+        const float over = s > 0.0f || s != s ? 1.0f / s : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= over;
+        const int token = p.group_div.quot(work.row0 + row), head = work.row0 + row - token * p.group;
+        Vec<__nv_bfloat16, 4>::store(static_cast<__nv_bfloat16*>(p.a.out) +
+                                         static_cast<int64_t>(work.seq.first + token) * p.a.out_token +
+                                         static_cast<int64_t>(work.head * p.group + head) * p.a.out_head + part * 4, y);
+      }
+      cluster_sync();  // no CTA goes while another reads its memory
     }
   } else {
     // ------------------------------------------------------------- converting
@@ -669,6 +731,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       mbar_arrive(&bars.scales_full[slot]);
       if (j + 1 < tiles) fetch(j + 1);
     }
+    if (p.cluster > 1) {
+      cluster_sync();
+      cluster_sync();
+    }
   }
   __syncthreads();
   if (warp == 15) {
@@ -683,11 +749,22 @@ cudaError_t launch_dims(const AttendDev& p, cudaStream_t stream) {
   const cudaError_t e = allow_smem(attend_prompt<DP, CAP>, Layout<DP>::kBytes, allowed);
   if (e != cudaSuccess) return e;
   const int64_t slots = first_slot(p.a.batch.tokens, p.a.batch.seqs, p.group, kRows);
-  PdlLaunch launch(dim3(static_cast<unsigned>(slots * p.a.cache.heads)), dim3(kThreads), Layout<DP>::kBytes, stream);
+  PdlLaunch launch(dim3(static_cast<unsigned>(slots * p.a.cache.heads * p.cluster)), dim3(kThreads), Layout<DP>::kBytes, stream,
+                   p.cluster);
   return launch(attend_prompt<DP, CAP>, p, static_cast<int>(slots));
 }
 
 }  // namespace
+
+int prompt_clusters(int cluster) {
+  // every instance has an SM to itself
+  static std::atomic<bool> allowed[kMaxDevices];
+  static std::atomic<int> known[3][kMaxDevices];
+  auto kernel = attend_prompt<128, false>;
+  if (allow_smem(kernel, Layout<128>::kBytes, allowed) != cudaSuccess) return 0;
+  return clusters_at_once(kernel, PdlLaunch(dim3(cluster), dim3(kThreads), Layout<128>::kBytes, nullptr, cluster),
+                          known[cluster == 8 ? 2 : cluster == 4]);
+}
 
 cudaError_t launch_attend_prompt(const AttendDev& p, cudaStream_t stream) {
   const bool cap = p.a.softcap > 0.0f;
