@@ -198,7 +198,9 @@ int xt_matmul_launch_noalloc(const xt_module* module, const char* func, void* co
  * once.  What only the device knows (positions, lengths, page tables) is
  * checked there: an entry that names something outside the arrays is not
  * followed, its results are NaN or left unwritten, and xt_device_error gives
- * 0x301 (rope position), 0x302 (append) or 0x303 (attention). */
+ * 0x301 (rope position), 0x302 (append) or 0x303 (attention).  The attention
+ * kernels' waits for their own copies and products are bounded like those of
+ * xt_launch; one that runs out gives 0x304, 0x305 or 0x307. */
 
 /* y = h * rsqrt(mean(h^2) + eps) * weight with h = x + residual, row by row.
  * y_elem XT_ELEM_I8: y = rint(v / s) with the row's s = max|v| / 127 in

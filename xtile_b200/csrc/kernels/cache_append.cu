@@ -9,8 +9,9 @@
 // largest magnitude and the rounding.  So a unit (one block of one head, of the
 // keys or of the values) belongs to as few lanes as hold it in registers
 // between the largest magnitude and the rounding, and what finds the block's
-// place is done once a warp: 17.5k tokens of 8 heads took 73 us with a CTA of
-// four warps a unit.
+// place is done once a warp: 17.1k tokens of 8 heads of 128 bf16
+// take 36.7 us (2860 GB/s), and took 73 with a CTA of four warps a unit; 64
+// single tokens take 3.6 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

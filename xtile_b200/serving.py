@@ -9,7 +9,8 @@
 raises ``TypeError`` (types) or ``ValueError`` (shapes, devices, layouts)
 before anything runs.  Positions, lengths and page tables live on the device:
 an entry outside the arrays is not followed, and ``device_error()`` reports it
-(0x301 rope, 0x302 append, 0x303 attention).
+(0x301 rope, 0x302 append, 0x303 attention; 0x304, 0x305 and 0x307 are bounded
+waits of the attention kernels that ran out).
 
 A ragged batch is described by three int32 tensors: ``starts`` [seqs + 1],
 ``lengths`` [seqs] and ``pages`` [seqs, width].  Sequence ``b`` has
@@ -167,8 +168,8 @@ def cache_attention(cache: KVCache, q, starts, lengths, pages, out=None, *, max_
     sequence's tokens up to its own (the last ``window`` of them if window > 0); one
     that sees none gives 0.  ``scale`` defaults to ``dim ** -0.5``; ``softcap`` > 0
     caps the scaled scores by ``softcap * tanh(score / softcap)``.  ``max_new``, the
-    most new tokens of one sequence, helps to choose the kernel; results do not
-    depend on it.
+    most new tokens of one sequence, helps to choose the kernel; it changes
+    nothing that is computed, only the order of sums and so their last bits.
     """
     if not isinstance(cache, KVCache):
         _no_cache(cache)
