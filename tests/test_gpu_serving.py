@@ -334,6 +334,23 @@ def test_cache_append(new, total, dim, rot, interleaved, dtype, page, block):
     check_append(cache, before, batch, kv[:, 0], kv[:, 1], table)
 
 
+@pytest.mark.parametrize("dim, rot, interleaved, dtype", [(128, 128, False, torch.float32), (80, 40, True, torch.float32),
+                                                          (80, 40, False, torch.bfloat16), (128, 64, True, torch.bfloat16)])
+@pytest.mark.parametrize("new, total", [([5 + i % 30 for i in range(100)], [40 + 3 * i for i in range(100)]), ([900], [1000])])
+def test_cache_append_many_blocks(new, total, dim, rot, interleaved, dtype):
+    """Enough blocks that each belongs to one warp, at the sizes where a few of them would have a CTA each."""
+    g = generator(dim)
+    batch = Batch(new, total, 64, seed=dim)
+    cache = filled_cache(g, batch.pages_held, 8, dim, 64, 16)
+    before = snapshot(cache)
+    kv = normal(g, batch.tokens, 2, 8, dim, dtype=dtype)
+    kv[:, :, 1] *= 3
+    kv[:, :, 2] *= 0.1
+    table = xt.RopeTable.build(max(total) + 1, rot, interleaved=interleaved)
+    xt.cache_append(cache, kv[:, 0], kv[:, 1], *batch.args, rope=table)
+    check_append(cache, before, batch, kv[:, 0], kv[:, 1], table)
+
+
 def test_cache_append_token_by_token_and_at_once():
     """A prompt appended at once and token by token: the same scales, values within the steps of the roundings."""
     g = generator(2)

@@ -251,10 +251,16 @@ cudaError_t launch_typed(const AppendArgs& a, cudaStream_t stream) {
     PdlLaunch launch(dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, stream);
     return launch(kernel, p);
   };
-  // the fewest lanes that hold a whole block (4 items a lane: 64 bf16 elements)
+  // the fewest lanes that hold a whole block in 64 registers each; few blocks of
+  // more than 128 items are quicker with a CTA each (17.1k tokens of 8 f32 heads
+  // of 128: 111 us with 256 lanes a block, 45 with 32; 600 of 2 heads 3.5 and 5.2;
+  // they meet near 1000 blocks)
   const int64_t items = static_cast<int64_t>(a.cache.block) * row;
   if (items <= 8) return go(cache_append_blocks<T, V, 8, 1>, 8);
   if (items <= 128) return go(cache_append_blocks<T, V, 32, 4>, 32);
+  if constexpr (V == 4) {
+    if (items <= 256 && slots * 2 * a.cache.heads >= 1024) return go(cache_append_blocks<T, V, 32, 8>, 32);
+  }
   return go(cache_append_blocks<T, V, kThreads, 4>, kThreads);
 }
 
