@@ -889,6 +889,18 @@ def test_dequantize(runs, run, dtype):
     assert torch.equal(got, (q.float() * s[:, None]).to(dtype))
 
 
+@pytest.mark.parametrize("run", [4096, 4097])
+def test_dequantize_behind_31_bits(run):
+    runs = (1 << 31) // run + 3
+    q = torch.empty(runs, run, dtype=torch.int8, device="cuda")
+    q.view(-1)[:] = 3
+    q[-5:] = torch.arange(-60, 60, dtype=torch.int8, device="cuda").repeat(run // 120 + 1)[:run]
+    s = torch.arange(runs, device="cuda").float()
+    got = xt.dequantize(q, s)
+    assert torch.equal(got[-9:], (q[-9:].float() * s[-9:, None]).bfloat16())
+    assert torch.equal(got[:, run // 2], (3 * s).bfloat16().where(torch.arange(runs, device="cuda") < runs - 5, got[:, run // 2]))
+
+
 def test_dequantize_cache_blocks():
     g = generator(1)
     cache = filled_cache(g, 5, 3, 80, 40, 20)

@@ -1,9 +1,13 @@
 // Rotary positions over heads, and int8 data read back as values.  Both are
 // bound by HBM: each element is read once and written once.  8192 tokens of 32
-// f32 heads of 128 take 45.3 us, 5970 GB/s; 67 million int8 values to bf16 33.7
-// us, 5980 GB/s; a decode step's 16 tokens 1.9 us.
+// f32 heads of 128 take 45.3 us, 5970 GB/s; 67 million int8 values to bf16 31.3
+// us, 6430 GB/s; a decode step's 16 tokens 1.9 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
 
 #include "../serve.h"
 #include "pdl.cuh"
@@ -81,92 +85,66 @@ cudaError_t launch_rope_typed(const RopeArgs& a, cudaStream_t stream) {
   return threads >= 4 * 148 * 1024 ? go(rope_heads<T, U, V, 4>, 4) : go(rope_heads<T, U, V, 1>, 1);
 }
 
-// 16 int8 values as f32 or bf16, one scale.
-template <class U>
-__device__ __forceinline__ void dequantize_16(const int4& w, float s, U* out) {
-  const int words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      y[e] = static_cast<float>(static_cast<int8_t>(words[2 * j + e / 4] >> (8 * (e % 4)))) * s;
-    Vec<U, 8>::store(out + 8 * j, y);
-  }
-}
-
-// Runs of whole 16-byte vectors: two a thread, both loads under way at once.
-template <class U>
-__global__ void __launch_bounds__(kThreads) dequantize_runs(const int8_t* __restrict__ q, const float* __restrict__ scales,
-                                                            U* __restrict__ out, int64_t vectors, int64_t run) {
+// An item is what makes 16 bytes of values; a thread has ITEMS of them, a CTA's
+// width apart and all under way at once, so that a warp reads and writes whole
+// lines (16 values a thread at once took 30 us where 25 million f32 ones take
+// 21).  ONE: runs are whole items, so an item has one scale.
+template <class U, bool ONE>
+__global__ void __launch_bounds__(kThreads) dequantize_items(const int8_t* __restrict__ q, const float* __restrict__ scales,
+                                                             U* __restrict__ out, int64_t n, int64_t run, FastDiv run_div) {
+  constexpr int kValues = 16 / sizeof(U), kItems = 32 / kValues;
+  using Word = typename std::conditional<kValues == 4, uint32_t, uint2>::type;
   griddep_launch_dependents();
   griddep_wait();
-  const int4* q4 = reinterpret_cast<const int4*>(q);
-  const int64_t run_vectors = run / 16;
-  auto scale_of = [&](int64_t i) {
-    return scales[(i | run_vectors) >> 32 ? i / run_vectors : static_cast<uint32_t>(i) / static_cast<uint32_t>(run_vectors)];
-  };
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * (2 * kThreads);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (2 * kThreads) + threadIdx.x; i < vectors; i += stride) {
-    const int64_t k = i + kThreads;
-    const bool two = k < vectors;
-    const int4 a = q4[i], b = two ? q4[k] : make_int4(0, 0, 0, 0);
-    const float sa = scale_of(i), sb = two ? scale_of(k) : 0.0f;
-    dequantize_16(a, sa, out + 16 * i);
-    if (two) dequantize_16(b, sb, out + 16 * k);
-  }
-}
-
-// Any runs: 16 values a thread, whose scales may change anywhere.
-template <class U>
-__global__ void __launch_bounds__(kThreads) dequantize_any(const int8_t* __restrict__ q, const float* __restrict__ scales,
-                                                           U* __restrict__ out, int64_t n, int64_t run) {
-  griddep_launch_dependents();
-  griddep_wait();
-  const int64_t vectors = (n + 15) / 16;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < vectors;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t at = i * 16;
-    int64_t r = (at | run) >> 32 ? at / run : static_cast<uint32_t>(at) / static_cast<uint32_t>(run);
-    if (at + 16 <= n) {
-      const int4 w = *reinterpret_cast<const int4*>(q + at);
-      const int words[4] = {w.x, w.y, w.z, w.w};
-      float s = scales[r];
-      int64_t left = (r + 1) * run - at;  // elements until the next scale
+  const int64_t items = n / kValues;
+  auto run_of = [&](int64_t at) { return run_div.d ? static_cast<int64_t>(run_div.quot(static_cast<uint32_t>(at))) : at / run; };
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kItems * kThreads) + threadIdx.x; base < items;
+       base += static_cast<int64_t>(gridDim.x) * (kItems * kThreads)) {
+    Word w[kItems];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (left == 0) {
-            s = scales[++r];
-            left = run;
-          }
-          --left;
-          y[e] = static_cast<float>(static_cast<int8_t>(words[2 * j + e / 4] >> (8 * (e % 4)))) * s;
-        }
-        Vec<U, 8>::store(out + at + 8 * j, y);
-      }
-    } else {
-      for (int64_t e = at; e < n; ++e) {
-        const float y[1] = {static_cast<float>(q[e]) * scales[e / run]};
-        Vec<U, 1>::store(out + e, y);
-      }
+    for (int k = 0; k < kItems; ++k) {
+      const int64_t i = base + k * kThreads;
+      w[k] = i < items ? reinterpret_cast<const Word*>(q)[i] : Word{};
     }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int64_t i = base + k * kThreads, at = i * kValues;
+      if (i >= items) break;
+      const int64_t r = run_of(at);
+      const float s = scales[r];
+      float y[kValues], next = s;
+      int left = kValues;  // values until the next scale
+      if (!ONE) {
+        left = static_cast<int>(min((r + 1) * run - at, static_cast<int64_t>(kValues)));
+        if (left < kValues) next = scales[r + 1];
+      }
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(&w[k]);
+#pragma unroll
+      for (int e = 0; e < kValues; ++e) {
+        // the byte plus 128 in the mantissa of 2^23: what the conversion unit gives at a quarter of the rate
+        const float x = __uint_as_float(__byte_perm(words[e / 4] ^ 0x80808080u, 0x4b000000u, 0x7440u | (e % 4))) - 8388736.0f;
+        // runs shorter than an item change more than once in it
+        y[e] = x * (ONE || e < left ? s : run >= kValues || e < left + run ? next : scales[run_of(at + e)]);
+      }
+      Vec<U, kValues>::store(out + at, y);
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x < n % kValues) {
+    const int64_t at = items * kValues + threadIdx.x;
+    const float y[1] = {static_cast<float>(q[at]) * scales[run_of(at)]};
+    Vec<U, 1>::store(out + at, y);
   }
 }
 
 template <class U>
 cudaError_t launch_dequantize_typed(const DequantArgs& a, cudaStream_t stream) {
-  U* out = static_cast<U*>(a.out);
-  const int64_t vectors = (a.n + 15) / 16;
-  auto grid = [](int64_t blocks) { return dim3(static_cast<unsigned>(blocks < (1 << 30) ? blocks : (1 << 30))); };
-  if (a.run % 16 == 0) {
-    PdlLaunch launch(grid((vectors + 2 * kThreads - 1) / (2 * kThreads)), dim3(kThreads), 0, stream);
-    return launch(dequantize_runs<U>, a.q, a.scales, out, vectors, a.run);
-  }
-  PdlLaunch launch(grid((vectors + kThreads - 1) / kThreads), dim3(kThreads), 0, stream);
-  return launch(dequantize_any<U>, a.q, a.scales, out, a.n, a.run);
+  constexpr int kCtaValues = 32 * kThreads;
+  FastDiv run_div{};  // 31-bit numbers, else none
+  if (a.n <= INT32_MAX) run_div.set(static_cast<uint32_t>(a.run));
+  const int64_t ctas = std::min<int64_t>((a.n + kCtaValues - 1) / kCtaValues, 1 << 30);
+  PdlLaunch launch(dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, stream);
+  return launch(a.run % (16 / sizeof(U)) == 0 ? dequantize_items<U, true> : dequantize_items<U, false>, a.q, a.scales,
+                static_cast<U*>(a.out), a.n, a.run, run_div);
 }
 
 }  // namespace
