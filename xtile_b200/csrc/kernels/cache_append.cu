@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
       row += carry;
       at -= carry * items;
     }
-    return Item{row, rope_span<V>(at, rot, a.interleaved)};
+    return Item{row, rope_span<V>(at, rot, dim, a.interleaved)};
   };
   auto fetch = [&](const Item& it, float (&u)[V], float (&v)[V]) {
     const T* from = x + min(it.row, new_rows - 1) * token_stride;
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
   };
   auto fetch_turns = [&](const Item& it, float2 (&cs)[V]) {
     const int64_t pos = min(static_cast<int64_t>(first + min(it.row, new_rows - 1)), a.rope_rows - 1);
-    load_turns<V>(a.rope + pos * (rot / 2) + max(it.span.pair, 0), cs);
+    load_turns<V>(a.rope + pos * (rot / 2), it.span, rot, a.interleaved, cs);
   };
   auto rotate = [&](const Item& it, float (&u)[V], float (&v)[V], const float2 (&cs)[V]) {
     if (it.span.pair >= 0) rope_item<V>(u, v, cs, a.interleaved);

@@ -33,12 +33,12 @@ __global__ void __launch_bounds__(kThreads) rope_heads(const RopeArgs a, int ite
     const int64_t token = static_cast<int64_t>(blockIdx.x) * tokens_per_cta + w / per_token;
     if (token >= a.tokens) return;
     const int group = w % per_token / items;
-    const RopeSpan span = rope_span<V>(w % items, static_cast<int>(a.rot), a.interleaved);
+    const RopeSpan span = rope_span<V>(w % items, static_cast<int>(a.rot), static_cast<int>(a.dim), a.interleaved);
     float2 cs[V];
     if (span.pair >= 0) {
       const int64_t pos = a.positions[token];
       if (pos >= 0 && pos < a.table_rows) {
-        load_turns<V>(a.table + pos * (a.rot / 2) + span.pair, cs);
+        load_turns<V>(a.table + pos * (a.rot / 2), span, static_cast<int>(a.rot), a.interleaved, cs);
       } else {
         if (group == 0) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrRopePosition));
 #pragma unroll
