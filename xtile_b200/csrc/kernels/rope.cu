@@ -1,6 +1,7 @@
 // Rotary positions over heads, and int8 data read back as values.  Both are
 // bound by HBM: each element is read once and written once.  8192 tokens of 32
-// f32 heads of 128 take 45.3 us, 5970 GB/s; 67 million int8 values to bf16 31.3
+// f32 heads of 128 take 41.5 us, 6520 GB/s (bf16
+// 29.3, 4720 GB/s); 67 million int8 values to bf16 31.3
 // us, 6430 GB/s; a decode step's 16 tokens 1.9 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -22,9 +23,14 @@ constexpr int kThreads = 256;
 
 // A thread turns the same item (two vectors of V elements) of HEADS heads of
 // one token, so that it reads the table's cosines and sines once for them all.
-// Both vectors are read before either is written: y may be x.
+// Both vectors are read before either is written: y may be x.  The heads come
+// before the table's row, whose address waits for the position, and stay packed
+// (unpacked at once, 8192 tokens of 32 bf16 heads took 37.0 us, 29.3 so).
 template <class T, class U, int V, int HEADS>
 __global__ void __launch_bounds__(kThreads) rope_heads(const RopeArgs a, int items, int groups, int tokens_per_cta) {
+  // as they lie in memory until a head's turn comes
+  using Word = typename std::conditional<V * sizeof(T) == 16, uint4,
+                                         typename std::conditional<V * sizeof(T) == 8, uint2, T>::type>::type;
   griddep_launch_dependents();
   griddep_wait();
   const int per_token = items * groups;
@@ -34,6 +40,16 @@ __global__ void __launch_bounds__(kThreads) rope_heads(const RopeArgs a, int ite
     if (token >= a.tokens) return;
     const int group = w % per_token / items;
     const RopeSpan span = rope_span<V>(w % items, static_cast<int>(a.rot), static_cast<int>(a.dim), a.interleaved);
+    const T* x = static_cast<const T*>(a.x) + token * a.x_token;
+    U* y = static_cast<U*>(a.y) + token * a.y_token;
+    Word u[HEADS], v[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+      const int64_t head = static_cast<int64_t>(group) * HEADS + i;
+      if (head >= a.heads) continue;
+      u[i] = *reinterpret_cast<const Word*>(x + head * a.x_head + span.first);
+      v[i] = *reinterpret_cast<const Word*>(x + head * a.x_head + span.second);
+    }
     float2 cs[V];
     if (span.pair >= 0) {
       const int64_t pos = a.positions[token];
@@ -49,23 +65,16 @@ __global__ void __launch_bounds__(kThreads) rope_heads(const RopeArgs a, int ite
         for (int j = 0; j < V; ++j) cs[j].y = -cs[j].y;
       }
     }
-    const T* x = static_cast<const T*>(a.x) + token * a.x_token;
-    U* y = static_cast<U*>(a.y) + token * a.y_token;
-    float u[HEADS][V], v[HEADS][V];
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
       const int64_t head = static_cast<int64_t>(group) * HEADS + i;
       if (head >= a.heads) continue;
-      Vec<T, V>::load(x + head * a.x_head + span.first, u[i]);
-      Vec<T, V>::load(x + head * a.x_head + span.second, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
-      const int64_t head = static_cast<int64_t>(group) * HEADS + i;
-      if (head >= a.heads) continue;
-      if (span.pair >= 0) rope_item<V>(u[i], v[i], cs, a.interleaved);
-      Vec<U, V>::store(y + head * a.y_head + span.first, u[i]);
-      Vec<U, V>::store(y + head * a.y_head + span.second, v[i]);
+      float p[V], q[V];
+      Vec<T, V>::load(reinterpret_cast<const T*>(&u[i]), p);
+      Vec<T, V>::load(reinterpret_cast<const T*>(&v[i]), q);
+      if (span.pair >= 0) rope_item<V>(p, q, cs, a.interleaved);
+      Vec<U, V>::store(y + head * a.y_head + span.first, p);
+      Vec<U, V>::store(y + head * a.y_head + span.second, q);
     }
   }
 }
