@@ -114,6 +114,11 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
   return a / b;
 }
 
+// Units that each worker takes.
+__device__ __forceinline__ int64_t units_each(const AttendDev& p, int64_t total) {
+  return max(divide(total + p.workers - 1, p.workers), static_cast<int64_t>(p.least));
+}
+
 __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   } else {
     int64_t unused;
     const int64_t total = count_units<kRows>(p, 0, &unused);
-    const int64_t per = divide(total + p.workers - 1, p.workers);
+    const int64_t per = units_each(p, total);
     worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
     const int64_t begin = worker * per;
     if (begin >= total) return;
@@ -885,7 +890,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
   if (mine_to_join) {
     int64_t front;
     const int64_t total = count_units<ROWS>(p, b, &front);
-    const int64_t per = divide(total + p.workers - 1, p.workers);
+    const int64_t per = units_each(p, total);
     const int64_t u0 = front + (static_cast<int64_t>(head) * seg.row_tiles + packed / ROWS) * tiles;
     first = divide(u0, per), last = divide(u0 + tiles - 1, per);
   }
@@ -1003,9 +1008,13 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   const int sms = sm_count(), dim = p.a.cache.dim, resident = sms * S::kCtas;
   static std::atomic<bool> allowed[3][kMaxDevices];
   const int64_t longest = longest_seen(p, kTile), tiles = (longest + kTile - 1) / kTile, segments = segments_of(p, S::kRows);
-  // A cluster a segment where the whole is small: 1.3 units a nanosecond make
-  // 16384 of them 12 us, of which an uneven share loses less than the join.
-  if (segments * tiles <= 16384) {
+  // A cluster a segment where the whole is small (1.3 units a nanosecond make
+  // 16384 of them 12 us, of which an uneven share loses less than the join) and no
+  // warp of a cluster has many units beyond an even share, at 0.7 us each (1.1 over
+  // 128 dims): one sequence of 4000 tokens and two kv heads takes 13.0 us in
+  // clusters and 14.4 shared out, of 8000 19.7 and 16.2, of 64000 112 and 34.
+  const int64_t even = segments * tiles / (static_cast<int64_t>(resident) * S::kWarps);
+  if (segments * tiles <= 16384 && tiles <= ((DP <= 128 ? 12 : 5) + even) * 8 * S::kWarps) {
     if (bytes) {
       *bytes = 0;
       return cudaSuccess;
@@ -1037,6 +1046,13 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
     return launch(warps, p.cluster)(kernel, p, CUtensorMap{}, CUtensorMap{});
   }
   p.workers = static_cast<int64_t>(resident) * S::kWarps;
+  const int64_t rows = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
+  // a row's partials are spread over eight warps where the rows alone would not fill the GPU
+  const int join_warps = rows <= 4 * sms ? 8 : 1;
+  // A worker's unit takes 0.7 us and a partial result 0.3 us of its row's warps in
+  // the join: few segments get as many units a worker as make the sum least (64000
+  // tokens of two kv heads: 55 us with a worker for each four units, 34 so).
+  p.least = std::max(1, static_cast<int>(std::sqrt(0.43f * tiles / join_warps)));
   if (bytes) {
     *bytes = static_cast<size_t>(p.workers) * 2 * S::kRows * (dim + 2) * sizeof(float);
     return cudaSuccess;
@@ -1058,9 +1074,7 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   PdlLaunch launch(dim3(static_cast<unsigned>(resident)), dim3(S::kWarps * 32), S::kBytes, stream);
   e = launch(kernel, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
-  const int64_t rows = static_cast<int64_t>(p.a.batch.tokens) * p.a.q_heads;
-  // a row's partials are spread over eight warps where the rows alone would not fill the GPU
-  if (rows <= 4 * sms) {
+  if (join_warps == 8) {
     PdlLaunch join(dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream);
     return join(attend_join<T, DP, S::kRows, 8>, p);
   }

@@ -24,6 +24,7 @@ struct AttendDev {
   float* part;        // [workers][2][rows][dim] partial outputs
   float2* part_ml;    // [workers][2][rows] (reference, sum)
   int64_t workers;
+  int least;          // units a worker takes at least
   int cluster;        // CTAs of a segment, which then has a cluster
 };
 
