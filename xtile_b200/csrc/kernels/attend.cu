@@ -1051,8 +1051,9 @@ cudaError_t launch_shape(AttendDev& p, cudaStream_t stream, size_t* bytes) {
   const int join_warps = rows <= 4 * sms ? 8 : 1;
   // A worker's unit takes 0.7 us and a partial result 0.3 us of its row's warps in
   // the join: few segments get as many units a worker as make the sum least (64000
-  // tokens of two kv heads: 55 us with a worker for each four units, 34 so).
-  p.least = std::max(1, static_cast<int>(std::sqrt(0.43f * tiles / join_warps)));
+  // tokens of two kv heads: 55 us with a worker for each four units, 34 so).  No more
+  // than 16: the sequences may be shorter than their table allows.
+  p.least = std::clamp(static_cast<int>(std::sqrt(0.43f * tiles / join_warps)), 1, 16);
   if (bytes) {
     *bytes = static_cast<size_t>(p.workers) * 2 * S::kRows * (dim + 2) * sizeof(float);
     return cudaSuccess;

@@ -1,8 +1,7 @@
 // Rotary positions over heads, and int8 data read back as values.  Both are
 // bound by HBM: each element is read once and written once.  8192 tokens of 32
-// f32 heads of 128 take 41.5 us, 6520 GB/s (bf16
-// 29.3, 4720 GB/s); 67 million int8 values to bf16 31.3
-// us, 6430 GB/s; a decode step's 16 tokens 1.9 us.
+// f32 heads of 128 take 41.5 us, 6520 GB/s (bf16 29.3, 4720 GB/s); 67 million
+// int8 values to bf16 31.3 us, 6430 GB/s; a decode step's 16 tokens 2.0 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
