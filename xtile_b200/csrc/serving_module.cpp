@@ -133,11 +133,13 @@ struct Launch {
   }
   void* handle() const { return on.stream(); }
 
-  // Scratch memory of this call, from the allocator's pool of its stream.
-  at::Tensor scratch(size_t bytes, at::Device device) const {
+  // A result or scratch memory of this call, from the allocator's pool of its
+  // stream: a block of another stream's pool may still be read there, and would
+  // return to that pool while this stream writes it.
+  at::Tensor empty(at::IntArrayRef shape, const at::TensorOptions& options) const {
     c10::cuda::OptionalCUDAStreamGuard allocate;
     if (given) allocate.reset_stream(on);
-    return at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(device));
+    return at::empty(shape, options);
   }
 
  private:
@@ -195,12 +197,13 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       raise(PyExc_TypeError, "weight must be a float32 or bfloat16 tensor");
     like(weight, "weight", {cols}, weight.scalar_type(), device);
     const std::optional<at::ScalarType> dtype = dtype_of(args[7]);
+    const Launch launch(device, args[8]);
     at::Tensor fresh, fresh_scales;
     const at::Tensor* out = maybe(args[2], "out");
     if (!out) {
       if (elem_of(dtype.value_or(x.scalar_type())) == XT_ELEM_OTHER)
         raise(PyExc_TypeError, "out must be float32, bfloat16 or int8, got " + text(*dtype));
-      fresh = at::empty({rows, cols}, x.options().dtype(dtype.value_or(x.scalar_type())));
+      fresh = launch.empty({rows, cols}, x.options().dtype(dtype.value_or(x.scalar_type())));
       out = &fresh;
     } else {
       if (elem_of(out->scalar_type()) == XT_ELEM_OTHER || (dtype && *dtype != out->scalar_type()))
@@ -212,7 +215,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* scales = maybe(args[5], "scales");
     if (y_elem == XT_ELEM_I8) {
       if (!scales) {
-        fresh_scales = at::empty({rows}, x.options().dtype(at::kFloat));
+        fresh_scales = launch.empty({rows}, x.options().dtype(at::kFloat));
         scales = &fresh_scales;
       } else {
         like(*scales, "scales", {rows}, at::kFloat, device);
@@ -227,7 +230,6 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       like(*sum, "residual_out", x.sizes(), x.scalar_type(), device);
       written(*sum, "residual_out");
     }
-    const Launch launch(device, args[8]);
     const xt_rms_norm_args a{x.data_ptr(),
                              residual ? residual->data_ptr() : nullptr,
                              weight.data_ptr(),
@@ -288,17 +290,17 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
       raise(PyExc_ValueError, "heads of " + std::to_string(x.size(2)) + " elements cannot turn " + std::to_string(rot) + " of them");
     const at::Tensor& positions = tensor(args[1], "positions");
     like(positions, "positions", {x.size(0)}, at::kInt, device);
+    const Launch launch(device, args[6]);
     at::Tensor fresh;
     const at::Tensor* out = maybe(args[4], "out");
     if (!out) {
-      fresh = at::empty(x.sizes(), x.options());
+      fresh = launch.empty(x.sizes(), x.options());
       out = &fresh;
     } else {
       const bool narrower = elem == XT_ELEM_F32 && out->scalar_type() == at::kBFloat16;
       like(*out, "out", x.sizes(), narrower ? at::kBFloat16 : x.scalar_type(), device);
       written(*out, "out");
     }
-    const Launch launch(device, args[6]);
     const xt_rope_args a{x.data_ptr(), out->data_ptr(), static_cast<const int32_t*>(positions.data_ptr()),
                          static_cast<const float*>(table.data_ptr()), x.size(0), x.size(1), x.size(2), rot,
                          table.size(0), x.stride(0), x.stride(1), out->stride(0), out->stride(1), elem,
@@ -398,16 +400,16 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       raise(PyExc_ValueError, "q " + text(q.sizes()) + " does not fit a cache of " + std::to_string(cache.heads) +
                                   " heads of " + std::to_string(cache.dim));
     const xt_batch batch = batch_view(args + 5, q.size(0), device);
+    const Launch launch(device, args[13]);
     at::Tensor fresh, scratch;
     const at::Tensor* out = maybe(args[8], "out");
     if (!out) {
-      fresh = at::empty(q.sizes(), q.options());
+      fresh = launch.empty(q.sizes(), q.options());
       out = &fresh;
     } else {
       like(*out, "out", q.sizes(), q.scalar_type(), device);
       written(*out, "out");
     }
-    const Launch launch(device, args[13]);
     xt_cache_attention_args a{cache, batch, q.data_ptr(), out->data_ptr(), q.stride(0), q.stride(1), out->stride(0),
                               out->stride(1), static_cast<int>(q.size(1)),
                               args[9] == Py_None ? 0 : small(args[9], "max_new"), small(args[11], "window"),
@@ -415,7 +417,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
                               static_cast<float>(number(args[12])), elem, nullptr, 0};
     check(xt_cache_attention_workspace(&a, &a.workspace_bytes), "cache_attention");
     if (a.workspace_bytes) {
-      scratch = launch.scratch(a.workspace_bytes, device);
+      scratch = launch.empty({static_cast<int64_t>(a.workspace_bytes)}, q.options().dtype(at::kByte));
       a.workspace = scratch.data_ptr();
     }
     check(xt_cache_attention(&a, launch.handle()), "cache_attention");
@@ -438,6 +440,7 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if ((count && !runs) || (runs && count % runs))
       raise(PyExc_ValueError, std::to_string(count) + " elements do not divide into " + std::to_string(runs) + " equal runs");
     const std::optional<at::ScalarType> dtype = dtype_of(args[3]);
+    const Launch launch(device, args[4]);
     at::Tensor fresh;
     const at::Tensor* out = maybe(args[2], "out");
     const at::ScalarType type = dtype ? *dtype : out ? out->scalar_type() : at::kBFloat16;
@@ -445,19 +448,17 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (elem != XT_ELEM_F32 && elem != XT_ELEM_BF16)
       raise(PyExc_TypeError, "out must be float32 or bfloat16, got " + text(type));
     if (!out) {
-      fresh = at::empty(q.sizes(), q.options().dtype(type));
+      fresh = launch.empty(q.sizes(), q.options().dtype(type));
       out = &fresh;
     } else {
       like(*out, "out", q.sizes(), type, device);
     }
     if (!q.is_contiguous() || !scales.is_contiguous() || !out->is_contiguous())
       raise(PyExc_ValueError, "q, scales and out must be contiguous");
-    if (count) {
-      const Launch launch(device, args[4]);
+    if (count)
       check(xt_dequantize(static_cast<const int8_t*>(q.data_ptr()), static_cast<const float*>(scales.data_ptr()),
                           out->data_ptr(), count, count / runs, elem, launch.handle()),
             "dequantize");
-    }
     return wrap_or(args[2], *out);
   });
 }

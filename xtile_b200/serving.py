@@ -12,6 +12,11 @@ an entry outside the arrays is not followed, and ``device_error()`` reports it
 (0x301 rope, 0x302 append, 0x303 attention; 0x304, 0x305 and 0x307 are bounded
 waits of the attention kernels that ran out).
 
+With ``stream`` given, that stream owns what the call allocates, as under
+``torch.cuda.stream(stream)``: another stream waits for it before it reads the
+result, and calls ``record_stream`` on a result that is dropped while its own
+reads are under way.  The same holds for the call's inputs on ``stream``.
+
 A ragged batch is described by three int32 tensors: ``starts`` [seqs + 1],
 ``lengths`` [seqs] and ``pages`` [seqs, width].  Sequence ``b`` has
 ``lengths[b]`` tokens; the last ``starts[b + 1] - starts[b]`` of them are new
