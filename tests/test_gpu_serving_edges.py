@@ -72,3 +72,58 @@ def test_a_result_takes_no_memory_that_its_stream_does_not_own():
         call(side)
         torch.cuda.synchronize()
         assert (seen == 3).all(), name
+
+
+# --------------------------------------------------------------- wrong tables
+
+def starts_of(new, first=0):
+    s = [first]
+    for n in new:
+        s.append(s[-1] + n)
+    return s
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+# new tokens of three sequences: one slot a token, and one a block
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 70]])
+@pytest.mark.parametrize("page, block", [(16, 16), (48, 8)])
+def test_append_reports_every_wrong_start(new, page, block):
+    a, b, c = new
+    batch = Batch(new, [n + 20 for n in new], page, seed=1)
+    lengths, table = batch.args[1:]
+    k = normal(generator(1), a + b + c, 2, 64)
+    start = filled_cache(generator(2), batch.pages_held, 2, 64, page, block)
+
+    def append(starts, lengths=lengths):
+        cache = xt.KVCache(start.k.clone(), start.v.clone(), start.k_scale.clone(), start.v_scale.clone())
+        xt.cache_append(cache, k, k, ints(starts), lengths, table)
+        return cache
+
+    def pages_of(cache, b):
+        held = torch.tensor(batch.table[b], device="cuda")
+        return [t[held] for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+
+    def same(x, y, b):
+        return all(torch.equal(s, t) for s, t in zip(pages_of(x, b), pages_of(y, b)))
+
+    good = append(starts_of(new))
+    assert xt.device_error() == 0 and not any(same(good, start, b) for b in range(3))
+    # starts that fall: a sequence that is wrong by itself is not stored, any other one may be missed
+    for wrong in ([0, a + b, a, a + b + c], [0, a, -1, a + b + c], [a, 0, a + b, a + b + c], [0, a, a + b, a - 1]):
+        cache = append(wrong)
+        assert xt.device_error() == 0x302, wrong
+        assert all(same(cache, start, b) for b in range(3) if not 0 <= wrong[b] <= wrong[b + 1]), wrong
+    # a negative start: the others' tokens are stored
+    for wrong in ([-1, a, a + b, a + b + c], [-1000, a, a + b, a + b + c]):
+        cache = append(wrong)
+        assert xt.device_error() == 0x302, wrong
+        assert same(cache, start, 0) and same(cache, good, 1) and same(cache, good, 2), wrong
+    # sequences without a token, or behind all rows
+    for wrong, n in (([-5, -5, -2, 0], lengths), ([1000, 1000, 1001, 1002], lengths), ([0, 0, 0, 0], ints([5, -1, 5])),
+                     ([0, 0, 0, 0], ints([5, 1 << 20, 5]))):
+        cache = append(wrong, n)
+        assert xt.device_error() == 0x302, wrong
+        assert all(same(cache, start, b) for b in range(3)), wrong

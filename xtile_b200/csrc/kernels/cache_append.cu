@@ -54,6 +54,16 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
   const AppendArgs& a = p.a;
   const BatchView& bt = a.batch;
   const int block = a.cache.block, page = a.cache.page, dim = a.cache.dim, heads = a.cache.heads;
+  if (blockIdx.x == 0) {
+    // Every sequence is looked at once: where starts fall the search may miss some,
+    // whose tokens are not stored then, and a wrong one without a token has no slot.
+    bool wrong = false;
+    for (int i = threadIdx.x; i < bt.seqs; i += kThreads) {
+      const Sequence t = load_sequence(bt, page, i);
+      wrong |= !t.ok || t.length < t.count;
+    }
+    if (wrong) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrAppendTable));
+  }
   const int index = kCta ? blockIdx.x : blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (index >= p.warps) return;
   const int slot = p.slot_div.quot(index);
@@ -67,13 +77,10 @@ __global__ void __launch_bounds__(kThreads) cache_append_blocks(const __grid_con
 
   const int b = p.by_token
                     ? last_at_most(bt.seqs, slot, [&](int i) { return static_cast<int64_t>(bt.starts[i]); })
-                    : last_at_most(bt.seqs, slot, [&](int i) { return p.block_div.quot(bt.starts[i]) + 2 * static_cast<int64_t>(i); });
+                    : last_at_most(bt.seqs, slot, [&](int i) { return p.block_div.quot(max(bt.starts[i], 0)) + 2 * static_cast<int64_t>(i); });
   const Sequence s = load_sequence(bt, page, b);
   const int begin = s.length - s.count;
-  if (!s.ok || begin < 0) {
-    if (lane == 0) atomicCAS(a.error_word, 0u, static_cast<uint32_t>(kErrAppendTable));
-    return;
-  }
+  if (!s.ok || begin < 0) return;  // recorded by the first CTA
   int lo;
   if (p.by_token) {
     const int i = slot - s.first, at = begin + i;
