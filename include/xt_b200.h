@@ -197,8 +197,10 @@ int xt_matmul_launch_noalloc(const xt_module* module, const char* func, void* co
  * the host, is asynchronous on ``stream``, and reads and writes each array
  * once.  What only the device knows (positions, lengths, page tables) is
  * checked there: an entry that names something outside the arrays is not
- * followed, its results are NaN or left unwritten, and xt_device_error gives
- * 0x301 (rope position), 0x302 (append) or 0x303 (attention).  The attention
+ * followed, its results are NaN (append: not stored), and xt_device_error gives
+ * 0x301 (rope position), 0x302 (append) or 0x303 (attention).  Where ``starts``
+ * fall, append may miss other sequences too and every row of an attention is
+ * NaN.  The attention
  * kernels' waits for their own copies and products are bounded like those of
  * xt_launch; one that runs out gives 0x304, 0x305 or 0x307. */
 

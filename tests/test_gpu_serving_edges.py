@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import xtile as xt
-from tests.test_gpu_serving import Batch, filled_cache, generator, normal
+from tests.test_gpu_serving import Batch, allowed, attend_64, filled_cache, generator, normal, widened, within
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +127,48 @@ def test_append_reports_every_wrong_start(new, page, block):
         cache = append(wrong, n)
         assert xt.device_error() == 0x302, wrong
         assert all(same(cache, start, b) for b in range(3)), wrong
+
+
+# the forms of the attention: clusters, runs of units over the GPU, whole prompts, prompts in clusters
+FORMS = {
+    "clusters": (([20, 3, 30], [70, 33, 60]), 64, 8, None),
+    "rows": (([20, 3, 30], [70, 33, 60]), 64, 8, "rows"),
+    "boxes": (([20, 3, 30], [70, 33, 60]), 64, 8, "boxes"),
+    "prompts": (([2000, 500, 900], [2000, 700, 1500]), 64, 8, None),
+    "prompt clusters": (([70, 3, 90], [4000, 70, 2500]), 128, 4, None),
+}
+
+
+def form_case(form):
+    (new, total), dim, group, wide = FORMS[form]
+    heads = 8 if form == "prompt clusters" else 2
+    dtype = torch.bfloat16 if "prompt" in form else torch.float32
+    batch = Batch(new, total, 64, seed=3)
+    cache = filled_cache(generator(5), batch.pages_held, heads, dim, 64, 16)
+    if wide:
+        widened(batch, cache, wide)
+    return new, batch, cache, normal(generator(6), batch.tokens, heads * group, dim, std=1.5, dtype=dtype)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_reports_every_wrong_start(form):
+    new, batch, cache, q = form_case(form)
+    (a, b, c), most = new, max(new)
+    lengths, table = batch.args[1:]
+    attend = lambda starts, n=lengths: xt.cache_attention(cache, q, ints(starts), n, table, max_new=most)  # noqa: E731
+    want, *rest = attend_64(cache, batch, q, cache.dim ** -0.5, 0, 0.0)
+    off = allowed(want, *rest, max(batch.total), q.dtype)
+    within(attend(starts_of(new)), want, off)
+    for wrong in ([0, a + b, a, a + b + c], [0, a, -1, a + b + c], [a, 0, a + b, a + b + c], [0, a, a + b, a - 1]):
+        y = attend(wrong)
+        assert xt.device_error() == 0x303, wrong
+        assert y.isnan().all(), wrong  # starts that fall: no row is sure
+    for wrong in ([-1, a, a + b, a + b + c], [-1000, a, a + b, a + b + c]):
+        y = attend(wrong)
+        assert xt.device_error() == 0x303, wrong
+        assert y[:a].isnan().all(), wrong
+        within(y[a:], want[a:], off[a:])
+    for wrong, n in (([-5, -5, -2, 0], lengths), ([100000, 100000, 100001, 100002], lengths), ([0, 0, 0, 0], ints([5, -1, 5])),
+                     ([0, 0, 0, 0], ints([5, 1 << 30, 5]))):
+        attend(wrong, n)
+        assert xt.device_error() == 0x303, wrong

@@ -96,9 +96,9 @@ struct Segments {
 };
 
 template <int ROWS>
-__device__ __forceinline__ Segments load_segments(const AttendDev& p, int b) {
+__device__ __forceinline__ Segments segments_of_sequence(const AttendDev& p, const Sequence& seq) {
   Segments g;
-  g.seq = load_sequence(p.a.batch, p.a.cache.page, b);
+  g.seq = seq;
   if (!g.seq.ok) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
   g.row_tiles = static_cast<int>((static_cast<int64_t>(g.seq.count) * p.group + ROWS - 1) / ROWS);
   const int64_t first_seen = p.a.window > 0 ? static_cast<int64_t>(g.seq.length) - g.seq.count - p.a.window + 1 : 0;
@@ -106,6 +106,11 @@ __device__ __forceinline__ Segments load_segments(const AttendDev& p, int b) {
   g.hi = (g.seq.length + kTile - 1) / kTile;
   if (g.lo > g.hi) g.lo = g.hi;
   return g;
+}
+
+template <int ROWS>
+__device__ __forceinline__ Segments load_segments(const AttendDev& p, int b) {
+  return segments_of_sequence<ROWS>(p, load_sequence(p.a.batch, p.a.cache.page, b));
 }
 
 // a / b of positive values; 64-bit division took a third of a microsecond.
@@ -125,17 +130,20 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
   return v;
 }
 
-// Units of all sequences, and of those before ``b``.  A whole warp calls.
+// Units of all sequences, and of those before ``b``; -1 where starts fall, and no
+// sequence is sure of its rows.  A whole warp calls.
 template <int ROWS>
 __device__ __forceinline__ int64_t count_units(const AttendDev& p, int b, int64_t* before) {
   int64_t total = 0, front = 0;
+  bool fall = false;
   for (int i = threadIdx.x & 31; i < p.a.batch.seqs; i += 32) {
     const int64_t u = load_segments<ROWS>(p, i).units(p.a.cache.heads);
     total += u;
     if (i < b) front += u;
+    fall |= p.a.batch.starts[i + 1] < p.a.batch.starts[i];
   }
   *before = warp_sum64(front);
-  return warp_sum64(total);
+  return __any_sync(0xffffffffu, fall) ? -1 : warp_sum64(total);
 }
 
 // A place in the line of units.
@@ -288,12 +296,17 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   int left;  // units to do
   if constexpr (kCluster) {
     const int rank = blockIdx.x % p.cluster, index = blockIdx.x / p.cluster, slot = index / cache.heads;
-    auto base = [&](int i) { return first_slot(p.a.batch.starts[i], i, p.group, kRows); };
-    at.b = last_at_most(p.a.batch.seqs, slot, base);
+    auto base = [&](int start, int i) { return first_slot(start, i, p.group, kRows); };
+    const Found found = find_sequence(p.a.batch, cache.page, slot, base);
+    at.b = found.b;
     at.head = index - slot * cache.heads;
-    at.seg = load_segments<kRows>(p, at.b);
-    const int64_t row_tile = slot - base(at.b);
+    at.seg = segments_of_sequence<kRows>(p, found.seq);
+    const int64_t row_tile = slot - base(found.start, found.b);
     // the cluster's CTAs return together
+    if (found.fall) {
+      refuse_batch<T>(p);
+      return;
+    }
     if (!at.seg.seq.ok) {
       if (row_tile == 0 && rank == 0) refuse_sequence<T>(p, at.b, at.head, threadIdx.x, blockDim.x);
       return;
@@ -885,11 +898,11 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
   const int i = token - seg.seq.first, tiles = seg.hi - seg.lo;
   const int head = p.group_div.quot(q_head);
   const int packed = i * p.group + q_head - head * p.group;
-  const bool mine_to_join = seg.seq.ok && i >= 0 && i < seg.seq.count && tiles > 0;
-  int64_t first = 0, last = 0;
+  int64_t first = 0, last = 0, front;
+  const int64_t total = count_units<ROWS>(p, b, &front);
+  const bool sure = total >= 0;
+  const bool mine_to_join = sure && seg.seq.ok && i >= 0 && i < seg.seq.count && tiles > 0;
   if (mine_to_join) {
-    int64_t front;
-    const int64_t total = count_units<ROWS>(p, b, &front);
     const int64_t per = units_each(p, total);
     const int64_t u0 = front + (static_cast<int64_t>(head) * seg.row_tiles + packed / ROWS) * tiles;
     first = divide(u0, per), last = divide(u0 + tiles - 1, per);
@@ -897,9 +910,9 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) attend_join(con
   griddep_wait();
   T* out = static_cast<T*>(p.a.out) + static_cast<int64_t>(token) * p.a.out_token + static_cast<int64_t>(q_head) * p.a.out_head;
   if (!mine_to_join) {
-    if (seg.seq.ok && (i < 0 || i >= seg.seq.count)) return;  // a row of no sequence
+    if (sure && seg.seq.ok && (i < 0 || i >= seg.seq.count)) return;  // a row of no sequence
     // no token at all: 0; a wrong table: recorded, and NaN
-    const float v[1] = {seg.seq.ok ? 0.0f : __int_as_float(0x7fc00000)};
+    const float v[1] = {sure && seg.seq.ok ? 0.0f : __int_as_float(0x7fc00000)};
     for (int d = lane; d < p.a.cache.dim; d += 32) Vec<T, 1>::store(out + d, v);
     return;
   }

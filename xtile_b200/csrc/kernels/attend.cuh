@@ -114,8 +114,12 @@ int clusters_at_once(K kernel, PdlLaunch launch, std::atomic<int> (&known)[kMaxD
 }
 
 // Segments without a scan: sequence b's row tiles of ROWS packed rows stand at
-// slots starts[b] * group / ROWS + b on, which leaves room for all of them.
-__host__ __device__ inline int64_t first_slot(int64_t start, int b, int group, int rows) { return start * group / rows + b; }
+// slots starts[b] * group / ROWS + b on, which leaves room for all of them
+// where starts never fall (0 for a start that is negative, whose sequence is
+// refused).
+__host__ __device__ inline int64_t first_slot(int64_t start, int b, int group, int rows) {
+  return (start > 0 ? start : 0) * group / rows + b;
+}
 
 // New tokens of a sequence, as far as the caller knows; else their mean.
 inline int new_tokens(const AttendDev& p) {
@@ -137,10 +141,9 @@ inline int64_t segments_of(const AttendDev& p, int rows) {
   return static_cast<int64_t>(p.a.batch.seqs) * p.a.cache.heads * tiles;
 }
 
-// A sequence whose table is wrong: recorded, and its rows of a kv head are NaN.
+// A sequence whose table is wrong: its rows of a kv head are NaN.
 template <class T>
-__device__ __forceinline__ void refuse_sequence(const AttendDev& p, int b, int head, int thread, int threads) {
-  if (thread == 0) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
+__device__ __noinline__ void refuse_sequence(const AttendDev& p, int b, int head, int thread, int threads) {
   const int dim = p.a.cache.dim;
   const int64_t first = max(p.a.batch.starts[b], 0), end = min(p.a.batch.starts[b + 1], p.a.batch.tokens);
   const int64_t each = static_cast<int64_t>(p.group) * dim;
@@ -148,6 +151,18 @@ __device__ __forceinline__ void refuse_sequence(const AttendDev& p, int b, int h
     const int64_t token = first + i / each, h = head * p.group + i % each / dim;
     static_cast<T*>(p.a.out)[token * p.a.out_token + h * p.a.out_head + i % dim] = static_cast<T>(__int_as_float(0x7fc00000));
   }
+}
+
+// Starts that fall: recorded, and every row of the batch is NaN.  Each CTA of the
+// grid has a share of them.
+template <class T>
+__device__ __noinline__ void refuse_batch(const AttendDev& p) {
+  if (threadIdx.x == 0) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
+  const int dim = p.a.cache.dim;
+  const int64_t each = static_cast<int64_t>(p.a.q_heads) * dim;
+  for (int64_t token = blockIdx.x; token < p.a.batch.tokens; token += gridDim.x)
+    for (int64_t i = threadIdx.x; i < each; i += blockDim.x)
+      static_cast<T*>(p.a.out)[token * p.a.out_token + i / dim * p.a.out_head + i % dim] = static_cast<T>(__int_as_float(0x7fc00000));
 }
 
 // The tcgen05 kernel for many query rows (attend_prompt.cu): bf16, dim <= 128.

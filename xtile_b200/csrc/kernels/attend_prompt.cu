@@ -194,12 +194,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
     const int index_of = static_cast<int>(blockIdx.x) / p.cluster;
     const int slot = slots - 1 - index_of / cache.heads;
     work.head = index_of % cache.heads;
-    auto base = [&](int i) { return first_slot(p.a.batch.starts[i], i, p.group, kRows); };
-    const int b = last_at_most(p.a.batch.seqs, slot, base);
-    work.seq = load_sequence(p.a.batch, cache.page, b);
+    auto base = [&](int start, int i) { return first_slot(start, i, p.group, kRows); };
+    const Found found = find_sequence(p.a.batch, cache.page, slot, base);
+    const int b = found.b;
+    work.seq = found.seq;
     work.table = p.a.batch.table + b * p.a.batch.table_stride;
-    const int64_t index = slot - base(b);
+    const int64_t index = slot - base(found.start, b);
+    if (found.fall) {
+      refuse_batch<__nv_bfloat16>(p);
+      return;
+    }
     if (!work.seq.ok) {
+      if (threadIdx.x == 0) atomicCAS(p.a.error_word, 0u, static_cast<uint32_t>(kErrAttendTable));
       if (index == 0) refuse_sequence<__nv_bfloat16>(p, b, work.head, threadIdx.x, kThreads);
       return;
     }

@@ -9,7 +9,8 @@
 raises ``TypeError`` (types) or ``ValueError`` (shapes, devices, layouts)
 before anything runs.  Positions, lengths and page tables live on the device:
 an entry outside the arrays is not followed, and ``device_error()`` reports it
-(0x301 rope, 0x302 append, 0x303 attention; 0x304, 0x305 and 0x307 are bounded
+(0x301 rope, 0x302 append, 0x303 attention; where ``starts`` fall, append may
+miss other sequences too, and every row of an attention is NaN; 0x304, 0x305 and 0x307 are bounded
 waits of the attention kernels that ran out).
 
 With ``stream`` given, that stream owns what the call allocates, as under
