@@ -172,3 +172,49 @@ def test_attention_reports_every_wrong_start(form):
                      ([0, 0, 0, 0], ints([5, 1 << 30, 5]))):
         attend(wrong, n)
         assert xt.device_error() == 0x303, wrong
+
+
+# --------------------------------------------------------- waits that run out
+
+def rows_good_or_nan(y, good):
+    """Every head of a token is what it should be, or NaN throughout.  How many are NaN."""
+    lost = y.isnan().all(-1)
+    assert torch.equal(y[~lost], good[~lost])
+    return int(lost.sum())
+
+
+WAITS = {
+    # new, total, q heads, kv heads, dim, type, form
+    "clusters": ([1] * 30, [100 + 60 * i for i in range(30)], 16, 4, 128, torch.bfloat16, None),
+    "one warp a segment": ([1] * 600, [96] * 600, 4, 4, 128, torch.bfloat16, None),
+    "rows": ([1] * 60, [2000 + 40 * i for i in range(60)], 16, 4, 128, torch.bfloat16, "rows"),
+    "boxes": ([1, 3] * 16, [4000 + 100 * i for i in range(32)], 32, 8, 128, torch.bfloat16, "boxes"),
+    "many segments a warp": ([1] * 1200, [20 + i % 50 for i in range(1200)], 8, 8, 128, torch.bfloat16, "boxes"),
+}
+
+
+@pytest.mark.parametrize("case", WAITS)
+def test_attention_waits_run_out(case):
+    """A wait limit of 1 ns: warps that find a tile not yet there give up, their rows are NaN, and the next call is
+    whole again.  No copy is lost or held back: every one lands before its warp ends."""
+    new, total, q_heads, heads, dim, dtype, form = WAITS[case]
+    batch = Batch(new, total, 64, seed=3)
+    cache = filled_cache(generator(5), batch.pages_held, heads, dim, 64, 16)
+    if form:
+        widened(batch, cache, form)
+    q = normal(generator(6), batch.tokens, q_heads, dim, std=1.5, dtype=dtype)
+    good = xt.cache_attention(cache, q, *batch.args, max_new=max(new))
+    assert good.isfinite().all() and xt.device_error() == 0
+    flush = torch.empty(1 << 28, dtype=torch.int8, device="cuda")
+    for _ in range(100):
+        flush.zero_()  # the tiles come from far, the queries do not
+        y = torch.zeros_like(q) + q * 0
+        with xt.wait_limit(1):
+            xt.cache_attention(cache, q, *batch.args, y, max_new=max(new))
+        lost = rows_good_or_nan(y, good)
+        code = xt.device_error()
+        assert code == (0x307 if lost else 0)
+        if lost:
+            break
+    assert lost, "no wait ran out"
+    assert torch.equal(xt.cache_attention(cache, q, *batch.args, max_new=max(new)), good)

@@ -348,6 +348,9 @@ std::shared_ptr<Plan> module_plan(const xt_module* module, const char* func) {
 // Records ``msg`` as the calling thread's last error and returns ``code``.
 int record_error(int code, const std::string& msg) { return fail(code, msg); }
 
+// The calling thread's limit on waits, in SM cycles (0: the kernels' default).
+uint64_t thread_wait_limit_cycles() { return wait_limit_cycles(); }
+
 // The current device's error word, which xt_device_error reads and clears.
 int device_error_word(uint32_t** out) {
   int device = 0;

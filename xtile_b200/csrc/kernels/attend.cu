@@ -554,11 +554,11 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   const uint32_t value_at[2] = {place<DP>(token_of_row<DP>(2 * t), DP == 64 ? g >> 1 : g) + (DP == 64 ? (g & 1) * 8 : 0),
                                 place<DP>(token_of_row<DP>(2 * t + 1), DP == 64 ? g >> 1 : g) + (DP == 64 ? (g & 1) * 8 : 0)};
   constexpr int kEight = 8 * kBox;  // eight rows on
-  const sm100::Abort ab{abort_flag, p.a.error_word, sm100::kWaitLimitCycles};
+  const sm100::Abort ab{abort_flag, p.a.error_word, sm100::wait_limit_or_default(p.a.wait_limit_cycles)};
   int stage = 0;
   uint32_t phase = 0;
   while (!kCluster || left > 0) {
-    if (!__all_sync(0xffffffffu, sm100::mbar_wait(&landed[stage], phase, ab, kErrUnitWait))) break;
+    if (!__all_sync(0xffffffffu, bounded_wait(&landed[stage], phase, ab, kErrUnitWait))) break;
     __syncwarp();  // every lane has read the stage before this one
     const float scales = scale[0];
 #pragma unroll
@@ -776,12 +776,32 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       ++at.tile;
     }
   }
-  // a wait gave up: what is under way lands before the memory goes
-  for (int i = 0; i < kStages - 1 && left - to_issue > i; ++i) {
-    sm100::mbar_wait_drain(&landed[stage], phase, 500000000ull);
-    if (++stage == kStages) {
-      stage = 0;
-      phase ^= 1;
+  if (left > 0) {
+    // a wait gave up: what is under way lands before the memory goes ...
+    for (int i = 0; i < kStages - 1 && left - to_issue > i; ++i) {
+      sm100::mbar_wait_drain(&landed[stage], phase, 500000000ull);
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    // ... and the rows of all units that were left are NaN
+    auto spoil = [&] {
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) sum[nr][0] = sum[nr][1] = __int_as_float(0x7fc00000);
+    };
+    spoil();
+    if constexpr (!kCluster) {
+      while (true) {
+        const int here = min(left, at.seg.hi - at.tile);
+        at.tile += here - 1;  // the last of them
+        left -= here;
+        finish_segment(at.tile + 1 == at.seg.hi);
+        if (left == 0) return;
+        at.advance(p);
+        whole = true;
+        spoil();
+      }
     }
   }
   if constexpr (kCluster) {

@@ -81,6 +81,24 @@ __device__ __forceinline__ float tanh_fast(float x) {
   return s < 0.0225f ? x * fmaf(s, fmaf(s, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f) : fmaf(-2.0f, r, 1.0f);
 }
 
+// mbar_wait for the attention kernels, whose waits are short: with a limit of the
+// caller's own (not the default) a poll does not suspend the warp and is followed
+// by a look at the clock, so that a wait of a microsecond can run out.  (One loop
+// for both took 129 us where 64 ragged contexts take 122.)
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, const sm100::Abort& ab, uint32_t code) {
+  if (ab.limit >= sm100::kWaitLimitCycles) return sm100::mbar_wait(bar, parity, ab, code);
+  const uint64_t t0 = clock64();
+  while (!sm100::mbar_test_wait(bar, parity)) {
+    if (*ab.flag) return false;
+    if (clock64() - t0 > ab.limit) {
+      *ab.flag = 1;
+      atomicCAS(ab.error_word, 0u, code);
+      return false;
+    }
+  }
+  return true;
+}
+
 constexpr int kMaxDevices = 64;
 
 // Grants ``kernel`` its shared memory, once a device.

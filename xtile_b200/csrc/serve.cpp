@@ -11,6 +11,7 @@
 namespace xt {
 int record_error(int code, const std::string& msg);  // capi.cpp
 int device_error_word(uint32_t** out);               // capi.cpp
+uint64_t thread_wait_limit_cycles();                 // capi.cpp
 }  // namespace xt
 
 namespace {
@@ -60,7 +61,8 @@ xt::dev::BatchView view(const xt_batch& b) {
 
 xt::dev::AttendArgs attend_args(const xt_cache_attention_args& a, uint32_t* error_word) {
   return {view(a.cache), view(a.batch), a.q, a.out, a.q_token, a.q_head, a.out_token, a.out_head, a.q_heads, a.max_new,
-          a.window, a.scale, a.softcap, code_of(a.elem), a.workspace, a.workspace_bytes, error_word};
+          a.window, a.scale, a.softcap, code_of(a.elem), a.workspace, a.workspace_bytes, error_word,
+          xt::thread_wait_limit_cycles()};
 }
 
 int check_attention(const char* who, const xt_cache_attention_args* a) {

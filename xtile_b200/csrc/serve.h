@@ -112,6 +112,7 @@ struct AttendArgs {
   void* workspace;
   size_t workspace_bytes;
   uint32_t* error_word;
+  uint64_t wait_limit_cycles;  // SM cycles a wait may take before the kernel gives up (0: 2 s)
 };
 // Bytes of device memory that launch_cache_attention needs beside its arguments.
 size_t attend_workspace_bytes(const AttendArgs& a);
