@@ -148,13 +148,14 @@ int xt_generated_source(const xt_module* module, const char* func, char** out_te
 int xt_compile_generated(const char* source, size_t* out_cubin_bytes);
 
 /* No counterpart in the reference.  Sets how long a pipeline wait (TMA data,
- * MMA completion, accumulator hand-off) of the gemm and conv kernels that the
- * calling thread launches later may take before the kernel gives up: it then
- * records a code in the error word (read with xt_device_error: 0x101-0x103
- * gemm, 0x201-0x203 conv), stops every role, lets issued copies and MMAs
- * land, frees its tensor memory and returns, leaving the context usable.
- * ``ns`` 0 restores the default (about 2 s); at most 60 s.  Every wait takes
- * at least a few tens of microseconds before it can give up, whatever the
+ * MMA completion, accumulator hand-off) of the gemm, conv and cache attention
+ * kernels that the calling thread launches later may take before the kernel
+ * gives up: it then records a code in the error word (read with
+ * xt_device_error: 0x101-0x103 gemm, 0x201-0x203 conv, 0x304-0x307 cache
+ * attention), stops every role, lets issued copies and MMAs land, frees its
+ * tensor memory and returns, leaving the context usable.  ``ns`` 0 restores the
+ * default (about 2 s); at most 60 s.  Every wait of the gemm and conv kernels
+ * takes at least a few tens of microseconds before it can give up, whatever the
  * limit.  Teardown drains keep their own limits.  Used to test the failure
  * path; production keeps the default. */
 int xt_set_wait_limit_ns(uint64_t ns);
@@ -202,7 +203,8 @@ int xt_matmul_launch_noalloc(const xt_module* module, const char* func, void* co
  * fall, append may miss other sequences too and every row of an attention is
  * NaN.  The attention
  * kernels' waits for their own copies and products are bounded like those of
- * xt_launch; one that runs out gives 0x304, 0x305 or 0x307. */
+ * xt_launch (xt_set_wait_limit_ns holds for them too); one that runs out gives
+ * 0x304, 0x305 or 0x307, and the rows that it kept from being whole are NaN. */
 
 /* y = h * rsqrt(mean(h^2) + eps) * weight with h = x + residual, row by row.
  * y_elem XT_ELEM_I8: y = rint(v / s) with the row's s = max|v| / 127 in

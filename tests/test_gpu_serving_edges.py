@@ -218,3 +218,33 @@ def test_attention_waits_run_out(case):
             break
     assert lost, "no wait ran out"
     assert torch.equal(xt.cache_attention(cache, q, *batch.args, max_new=max(new)), good)
+
+
+@pytest.mark.parametrize("limit_ns", [1, 1000, 3000])
+@pytest.mark.parametrize("new, total, dim, heads, group, window, softcap", [
+    ([700, 64, 900], [700, 300, 2500], 128, 2, 4, 0, 0.0),
+    ([700, 64, 900], [700, 300, 2500], 64, 2, 8, 130, 0.0),
+    ([1700], [1700], 96, 1, 10, 0, 20.0),
+    ([128], [1600], 128, 8, 4, 0, 0.0),  # clusters, as the two below
+    ([70, 3, 90], [4000, 70, 2500], 128, 8, 4, 1300, 0.0),
+    ([512], [1600], 64, 8, 8, 0, 20.0),
+])
+def test_attention_prompt_waits_run_out(new, total, dim, heads, group, window, softcap, limit_ns):
+    """The tcgen05 kernel's waits run out: every row is whole or NaN, the products that were issued land, the tensor
+    memory is freed, and the next call is whole again."""
+    batch = Batch(new, total, 64, seed=3)
+    cache = filled_cache(generator(5), batch.pages_held, heads, dim, 64, 16)
+    q = normal(generator(6), batch.tokens, heads * group, dim, std=1.5, dtype=torch.bfloat16)
+    attend = lambda out=None: xt.cache_attention(cache, q, *batch.args, out, window=window, softcap=softcap,  # noqa: E731
+                                                 max_new=max(new))
+    good = attend()
+    assert good.isfinite().all() and xt.device_error() == 0
+    for _ in range(3):
+        y = torch.zeros_like(q)
+        with xt.wait_limit(limit_ns):
+            attend(y)
+        lost = rows_good_or_nan(y, good)
+        code = xt.device_error()
+        assert code in ((0x304, 0x305) if lost else (0,))
+        assert lost or limit_ns > 1
+        assert torch.equal(attend(), good) and xt.device_error() == 0

@@ -108,7 +108,7 @@ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > h
 // SM budget of the persistent (gemm, conv) kernels launched by this thread.
 thread_local int t_sm_budget = 0;
 
-// Pipeline wait limit of the gemm and conv kernels launched by this thread,
+// Wait limit of the gemm, conv and cache attention kernels launched by this thread,
 // in nanoseconds (0: the kernels' default of about 2 s).  Kernels count SM
 // cycles; at the B200's 1.9-2.0 GHz SM clock a nanosecond is 2 cycles.
 thread_local uint64_t t_wait_limit_ns = 0;

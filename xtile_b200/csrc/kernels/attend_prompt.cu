@@ -106,20 +106,24 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 // Waits for a phase as mbar_wait does; a whole warp calls.  The limit is
-// looked at once in 256 polls, each of which the hardware may suspend.
+// looked at once in 256 polls, each of which the hardware may suspend; a limit of
+// the caller's own (not the default) with every poll, none of which it suspends.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const Abort& ab, uint32_t code) {
   const uint32_t at = smem_addr(bar);
+  const uint32_t own = ab.limit < kWaitLimitCycles;
   uint64_t t0 = 0;
   while (true) {
 #pragma unroll 1
-    for (int poll = 0; poll < 256; ++poll) {
+    for (int poll = own ? 255 : 0; poll < 256; ++poll) {
       uint32_t ok;
       asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 q, %3, 0;\n\t"
+          "@q mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "@!q mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
           "selp.u32 %0, 1, 0, p;\n\t}"
           : "=r"(ok)
-          : "r"(at), "r"(parity)
+          : "r"(at), "r"(parity), "r"(own)
           : "memory");
       if (__any_sync(0xffffffffu, ok)) return true;  // the phase is over for every lane, then
     }
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  const Abort ab{&bars.abort, p.a.error_word, kWaitLimitCycles};
+  const Abort ab{&bars.abort, p.a.error_word, wait_limit_or_default(p.a.wait_limit_cycles)};
   // TMEM columns: scores and weights of the two query tiles, then outputs
   auto score_at = [&](int w) { return tmem + w * 128; };
   auto out_at = [&](int w) { return tmem + 256 + w * 128; };
@@ -533,11 +537,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
       meet();  // the query tile stands in shared memory
       if (issuer && tiles > 0) ok = score(0);
       for (int j = 0; j < tiles; ++j) {
-        // A wait that gives up leaves the rest of the loop to run on whatever is
-        // there, without another long wait: the barriers below stay whole.
-        ok = wait_phase(&bars.s_full[w], j & 1, ab, kErrSoftmaxWait) && ok;
-        ok = wait_phase(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, ab, kErrSoftmaxWait) && ok;
+        // A warp whose wait gave up touches no more of the tensor memory and issues
+        // no more products; it still meets the others of its query tile.
+        ok = ok && wait_phase(&bars.s_full[w], j & 1, ab, kErrSoftmaxWait);
+        ok = ok && wait_phase(&bars.scales_full[j % kScaleSlots], (j / kScaleSlots) & 1, ab, kErrSoftmaxWait);
         tc_fence_after();
+        if (!ok) {
+          meet();
+          continue;
+        }
         key_scales = base + L::kScales + (j % kScaleSlots) * 2 * kTokens * 4;
         value_scales = key_scales + kTokens * 4;
         const float* most4 = bars.most[j % kScaleSlots];
@@ -554,14 +562,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         tmem_wait_st();
         meet();
         if (issuer) {
-          ok = output(j) && ok;
-          if (j + 1 < tiles) ok = score(j + 1) && ok;
+          ok = output(j);
+          if (ok && j + 1 < tiles) ok = score(j + 1);
         }
       }
 
       // --- the result: output over the sum
-      if (tiles > 0) ok = wait_phase(&bars.o_full[w], 0, ab, kErrSoftmaxWait) && ok;
+      if (tiles > 0) ok = ok && wait_phase(&bars.o_full[w], 0, ab, kErrSoftmaxWait);
+      if (issuer && !ok) {
+        // what was issued still ends before the memory goes
+        if (elect_sync()) umma_commit(&bars.drain[w]);
+        __syncwarp();
+        mbar_wait_drain(&bars.drain[w], 0, 500000000ull);
+      }
       tc_fence_after();
+      const bool there = ok && tiles > 0;  // the tensor memory holds the result
       float s0, s1;
       unpack2(sum, s0, s1);
       s0 += s1;
@@ -570,26 +585,27 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
 #pragma unroll 1
         for (int d = 0; d < DP; d += 32) {
           uint32_t r[32];
-          if (tiles > 0) {
+          if (there) {
             tmem_ld_32x32b_x32(result + d, r);
             tmem_wait_ld();
           }
 #pragma unroll
           for (int h = 0; h < 8; ++h)
             *reinterpret_cast<uint4*>(part_at(local, d / 4 + h)) =
-                tiles > 0 ? make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]) : make_uint4(0, 0, 0, 0);
+                there ? make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]) : make_uint4(0, 0, 0, 0);
         }
         // the weights carry 2^(up - ref); a wait that gave up leaves NaN
         *part_sum(local) = make_float2(ref - up, ok ? s0 : __int_as_float(0x7fc00000));
       } else {
         const float over = s0 > 0.0f || s0 != s0 ? 1.0f / s0 : 0.0f;
+        const uint32_t none = ok ? 0u : 0x7fc07fc0u;  // a wait that gave up leaves NaN
         // the row's values to the query tile's room (its last product is done), from
         // where DP / 8 lanes store each row
         uint8_t* room = smem + L::kQuery + w * L::kMatrix + (warp & 3) * 32 * DP * 2;
 #pragma unroll 1
         for (int d = 0; d < DP; d += 32) {
           uint32_t r[32];
-          if (tiles > 0) {
+          if (there) {
             tmem_ld_32x32b_x32(result + d, r);
             tmem_wait_ld();
           }
@@ -598,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
             uint32_t v[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              v[x] = tiles > 0 ? pack_bf16(__uint_as_float(r[8 * h + 2 * x]) * over, __uint_as_float(r[8 * h + 2 * x + 1]) * over) : 0;
+              v[x] = there ? pack_bf16(__uint_as_float(r[8 * h + 2 * x]) * over, __uint_as_float(r[8 * h + 2 * x + 1]) * over) : none;
             *reinterpret_cast<uint4*>(room + lane * DP * 2 + (((d / 8 + h) ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
@@ -608,18 +624,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
         for (int x = 0; x < kSteps; ++x) {
           const int at = x * kWarpRows + sub;
           const uint4 v = *reinterpret_cast<const uint4*>(room + at * DP * 2 + ((part ^ (at & 7)) << 4));
-          if (row.at < work.rows && part_there && ok)
+          if (row.at < work.rows && part_there)
             *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + offset(row, p.a.out_token, p.a.out_head)) = v;
           next_row(row);
         }
       }
       tc_fence_before();
-      if (issuer && *ab.flag) {
-        // what was issued still ends before the memory goes
-        if (elect_sync()) umma_commit(&bars.drain[w]);
-        __syncwarp();
-        mbar_wait_drain(&bars.drain[w], 0, 500000000ull);
-      }
     }
     if (p.cluster > 1) {
       cluster_sync();

@@ -166,7 +166,7 @@ def device_error() -> int:
 
 
 class wait_limit:
-    """Limits how long a pipeline wait of the gemm and conv kernels launched
+    """Limits how long a pipeline wait of the gemm, conv and cache attention kernels launched
     by this thread inside a ``with`` block may take, in nanoseconds, before
     the kernel gives up, records an error code (``device_error()``), drains
     and returns.  For testing the failure path; the default is about 2 s."""
