@@ -4,7 +4,8 @@
   planner and the sm_100a kernels (nvcc, -gencode arch=compute_100a,code=sm_100a);
 * ``_xtile*.so``     -- the Python extension (pybind11) over that library;
 * ``_serving*.so``   -- the serving operators on torch tensors, built against
-  torch's headers and loaded with torch at their first use.
+  torch's headers and loaded with torch at their first use (left out where
+  torch is not installed; nothing else needs it).
 
 Objects go to ``xtile_b200/_build``; a source is recompiled when it or any
 header it can include is newer than its object.
@@ -84,19 +85,19 @@ def _embed_op_math() -> None:
         inc.write_text(body)
 
 
-def _torch_dir() -> Path:
+def _torch_dir() -> Path | None:
+    """Where torch is installed, found without importing it; None where it is not."""
     import importlib.util
 
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
-        raise RuntimeError("the serving extension is built against torch, which is not installed")
+        return None
     return Path(spec.submodule_search_locations[0])
 
 
-def _build_serving(force: bool, deps: list[Path]) -> bool:
+def _build_serving(torch: Path, force: bool, deps: list[Path]) -> bool:
     """Compiles the serving extension's object; True if it is newer than the extension."""
     src, obj = CSRC / "serving_module.cpp", BUILD / "serving_module.o"
-    torch = _torch_dir()
     if force or _stale(obj, src, [d for d in deps if d.parent == ROOT / "include"]):
         inc = torch / "include"
         _run(["g++", "-O2", "-fPIC", "-std=c++20", f"-I{sysconfig.get_paths()['include']}", f"-I{inc}",
@@ -110,10 +111,10 @@ def build(force: bool = False, verbose: bool = False) -> None:
     deps = _headers()
     lib_srcs = [p for p in sorted(CSRC.rglob("*.cpp")) if p.name not in ("xt_module.cpp", "serving_module.cpp")]
     lib_srcs += sorted(CSRC.rglob("*.cu"))
+    torch = _torch_dir()
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as pool:
-        serving = pool.submit(_build_serving, force, deps)
+        serving = pool.submit(_build_serving, torch, force, deps) if torch else None
         objs = list(pool.map(lambda s: _compile(s, force, deps), lib_srcs))
-        link_serving = serving.result()
     if force or not LIB.exists() or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs):
         _run([NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objs), "-lcudart_static", "-ldl",
               "-lrt", "-lpthread"])
@@ -135,8 +136,11 @@ def build(force: bool = False, verbose: bool = False) -> None:
               "-Wl,-rpath,$ORIGIN"])
         if verbose:
             print("linked", EXT)
-    if force or link_serving or LIB.stat().st_mtime > SERVING_EXT.stat().st_mtime:
-        lib = _torch_dir() / "lib"
+    if serving is None:
+        if verbose:
+            print("torch is not installed:", SERVING_EXT.name, "is left out")
+    elif serving.result() or LIB.stat().st_mtime > SERVING_EXT.stat().st_mtime or force:
+        lib = torch / "lib"
         _run(["g++", "-shared", "-o", str(SERVING_EXT), str(BUILD / "serving_module.o"), f"-L{PKG}", "-lxt_b200",
               f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN",
               f"-Wl,-rpath,{lib}"])
