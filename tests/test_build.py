@@ -42,3 +42,22 @@ def test_the_library_and_the_extension_build_without_torch(built, monkeypatch):
     outputs.clear()
     module.build()
     assert outputs == []
+
+
+def test_the_serving_extension_follows_torch(built, monkeypatch, tmp_path):
+    module, outputs = built
+    torch = tmp_path / "torch"
+    torch.mkdir()
+    (torch / "version.py").write_text("__version__ = '1'\n")
+    monkeypatch.setattr(module, "_torch_dir", lambda: torch)
+    module.build()
+    assert {"serving_module.o", module.SERVING_EXT.name} <= set(outputs)
+    outputs.clear()
+    module.build()
+    assert outputs == []
+    (torch / "version.py").write_text("__version__ = '2'\n")  # another torch in its place
+    module.build()
+    assert outputs == ["serving_module.o", module.SERVING_EXT.name]
+    outputs.clear()
+    module.build()
+    assert outputs == []

@@ -8,7 +8,8 @@
   torch is not installed; nothing else needs it).
 
 Objects go to ``xtile_b200/_build``; a source is recompiled when it or any
-header it can include is newer than its object.
+header it can include is newer than its object (the serving extension's also
+when another torch is installed).
 
     python xtile_b200/build.py [--force]
 """
@@ -98,10 +99,15 @@ def _torch_dir() -> Path | None:
 def _build_serving(torch: Path, force: bool, deps: list[Path]) -> bool:
     """Compiles the serving extension's object; True if it is newer than the extension."""
     src, obj = CSRC / "serving_module.cpp", BUILD / "serving_module.o"
-    if force or _stale(obj, src, [d for d in deps if d.parent == ROOT / "include"]):
+    # torch's headers count by its version and place: an installed file may be older than the object
+    version, built_with = torch / "version.py", BUILD / "serving_torch.txt"
+    against = f"{torch}\n{version.read_text() if version.exists() else ''}"
+    other = not built_with.exists() or built_with.read_text() != against
+    if force or other or _stale(obj, src, [d for d in deps if d.parent == ROOT / "include"]):
         inc = torch / "include"
         _run(["g++", "-O2", "-fPIC", "-std=c++20", f"-I{sysconfig.get_paths()['include']}", f"-I{inc}",
               f"-I{inc / 'torch/csrc/api/include'}", f"-I{CUDA / 'include'}", "-c", str(src), "-o", str(obj)])
+        built_with.write_text(against)
     return not SERVING_EXT.exists() or obj.stat().st_mtime > SERVING_EXT.stat().st_mtime
 
 
