@@ -248,3 +248,20 @@ def test_attention_prompt_waits_run_out(new, total, dim, heads, group, window, s
         assert code in ((0x304, 0x305) if lost else (0,))
         assert lost or limit_ns > 1
         assert torch.equal(attend(), good) and xt.device_error() == 0
+
+
+# --------------------------------------------------------------- sizes at edges
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("new", [[1, 1], [40, 30], [700, 900]])
+def test_attention_of_an_empty_page_table(new, dtype):
+    """No page at all and so no token: every row is 0."""
+    cache = filled_cache(generator(1), 3, 2, 64, 16, 16)
+    q = normal(generator(2), sum(new), 16, 64, dtype=dtype)
+    pages = torch.empty(2, 0, dtype=torch.int32, device="cuda")
+    y = torch.full_like(q, 7)
+    xt.cache_attention(cache, q, ints(starts_of(new)), ints([0, 0]), pages, y, max_new=max(new))
+    assert (y == 0).all()
+    xt.cache_attention(cache, q, ints(starts_of(new)), ints([0, 5]), pages, y, max_new=max(new))
+    assert xt.device_error() == 0x303
+    assert (y[:new[0]] == 0).all() and y[new[0]:].isnan().all()

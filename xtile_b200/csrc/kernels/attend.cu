@@ -1133,6 +1133,7 @@ bool for_prompt(AttendDev& p) {
   if (p.a.elem != kBF16 || p.a.cache.dim > 128 || !vectors || rows <= 16) return false;
   const bool small = p.a.cache.dim <= 64;
   const int64_t longest = longest_seen(p, 128), tiles = (longest + 127) / 128, segments = segments_of(p, 256);
+  if (tiles == 0) return false;  // no page at all
   const float tile_us = small ? (rows <= 128 ? 2.2f : 2.8f) : rows <= 128 ? 2.7f : 3.4f;
   float best = 0.0f;
   for (int cluster = 1; cluster <= 8 && cluster <= tiles; cluster *= 2) {
