@@ -265,3 +265,14 @@ def test_attention_of_an_empty_page_table(new, dtype):
     xt.cache_attention(cache, q, ints(starts_of(new)), ints([0, 5]), pages, y, max_new=max(new))
     assert xt.device_error() == 0x303
     assert (y[:new[0]] == 0).all() and y[new[0]:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_of_the_widest_window(dtype):
+    """The largest window there is hides nothing, also behind queries that see no token."""
+    batch = Batch([900, 300], [400, 1500], 64, seed=3)
+    cache = filled_cache(generator(1), batch.pages_held, 2, 64, 64, 16)
+    q = normal(generator(2), batch.tokens, 16, 64, dtype=dtype)
+    want = xt.cache_attention(cache, q, *batch.args, max_new=900)
+    for window in (1 << 30, (1 << 31) - 1):
+        assert torch.equal(xt.cache_attention(cache, q, *batch.args, max_new=900, window=window), want)

@@ -220,8 +220,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
     const int before = work.seq.length - work.seq.count;
     const int pos_first = before + p.group_div.quot(work.row0);
     const int pos_last = before + p.group_div.quot(work.row0 + work.rows - 1);
-    const int seen_from = p.a.window > 0 ? pos_first - p.a.window + 1 : 0;
-    work.lo = seen_from > 0 ? seen_from / kTokens : 0;
+    // 64 bits: with more new tokens than tokens the first position is negative
+    const int64_t seen_from = p.a.window > 0 ? static_cast<int64_t>(pos_first) - p.a.window + 1 : 0;
+    work.lo = seen_from > 0 ? static_cast<int>(seen_from) / kTokens : 0;
     work.hi = pos_last < 0 ? work.lo : max(pos_last / kTokens + 1, work.lo);
     // a cluster's CTAs share them out (and returned together above)
     const int all_tiles = work.hi - work.lo, first = all_tiles * rank / p.cluster;
