@@ -209,7 +209,7 @@ int xt_matmul_launch_noalloc(const xt_module* module, const char* func, void* co
 /* y = h * rsqrt(mean(h^2) + eps) * weight with h = x + residual, row by row.
  * y_elem XT_ELEM_I8: y = rint(v / s) with the row's s = max|v| / 127 in
  * scales (v: the normed row; s is 0 for rows under 1e-36, NaN for rows with
- * NaN).  Sums are f32; the norm is of h before it is rounded into sum. */
+ * NaN or infinities).  Sums are f32; the norm is of h before it is rounded into sum. */
 typedef struct xt_rms_norm_args {
   const void* x;         /* [rows, cols], elem */
   const void* residual;  /* like x, or NULL */
@@ -268,7 +268,7 @@ typedef struct xt_batch {
  * by xt_rope at their positions if ``rope`` is given.  A block's scale becomes
  * the larger of what it was (if it holds earlier tokens of the sequence) and
  * max|x| / 127 over its new tokens; where it rises, the earlier tokens' rows
- * are rounded anew.  A NaN makes its block's scale NaN.  Blocks of one call
+ * are rounded anew.  A NaN or an infinity makes its block's scale NaN.  Blocks of one call
  * must not be shared by two sequences. */
 typedef struct xt_cache_append_args {
   xt_cache cache;

@@ -276,3 +276,25 @@ def test_attention_of_the_widest_window(dtype):
     want = xt.cache_attention(cache, q, *batch.args, max_new=900)
     for window in (1 << 30, (1 << 31) - 1):
         assert torch.equal(xt.cache_attention(cache, q, *batch.args, max_new=900, window=window), want)
+
+
+@pytest.mark.parametrize("block", [1, 16])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinities_do_not_come_back_as_values(block, sign):
+    """int8 data that cannot hold an infinity says so: its scale is NaN, like that of a NaN."""
+    batch = Batch([3], [20], 16, seed=1)
+    cache = filled_cache(generator(1), batch.pages_held, 2, 64, 16, block)
+    before = cache.k_scale.clone()
+    k = normal(generator(2), 3, 2, 64)
+    v = k.clone()
+    k[1, 0, 5] = sign * float("inf")
+    xt.cache_append(cache, k, v, *batch.args)
+    into, row = batch.table[0][1], 18 % 16
+    assert cache.k_scale[into, 0, row // block].isnan()
+    assert cache.k_scale[into, 1].isfinite().all() and cache.v_scale.isfinite().all()
+    assert torch.equal(cache.k_scale[batch.table[0][0]], before[batch.table[0][0]])
+    y = xt.cache_attention(cache, k.nan_to_num(posinf=1, neginf=1), *batch.args)
+    assert y[1:, 0].isnan().all() and y[:, 1].isfinite().all()
+    x, w = torch.ones(2, 64, device="cuda"), torch.ones(64, device="cuda")
+    w[3] = sign * float("inf")
+    assert xt.rms_norm(x, w, dtype=torch.int8)[1].isnan().all()

@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 
 namespace xt {
@@ -92,16 +93,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // int8 scale of values whose largest magnitude is ``top``: top / 127, and 0
 // (all values round to 0) for a top under 1e-36, whose reciprocal would leave
-// f32's range.  A NaN top gives a NaN scale, so that whoever reads the values
-// back sees it.
+// f32's range.  A top that is NaN or infinite gives a NaN scale, so that whoever
+// reads the values back sees it (of an infinite one the bytes have no sign).
 constexpr float kQuantTiny = 1e-36f;
-__device__ __forceinline__ float quant_scale(float top) { return top < kQuantTiny ? 0.0f : top * (1.0f / 127.0f); }
+__device__ __forceinline__ float quant_scale(float top) {
+  return top < kQuantTiny ? 0.0f : top < INFINITY ? top * (1.0f / 127.0f) : __int_as_float(0x7fc00000);
+}
 __device__ __forceinline__ float quant_inverse(float scale) { return scale > 0.0f ? 1.0f / scale : 0.0f; }
 
 // x * inverse rounded to the nearest whole number (ties to even) in the low
 // byte of a float's bits: 1.5 * 2^23 leaves no bits behind the point.  For
-// |x * inverse| < 2^22, so for any value under its block's scale; NaN gives
-// some byte (its scale is NaN).
+// |x * inverse| < 2^22, so for any value under its block's scale; NaN and
+// infinities give some byte (their scale is NaN).
 __device__ __forceinline__ uint32_t quantize_bits(float x, float inverse) {
   return __float_as_uint(__fmaf_rn(x, inverse, 12582912.0f));
 }
