@@ -298,3 +298,41 @@ def test_infinities_do_not_come_back_as_values(block, sign):
     x, w = torch.ones(2, 64, device="cuda"), torch.ones(64, device="cuda")
     w[3] = sign * float("inf")
     assert xt.rms_norm(x, w, dtype=torch.int8)[1].isnan().all()
+
+
+# ------------------------------------------------------------ torch's own rules
+
+def test_written_tensors_have_a_new_version():
+    """Autograd finds a tensor that was saved and then written by its version, as after torch's own in-place calls."""
+    g = generator(3)
+    x, w = normal(g, 4, 128, dtype=torch.bfloat16), normal(g, 128)
+    r, total, y = x.clone(), torch.empty_like(x), torch.empty_like(x)
+    q8, s = torch.empty(4, 128, dtype=torch.int8, device="cuda"), torch.empty(4, device="cuda")
+    heads, pos, table = x.view(4, 2, 64), ints([0, 1, 2, 3]), xt.RopeTable.build(8, 64)
+    batch = Batch([4], [4], 16, seed=1)
+    cache = filled_cache(g, batch.pages_held, 2, 64, 16, 16)
+    turned, seen, back = torch.empty_like(heads), torch.empty_like(heads), torch.empty_like(cache.k, dtype=torch.float32)
+    calls = [
+        (lambda: xt.rms_norm(x, w, y, residual=r, residual_out=total), [y, total], [x, w, r]),
+        (lambda: xt.rms_norm(x, w, q8, scales=s), [q8, s], [x, w]),
+        (lambda: xt.rope(heads, pos, table, turned), [turned], [heads, pos, table.cos_sin]),
+        (lambda: xt.cache_append(cache, heads, heads, *batch.args, rope=table),
+         [cache.k, cache.v, cache.k_scale, cache.v_scale], [heads, *batch.args]),
+        (lambda: xt.cache_attention(cache, heads, *batch.args, seen), [seen], [heads, cache.k, cache.v_scale]),
+        (lambda: xt.dequantize(cache.k, cache.k_scale, back), [back], [cache.k, cache.k_scale]),
+    ]
+    for i, (call, written, read) in enumerate(calls):
+        before = [t._version for t in written], [t._version for t in read]
+        call()
+        assert all(t._version > v for t, v in zip(written, before[0])), i
+        assert all(t._version == v for t, v in zip(read, before[1])), i
+    with torch.inference_mode():
+        held = torch.empty_like(heads)
+    xt.rope(heads, pos, table, held)  # has no version
+    assert torch.equal(held, turned)
+    leaf = x.float().requires_grad_()
+    square = (leaf * 1).square_()
+    saved = square * square
+    xt.rms_norm(square.detach(), w, square.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.sum().backward()

@@ -99,6 +99,11 @@ void written(const at::Tensor& t, const char* name) {
       raise(PyExc_ValueError, std::string(name) + " is written and must not be broadcast");
 }
 
+// Tells autograd that a tensor has changed (an inference tensor has no version).
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 std::optional<at::ScalarType> dtype_of(PyObject* o) {
   if (o == Py_None) return std::nullopt;
   if (!THPDtype_Check(o)) raise(PyExc_TypeError, std::string("dtype must be a torch dtype, got ") + Py_TYPE(o)->tp_name);
@@ -247,6 +252,9 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
                              y_elem,
                              static_cast<float>(number(args[6]))};
     check(xt_rms_norm(&a, launch.handle()), "rms_norm");
+    changed(*out);
+    if (sum) changed(*sum);
+    if (scales) changed(*scales);
     PyObject* y = wrap_or(args[2], *out);
     if (y_elem != XT_ELEM_I8) return y;
     PyObject* s = wrap_or(args[5], *scales);
@@ -306,6 +314,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
                          table.size(0), x.stride(0), x.stride(1), out->stride(0), out->stride(1), elem,
                          elem_of(out->scalar_type()), PyObject_IsTrue(args[3]), PyObject_IsTrue(args[5])};
     check(xt_rope(&a, launch.handle()), "rope");
+    changed(*out);
     return wrap_or(args[4], *out);
   });
 }
@@ -384,6 +393,7 @@ PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                  table ? 2 * table->size(1) : 0, table ? table->size(0) : 0, elem,
                                  PyObject_IsTrue(args[10])};
     check(xt_cache_append(&a, launch.handle()), "cache_append");
+    for (int i = 0; i < 4; ++i) changed(THPVariable_Unpack(args[i]));
     return none();
   });
 }
@@ -421,6 +431,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       a.workspace = scratch.data_ptr();
     }
     check(xt_cache_attention(&a, launch.handle()), "cache_attention");
+    changed(*out);
     return wrap_or(args[8], *out);
   });
 }
@@ -459,6 +470,7 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
       check(xt_dequantize(static_cast<const int8_t*>(q.data_ptr()), static_cast<const float*>(scales.data_ptr()),
                           out->data_ptr(), count, count / runs, elem, launch.handle()),
             "dequantize");
+    changed(*out);
     return wrap_or(args[2], *out);
   });
 }

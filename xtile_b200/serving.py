@@ -18,6 +18,10 @@ With ``stream`` given, that stream owns what the call allocates, as under
 result, and calls ``record_stream`` on a result that is dropped while its own
 reads are under way.  The same holds for the call's inputs on ``stream``.
 
+The calls are outside autograd: results carry no gradient, whatever the inputs
+require, and a tensor that is written gets a new version, so that a backward
+pass that saved it finds out.
+
 A ragged batch is described by three int32 tensors: ``starts`` [seqs + 1],
 ``lengths`` [seqs] and ``pages`` [seqs, width].  Sequence ``b`` has
 ``lengths[b]`` tokens; the last ``starts[b + 1] - starts[b]`` of them are new
