@@ -336,3 +336,12 @@ def test_written_tensors_have_a_new_version():
     xt.rms_norm(square.detach(), w, square.detach())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         saved.sum().backward()
+
+
+def test_a_flag_without_a_truth_value_is_refused():
+    x, pos, table = torch.ones(4, 2, 64, device="cuda"), ints([0, 1, 2, 3]), xt.RopeTable.build(8, 64)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        xt.rope(x, pos, table, inverse=torch.ones(2))
+    table.interleaved = torch.ones(2)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        xt.rope(x, pos, table)

@@ -126,6 +126,12 @@ int small(PyObject* o, const char* name) {
   return static_cast<int>(v);
 }
 
+int truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PyFailure();
+  return v;
+}
+
 // The stream a call runs on: torch's current one of the device, or the given
 // torch stream or raw handle.  Holds the device current for the call.
 struct Launch {
@@ -312,7 +318,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const xt_rope_args a{x.data_ptr(), out->data_ptr(), static_cast<const int32_t*>(positions.data_ptr()),
                          static_cast<const float*>(table.data_ptr()), x.size(0), x.size(1), x.size(2), rot,
                          table.size(0), x.stride(0), x.stride(1), out->stride(0), out->stride(1), elem,
-                         elem_of(out->scalar_type()), PyObject_IsTrue(args[3]), PyObject_IsTrue(args[5])};
+                         elem_of(out->scalar_type()), truth(args[3]), truth(args[5])};
     check(xt_rope(&a, launch.handle()), "rope");
     changed(*out);
     return wrap_or(args[4], *out);
@@ -391,7 +397,7 @@ PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const xt_cache_append_args a{cache, batch, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                  table ? static_cast<const float*>(table->data_ptr()) : nullptr,
                                  table ? 2 * table->size(1) : 0, table ? table->size(0) : 0, elem,
-                                 PyObject_IsTrue(args[10])};
+                                 truth(args[10])};
     check(xt_cache_append(&a, launch.handle()), "cache_append");
     for (int i = 0; i < 4; ++i) changed(THPVariable_Unpack(args[i]));
     return none();
