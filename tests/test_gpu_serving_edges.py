@@ -1,6 +1,10 @@
 """The serving operators where a call meets the rest of a program: streams and
 their memory, wrong tables, waits that run out, and values at the edges of
 their types.  Tolerances are those of ``test_gpu_serving``."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -345,3 +349,36 @@ def test_a_flag_without_a_truth_value_is_refused():
     table.interleaved = torch.ones(2)
     with pytest.raises(RuntimeError, match="ambiguous"):
         xt.rope(x, pos, table)
+
+
+FIRST_IN_A_GRAPH = """
+import torch, xtile as xt
+x = torch.randn(600, 512, device="cuda").bfloat16(); w = torch.ones(512, device="cuda")
+heads = x.view(600, 8, 64); kv = heads[:, :2]
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+args = ints([0, 600]), ints([600]), torch.arange(4096, dtype=torch.int32, device="cuda").view(1, -1) % 10
+one = ints([0, 1]), args[1], args[2]
+pos = torch.arange(600, dtype=torch.int32, device="cuda")
+table, cache = xt.RopeTable.build(600, 64), xt.KVCache.empty(10, 2, 64)
+def calls():
+    xt.cache_append(cache, kv, kv, *args, rope=table)
+    q8, s = xt.rms_norm(x, w, dtype=torch.int8)
+    q = xt.rope(xt.dequantize(q8, s).view(600, 8, 64), pos, table)
+    return (xt.cache_attention(cache, q, *args, max_new=600), xt.cache_attention(cache, q[-1:], *one, max_new=1),
+            xt.cache_attention(cache, q[-1:], one[0], one[1], args[2][:, :10], max_new=1))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, calls())) and xt.device_error() == 0
+print("whole")
+"""
+
+
+def test_the_first_calls_may_be_captured():
+    """A process whose first calls are captured in a graph: nothing that they set up breaks the capture."""
+    run = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0 and "whole" in run.stdout, run.stderr[-2000:]

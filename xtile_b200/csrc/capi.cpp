@@ -80,11 +80,23 @@ cudaError_t workspace(int device, Workspace** out) {
   std::lock_guard<std::mutex> lock(g_ws_mu);
   auto it = g_ws.find(device);
   if (it == g_ws.end()) {
+    // The first call may be one that is being captured in a graph: what it sets up
+    // is not part of that, and goes over a stream of its own, done before any launch.
     Workspace w;
-    cudaError_t e = cudaMalloc(&w.error_word, 256);
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) return e;
-    e = cudaMemset(w.error_word, 0, 256);
-    if (e != cudaSuccess) return e;
+    cudaStream_t stream = nullptr;
+    e = cudaMalloc(&w.error_word, 256);
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(w.error_word, 0, 256, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (stream) cudaStreamDestroy(stream);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
+      cudaFree(w.error_word);
+      return e;
+    }
     it = g_ws.emplace(device, w).first;
   }
   *out = &it->second;
