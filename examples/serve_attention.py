@@ -149,6 +149,12 @@ class Server:
         return [t.transpose(1, 2).reshape(-1, cache.heads, cache.dim)[:length] for t in (keys, values)]
 
 
+def raise_for_device_error() -> None:
+    code = xt.device_error()  # which clears it
+    if code:
+        raise RuntimeError(f"a kernel reported {code:#x}")
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--layers", type=int, default=2)
@@ -171,8 +177,7 @@ def main() -> None:
         last = server.decode(last)
     events[3].record()
     torch.cuda.synchronize()
-    if xt.device_error():
-        raise RuntimeError(f"a kernel reported {xt.device_error():#x}")
+    raise_for_device_error()
     print(f"{sum(a.prompts)} prompt tokens: {events[0].elapsed_time(events[1]):.3f} ms")
     if a.steps > 1:
         print(f"{len(a.prompts)} tokens a step: {events[2].elapsed_time(events[3]) / (a.steps - 1) * 1e3:.1f} us")

@@ -166,3 +166,16 @@ def test_python_calls_refuse_cpu_tensors_and_wrong_types():
         xt.dequantize(x, w)
     with pytest.raises(ValueError, match="CUDA"):
         xt.dequantize(x.to(torch.int8), w)
+
+
+def test_the_example_names_the_device_error(monkeypatch):
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("serve_attention", Path(__file__).resolve().parents[1] / "examples" / "serve_attention.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    codes = [0x303, 0]  # read and cleared
+    monkeypatch.setattr(example.xt, "device_error", lambda: codes.pop(0))
+    with pytest.raises(RuntimeError, match="0x303"):
+        example.raise_for_device_error()
+    example.raise_for_device_error()
