@@ -382,3 +382,25 @@ def test_the_first_calls_may_be_captured():
     run = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], capture_output=True, text=True, timeout=300,
                          cwd=Path(__file__).resolve().parents[1])
     assert run.returncode == 0 and "whole" in run.stdout, run.stderr[-2000:]
+
+
+# ------------------------------------------------------------- what bits are held
+
+@pytest.mark.parametrize("new, total", [([1], [300]), ([400], [700])])
+def test_small_elements_of_a_bf16_query(new, total):
+    """A row's elements of 2^-20 to 2^-40 of its largest, before keys that are 0 where that one is: what they score is
+    off by half a step of the f16 that they enter as, 2^-35 of the row's largest each."""
+    batch = Batch(new, total, 64, seed=3)
+    cache = filled_cache(generator(1), batch.pages_held, 2, 128, 64, 16)
+    cache.k[..., 0] = 0
+    q = normal(generator(2), batch.tokens, 16, 128, dtype=torch.float32)
+    q *= 2.0 ** -torch.randint(20, 41, q.shape, generator=generator(3), device="cuda").float()
+    q[..., 0] = 1.0
+    q = q.bfloat16()
+    scale = 2.0 ** 20
+    y = xt.cache_attention(cache, q, *batch.args, scale=scale, max_new=max(new))
+    want, *rest = attend_64(cache, batch, q, scale, 0, 0.0)
+    keys = cache.k.float().view(-1, 2, 4, 16, 128) * cache.k_scale[..., None, None]
+    off = scale * 2.0 ** -35 * keys.abs().sum(-1).max().item()  # of a score, in the exponent of a weight and of the sum
+    assert 2 ** -10 < off < 2 ** -4  # far over the rounding of the scores' sums
+    within(y, want, allowed(want, *rest, max(total), q.dtype) + 2.2 * off * rest[0])

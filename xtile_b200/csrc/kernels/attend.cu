@@ -27,14 +27,18 @@
 // Tokens (and the output's dims) are the products' m, query rows their n: the
 // converted cache bytes are A operands that all of a segment's rows share, and
 // a group of up to 8 heads fills one n8 tile.  What a unit costs is mostly the
-// conversion of its bytes (three instructions for four key bytes, six for four
-// value bytes), not the products.
+// conversion of its bytes (five instructions for four key bytes, six for four
+// value bytes), not the products.  Keys that entered as the f16 subnormals (byte +
+// 128) 2^-24 would take three (64 ragged contexts 122.3 us, 125.7 so), but the
+// sums would be rounded at the size of what the 128s add, which is not small
+// where a query's large elements meet keys near 0.
 //
 // int8 values are exact in f16, and so is a bf16 query divided by a power of
-// two that brings its row's largest magnitude near 2^10 (elements under 2^-35
-// of that lose bits).  The scales of the tokens' blocks stay outside the
-// products: the key's multiplies the score in f32, the value's the weight,
-// which is rounded once to f16 (11 bits) on its way into the second product.
+// two that brings its row's largest magnitude near 2^10: elements under 2^-27 of
+// that lose bits, those under 2^-35 are gone, all at most 2^-35 of it off.  The
+// scales of the tokens' blocks stay outside the products: the key's multiplies
+// the score in f32, the value's the weight, which is rounded once to f16 (11
+// bits) on its way into the second product.
 // f32 queries go in as two f16 terms, and so do their weights: 22 bits.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -423,8 +427,8 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
   float o[kOut][NR][4];
   // rows 2 t and 2 t + 1 of each n8 tile: reference of the exponents, sum of
   // the weights, factor of the score in the exponent (1 behind a cap, whose own
-  // factor is capped_scale), the score's start, position of the query
-  float ref[NR][2], sum[NR][2], row_scale[NR][2], capped_scale[NR][2], start[NR][2];
+  // factor is capped_scale), position of the query
+  float ref[NR][2], sum[NR][2], row_scale[NR][2], capped_scale[NR][2];
   int row_pos[NR][2];
   int pos_min = 0, pos_max = 0;
   int value_exp = 0;                     // the weights carry vs 2^(10 - value_exp); set by the first token seen
@@ -473,7 +477,6 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       // the row times 2^(10 - exponent of its largest magnitude), and the scale's sign
       const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 243);
       const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23 | (negative ? 0x80000000u : 0u));
-      float total_q = 0.0f;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
@@ -483,26 +486,15 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
           query[(nr * kSteps + s) * 32 + lane] = f;  // read back by this lane alone
         else
           qf[nr][s] = f;
-        if constexpr (F32) {
+        if constexpr (F32)
           query[((NR + nr) * kSteps + s) * 32 + lane] =
               make_uint2(rest_half2(q[s][0], q[s][1], f.x), rest_half2(q[s][2], q[s][3], f.y));
-        } else {
-          const float2 a = unpack_half2(f.x), b = unpack_half2(f.y);
-          total_q += (a.x + a.y) + (b.x + b.y);
-        }
       }
-      total_q += __shfl_xor_sync(0xffffffffu, total_q, 1);
-      total_q += __shfl_xor_sync(0xffffffffu, total_q, 2);
-      // The keys' bytes enter as f16 subnormals (byte + 128) 2^-24: the score
-      // starts at what the 128s will add.  In f32 they enter as themselves.
-      const float down = __uint_as_float(static_cast<uint32_t>(e - 10) << 23) * (F32 ? 1.0f : 16777216.0f) *
-                         fabsf(p.a.scale) * (cap > 0.0f ? 1.0f / cap : kLog2e);
-      const float offset = F32 ? 0.0f : total_q * (-128.0f / 16777216.0f);
+      const float down = __uint_as_float(static_cast<uint32_t>(e - 10) << 23) * fabsf(p.a.scale) * (cap > 0.0f ? 1.0f / cap : kLog2e);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         capped_scale[nr][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
         row_scale[nr][c] = cap > 0.0f ? 1.0f : capped_scale[nr][c];
-        start[nr][c] = __shfl_sync(0xffffffffu, offset, (2 * t + c) * 4);
         row_pos[nr][c] = before + static_cast<int>(p.group_div.quot(at.row_tile * kRows + 8 * nr + 2 * t + c));
         ref[nr][c] = kNone;
         sum[nr][c] = 0.0f;
@@ -572,7 +564,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[nr][e] = start[nr][e & 1];
+      for (int e = 0; e < 4; ++e) z[nr][e] = 0.0f;
 #pragma unroll
     for (int j = 0; j < DP / 64; ++j) {
       uint32_t u[4], w[4];
@@ -583,14 +575,8 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       for (int s = 0; s < 4; ++s) {
         const uint32_t x = u[s] ^ 0x80808080u, y = w[s] ^ 0x80808080u;
         const int step = 4 * j + s;
-        uint32_t a0, a1, a2, a3;
-        if constexpr (F32) {
-          a0 = bytes_to_half2<kLow>(x), a2 = bytes_to_half2<kHigh>(x);
-          a1 = bytes_to_half2<kLow>(y), a3 = bytes_to_half2<kHigh>(y);
-        } else {
-          a0 = __byte_perm(x, 0, kLow), a2 = __byte_perm(x, 0, kHigh);
-          a1 = __byte_perm(y, 0, kLow), a3 = __byte_perm(y, 0, kHigh);
-        }
+        const uint32_t a0 = bytes_to_half2<kLow>(x), a2 = bytes_to_half2<kHigh>(x);
+        const uint32_t a1 = bytes_to_half2<kLow>(y), a3 = bytes_to_half2<kHigh>(y);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
           if constexpr (S::kQueryInSmem) {
