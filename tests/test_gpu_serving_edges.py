@@ -404,3 +404,17 @@ def test_small_elements_of_a_bf16_query(new, total):
     off = scale * 2.0 ** -35 * keys.abs().sum(-1).max().item()  # of a score, in the exponent of a weight and of the sum
     assert 2 ** -10 < off < 2 ** -4  # far over the rounding of the scores' sums
     within(y, want, allowed(want, *rest, max(total), q.dtype) + 2.2 * off * rest[0])
+
+
+@pytest.mark.parametrize("new, total", [([1], [300]), ([400], [700])])
+def test_the_largest_bf16_queries(new, total):
+    """Queries up to the end of their range, whose scores a small scale brings back."""
+    batch = Batch(new, total, 64, seed=3)
+    cache = filled_cache(generator(1), batch.pages_held, 2, 128, 64, 16)
+    q = normal(generator(2), batch.tokens, 16, 128, dtype=torch.float32)
+    q = (q * 2.0 ** torch.arange(110, 126, device="cuda").float()[:, None]).bfloat16()  # sizes head by head
+    assert q.isfinite().all() and q.abs().max() > 1e38
+    for scale in (2.0 ** -126, 2.0 ** -110):
+        y = xt.cache_attention(cache, q, *batch.args, scale=scale, max_new=max(new))
+        want, *rest = attend_64(cache, batch, q, scale, 0, 0.0)
+        within(y, want, allowed(want, *rest, max(total), q.dtype))

@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // the row times 2^(10 - exponent of its largest magnitude), and the scale's sign
-      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 243);
+      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 254);
       const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23 | (negative ? 0x80000000u : 0u));
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_prompt(const __grid_consta
           for (int y = 0; y < 4; ++y) top = max3(top, fabsf(bf16_lo(v[y])), fabsf(bf16_hi(v[y])));
 #pragma unroll
           for (int o = kRowLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 243);
+          const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 11), 254);
           const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23 | (p.a.scale < 0.0f ? 0x80000000u : 0u));
           const float down = __uint_as_float(static_cast<uint32_t>(e - 10) << 23) * fabsf(p.a.scale) *
                              (CAP ? 1.0f / cap : kLog2e);
