@@ -195,16 +195,15 @@ int xt_matmul_launch_noalloc(const xt_module* module, const char* func, void* co
  * positions, an int8 paged cache with its attention, and int8 data read back.
  * Arrays are device memory of XT_ELEM_* types; a row's (head's) elements are
  * contiguous and strides are in elements.  Every call checks its arguments on
- * the host, is asynchronous on ``stream``, and reads and writes each array
- * once.  What only the device knows (positions, lengths, page tables) is
- * checked there: an entry that names something outside the arrays is not
- * followed, its results are NaN (append: not stored), and xt_device_error gives
- * 0x301 (rope position), 0x302 (append) or 0x303 (attention).  Where ``starts``
- * fall, append may miss other sequences too and every row of an attention is
- * NaN.  The attention
- * kernels' waits for their own copies and products are bounded like those of
- * xt_launch (xt_set_wait_limit_ns holds for them too); one that runs out gives
- * 0x304, 0x305 or 0x307, and the rows that it kept from being whole are NaN. */
+ * the host and is asynchronous on ``stream``.  What only the device knows
+ * (positions, lengths, page tables) is checked there: an entry that names
+ * something outside the arrays is not followed, its results are NaN (append: not
+ * stored), and xt_device_error gives 0x301 (rope position), 0x302 (append) or
+ * 0x303 (attention).  Where ``starts`` fall, append may miss other sequences too
+ * and every row of an attention is NaN.  The attention kernels' waits for
+ * their own copies and products are bounded like those of xt_launch
+ * (xt_set_wait_limit_ns holds for them too); one that runs out gives 0x304, 0x305
+ * or 0x307, and the rows that it kept from being whole are NaN. */
 
 /* y = h * rsqrt(mean(h^2) + eps) * weight with h = x + residual, row by row.
  * y_elem XT_ELEM_I8: y = rint(v / s) with the row's s = max|v| / 127 in
@@ -268,8 +267,8 @@ typedef struct xt_batch {
  * by xt_rope at their positions if ``rope`` is given.  A block's scale becomes
  * the larger of what it was (if it holds earlier tokens of the sequence) and
  * max|x| / 127 over its new tokens; where it rises, the earlier tokens' rows
- * are rounded anew.  A NaN or an infinity makes its block's scale NaN.  Blocks of one call
- * must not be shared by two sequences. */
+ * are rounded anew.  A NaN or an infinity makes its block's scale NaN.  Blocks
+ * of one call must not be shared by two sequences. */
 typedef struct xt_cache_append_args {
   xt_cache cache;
   xt_batch batch;

@@ -418,3 +418,36 @@ def test_the_largest_bf16_queries(new, total):
         y = xt.cache_attention(cache, q, *batch.args, scale=scale, max_new=max(new))
         want, *rest = attend_64(cache, batch, q, scale, 0, 0.0)
         within(y, want, allowed(want, *rest, max(total), q.dtype))
+
+
+# ------------------------------------------------------------------ int8 chains
+
+@xt.kernel
+def int8_product(rows, w, by_column, out, tm, tn, tk):
+    i, j = xt.bid(0), xt.bid(1)
+    p = xt.matmul(xt.load(rows, index=(i, 0), shape=(tm, tk)), xt.load(w, index=(0, j), shape=(tk, tn), shared=1))
+    xt.store(out, index=(i, j), tile=p * xt.load(by_column, index=(0, j), shape=(1, tn)))
+
+
+@xt.kernel
+def rows_scaled(p, by_row, out, tm, tn):
+    i, j = xt.bid(0), xt.bid(1)
+    xt.store(out, index=(i, j), tile=xt.load(p, index=(i, j), shape=(tm, tn)) * xt.load(by_row, index=(i, 0), shape=(tm, 1)))
+
+
+def test_int8_rows_through_an_int8_product():
+    """``rms_norm``'s int8 rows times int8 weights: the matmul program scales the columns, a program behind it the rows."""
+    m, k, n = 256, 512, 384
+    g = generator(9)
+    x, w = normal(g, m, k, dtype=torch.bfloat16), normal(g, k)
+    q8, s = xt.rms_norm(x, w, dtype=torch.int8)
+    w8 = torch.randint(-127, 128, (k, n), generator=g, device="cuda", dtype=torch.int8)
+    columns = torch.rand(1, n, generator=g, device="cuda")
+    product, y = torch.empty(m, n, device="cuda"), torch.empty(m, n, device="cuda")
+    A = xt.Array
+    xt.launch(xt.convert(int8_product, args=(A((m, k), xt.int8), A((k, n), xt.int8), A((1, n), xt.float32), A((m, n), xt.float32),
+                                             128, 128, k), grid=(m // 128, n // 128, 1)), q8, w8, columns, product)
+    xt.launch(xt.convert(rows_scaled, args=(A((m, n), xt.float32), A((m, 1), xt.float32), A((m, n), xt.float32), 8, n),
+                         grid=(m // 8, 1, 1)), product, s.view(m, 1), y)
+    want = (q8.double() @ w8.double()) * columns.double() * s.double()[:, None]
+    within(y, want, 3 * 2.0 ** -24 * want.abs())  # whole numbers under 2^24, times two scales

@@ -21,8 +21,9 @@
 // calls give each segment to a cluster instead, whose warps split its tokens
 // and join in shared memory.
 //
-// 64 sequences of up to 8192 tokens, 32 query heads over 8 of 128: 122 us, 5520
-// GB/s of their 674 MB; one sequence of 777 tokens 7.1 us.
+// 64 sequences of up to 8192 tokens, 32 query heads over 8 of 128: 124 us, 5420
+// GB/s of their 674 MB (graph replay; 126 to 141 as calls among others, by GPU);
+// one sequence of 777 tokens 7.5 us.
 //
 // Tokens (and the output's dims) are the products' m, query rows their n: the
 // converted cache bytes are A operands that all of a segment's rows share, and

@@ -2,8 +2,10 @@
 // bound by the tensor cores, where attend.cu's split by tokens is bound by the
 // conversion of the cache's bytes.  The mathematics and the roundings are the
 // same (attend.cu).  Two chunks of 2048 new tokens behind 2048, 32 query heads
-// over 8 of 128: 256 us, 538 TFLOP/s; the softmax of a tile takes 4000 cycles
-// beside products of 1700.
+// over 8 of 128: 259 us, 532 TFLOP/s.  A query tile's token tile takes 4000 to
+// 4500 cycles of its SM, as if the two query tiles' softmaxes ran one after the
+// other, and about 1050 of products: the tensor pipe is busy 26% of the time, the
+// issue slots 47%; warps wait for their loads from TMEM and shared memory.
 //
 // One CTA has 256 packed query rows (new token, head of the group) of one kv
 // head, as two tiles of 128, and walks over the cache in tiles of 128 tokens:

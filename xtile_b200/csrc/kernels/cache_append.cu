@@ -4,14 +4,17 @@
 //   s' = max(s, max|x| / 127)   (s: the block's scale, if it has earlier tokens)
 //   q  = rint(x / s');  the earlier tokens' rows become rint(q s / s') if s' > s.
 //
-// Each new element is read once and one byte of it written, but what bounds a
-// prompt is instructions: about 20 an element pair for the rotation, the
-// largest magnitude and the rounding.  So a unit (one block of one head, of the
+// Each new element is read once (the rest of a block that a CTA's registers do not
+// hold, twice) and one byte of it written.  What bounds a prompt is the latency
+// of its loads: issue slots are 49% busy and DRAM 29%, and of 7 cycles between
+// a warp's issues 2.8 go to global loads, which two CTAs an SM do not cover.  So a unit (one block of one head, of the
 // keys or of the values) belongs to as few lanes as hold it in registers
 // between the largest magnitude and the rounding, and what finds the block's
 // place is done once a warp: 17.1k tokens of 8 heads of 128 bf16
-// take 36.7 us (2860 GB/s), and took 73 with a CTA of four warps a unit; 64
-// single tokens take 3.6 us.
+// take 36.0 us (2920 GB/s), and took 73 with a CTA of four warps a unit.  64
+// single tokens take 3.7 us where cache and tokens are in L2, 4.8 where they are
+// not, and 7.5 where besides every block's scale rises, so that its earlier
+// tokens' rows are read and rounded anew.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -7,7 +7,8 @@
 // Bound by HBM: each element is read once and written once.  A row's h stays
 // in registers between the sum of squares, the largest magnitude and the
 // stores.  Sums are f32.  8192 rows of 4096 bf16 with a residual to int8 take
-// 38.9 us, 6040 GB/s of their 235 MB; 8 such rows 2.4 us.
+// 39.8 us, 5910 GB/s of their 235 MB; 8 such rows 2.5 us; 8192 rows of 4095, off
+// the vector boundary and so with each weight loaded alone, 70 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -10,8 +10,9 @@ raises ``TypeError`` (types) or ``ValueError`` (shapes, devices, layouts)
 before anything runs.  Positions, lengths and page tables live on the device:
 an entry outside the arrays is not followed, and ``device_error()`` reports it
 (0x301 rope, 0x302 append, 0x303 attention; where ``starts`` fall, append may
-miss other sequences too, and every row of an attention is NaN; 0x304, 0x305 and 0x307 are bounded
-waits of the attention kernels that ran out).
+miss other sequences too, and every row of an attention is NaN; 0x304, 0x305 and
+0x307 are bounded waits of the attention kernels that ran out, whose rows are
+NaN).
 
 With ``stream`` given, that stream owns what the call allocates, as under
 ``torch.cuda.stream(stream)``: another stream waits for it before it reads the
@@ -58,7 +59,10 @@ def rms_norm(x, weight, out=None, *, residual=None, residual_out=None, scales=No
     receives h, and may be ``residual`` or ``x``) are like it; ``weight`` [cols]
     is f32 or bf16.  ``out`` is f32, bf16 or int8 (``dtype`` chooses where it is
     left out; default x's).  Int8 rows carry one f32 scale each in ``scales``
-    [rows]: ``int8 = rint(value / scale)``, ``scale = max|value| / 127``.
+    [rows]: ``int8 = rint(value / scale)``, ``scale = max|value| / 127`` (NaN for a
+    row with a NaN or an infinity).  A matmul program takes such rows as they are,
+    and a program behind it multiplies the product's rows by ``scales``: its own
+    epilogue scales columns only.
     Returns ``out``, for int8 rows ``(out, scales)``.
     """
     return (_native or _load()).rms_norm(x, weight, out, residual, residual_out, scales, eps, dtype, stream)
@@ -156,7 +160,8 @@ def cache_append(cache: KVCache, k, v, starts, lengths, pages, *, rope: RopeTabl
     ``k`` and ``v`` [tokens, heads, dim] are f32 or bf16; ``lengths`` already
     counts the new tokens.  A block's scale becomes the larger of its old one (if
     it holds earlier tokens) and ``max|x| / 127`` of its new tokens; where it
-    rises, the rows of the earlier tokens are rounded anew to it.
+    rises, the rows of the earlier tokens are rounded anew to it.  A NaN or an
+    infinity makes its block's scale NaN.
     """
     if not isinstance(cache, KVCache):
         _no_cache(cache)
@@ -176,7 +181,9 @@ def cache_attention(cache: KVCache, q, starts, lengths, pages, out=None, *, max_
     ``q`` [tokens, q_heads, dim] is f32 or bf16, ``out`` like it; consecutive
     ``q_heads / heads`` query heads share a cache head.  A query sees its
     sequence's tokens up to its own (the last ``window`` of them if window > 0); one
-    that sees none gives 0.  ``scale`` defaults to ``dim ** -0.5``; ``softcap`` > 0
+    that sees none gives 0, and a row of no sequence stays as it is.  Heads start
+    on four elements' bytes; prompts of bf16 queries whose heads start on 16 bytes
+    can run on the tensor cores' own kernel.  ``scale`` defaults to ``dim ** -0.5``; ``softcap`` > 0
     caps the scaled scores by ``softcap * tanh(score / softcap)``.  ``max_new``, the
     most new tokens of one sequence, helps to choose the kernel; it changes
     nothing that is computed, only the order of sums and so their last bits.
@@ -192,6 +199,7 @@ def dequantize(q, scales, out=None, *, dtype=None, stream=None):
 
     ``rms_norm``'s rows and their scales, or a cache's ``k`` and ``k_scale`` (whose
     blocks are contiguous): the run is ``q.numel() / scales.numel()`` elements.
+    All are contiguous, and ``q`` and ``out`` start on 16 bytes.
     ``out`` is f32 or bf16 (``dtype`` chooses where it is left out; default bf16).
     """
     return (_native or _load()).dequantize(q, scales, out, dtype, stream)
