@@ -179,3 +179,11 @@ def test_the_example_names_the_device_error(monkeypatch):
     with pytest.raises(RuntimeError, match="0x303"):
         example.raise_for_device_error()
     example.raise_for_device_error()
+
+
+def test_cache_attention_refuses_an_infinite_cap():
+    base = parts({})
+    args = Attend(**base, q=AT, out=AT, q_token=128, q_head=64, out_token=128, out_head=64, q_heads=2, scale=0.125,
+                  elem=BF16, softcap=float("inf"))  # its tanh is 0 and the product of both NaN
+    assert LIB.xt_cache_attention(ctypes.byref(args), None) == ARGUMENT
+    assert "softcap" in LIB.xt_last_error().decode()

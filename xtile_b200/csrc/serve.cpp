@@ -73,7 +73,8 @@ int check_attention(const char* who, const xt_cache_attention_args* a) {
   if (a->q_heads < 1 || a->q_heads % a->cache.heads != 0) return bad(who, "q_heads must be a multiple of the cache's heads");
   if (static_cast<int64_t>(a->batch.tokens) * a->q_heads > kMaxInt - 256) return bad(who, "too many query rows");
   if (a->window < 0 || a->max_new < 0) return bad(who, "negative window or max_new");
-  if (!(a->softcap >= 0.0f)) return bad(who, "softcap must be 0 or positive");
+  if (!(a->softcap >= 0.0f && a->softcap <= std::numeric_limits<float>::max()))
+    return bad(who, "softcap must be 0 or positive, and finite");
   return XT_OK;
 }
 
