@@ -254,6 +254,18 @@ def test_attention_prompt_waits_run_out(new, total, dim, heads, group, window, s
         assert torch.equal(attend(), good) and xt.device_error() == 0
 
 
+def test_attention_prompt_waits_have_their_codes():
+    """At once the softmax warps give up; with 2000 cycles, which the scores take less than and a stage's way through
+    softmax and products more, the converting ones do."""
+    batch = Batch([700, 64, 900], [700, 300, 2500], 64, seed=3)
+    cache = filled_cache(generator(5), batch.pages_held, 2, 128, 64, 16)
+    q = normal(generator(6), batch.tokens, 8, 128, std=1.5, dtype=torch.bfloat16)
+    for limit_ns, code in ((1, 0x304), (1000, 0x305)):
+        with xt.wait_limit(limit_ns):
+            xt.cache_attention(cache, q, *batch.args, max_new=900)
+        assert xt.device_error() == code
+
+
 # --------------------------------------------------------------- sizes at edges
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
