@@ -432,6 +432,20 @@ def test_the_largest_bf16_queries(new, total):
         within(y, want, allowed(want, *rest, max(total), q.dtype))
 
 
+@pytest.mark.parametrize("new, total", [([1] * 4, [307, 250, 120, 77]), ([1, 1], [3000, 2000]), ([5, 40], [900, 700])])
+@pytest.mark.parametrize("dim, heads, group", [(256, 4, 1), (256, 2, 8), (128, 4, 4), (80, 2, 16)])
+def test_f32_attention_holds_its_bits(new, total, dim, heads, group):
+    """The 2-norm of the error, of scores of about 1.  Root mean squares of what a weight is off by: exp2 2^-22.7, the
+    query's and the weight's two f16 terms 2^-23 each, four partial scores of eight sums, each rounded toward zero by
+    2^-24 of half a score, 2^-21.9; together 3.5e-7, and a mean of values is off by as much.  Twice that is allowed."""
+    batch = Batch(new, total, 64, seed=3)
+    cache = filled_cache(generator(1), batch.pages_held, heads, dim, 64, 16, 0.015, 0.035)
+    q = normal(generator(2), batch.tokens, heads * group, dim)
+    want = attend_64(cache, batch, q, dim ** -0.5, 0, 0.0)[0]
+    y = xt.cache_attention(cache, q, *batch.args, max_new=max(new))
+    assert (y.double() - want).norm() <= 7e-7 * want.norm()
+
+
 # ------------------------------------------------------------------ int8 chains
 
 @xt.kernel

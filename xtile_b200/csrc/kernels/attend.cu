@@ -569,6 +569,7 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
 #pragma unroll
     for (int j = 0; j < DP / 64; ++j) {
       uint32_t u[4], w[4];
+      float part[NR][4] = {};  // f32: a fresh sum for 64 dims, added in f32, as the tensor cores' own sums round toward zero
       const uint32_t from = keys + (key_at ^ ((j & 1) << 6)) + (j >> 1) * kTile * 128;
       lds128(u, from);
       lds128(w, from + kEight);
@@ -580,13 +581,21 @@ __global__ void __launch_bounds__(Shape<DP, F32, NR>::kWarps * 32, Shape<DP, F32
         const uint32_t a1 = bytes_to_half2<kLow>(y), a3 = bytes_to_half2<kHigh>(y);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
-          if constexpr (S::kQueryInSmem) {
+          if constexpr (F32) {
+            mma_16816(part[nr], a0, a1, a2, a3, query[((NR + nr) * kSteps + step) * 32 + lane]);
+            mma_16816(part[nr], a0, a1, a2, a3, query[(nr * kSteps + step) * 32 + lane]);
+          } else if constexpr (S::kQueryInSmem) {
             mma_16816(z[nr], a0, a1, a2, a3, query[(nr * kSteps + step) * 32 + lane]);
-            if constexpr (F32) mma_16816(z[nr], a0, a1, a2, a3, query[((NR + nr) * kSteps + step) * 32 + lane]);
           } else {
             mma_16816(z[nr], a0, a1, a2, a3, qf[nr][step]);
           }
         }
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[nr][e] += part[nr][e];
       }
     }
 
